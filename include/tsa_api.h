@@ -43,6 +43,13 @@
  *   tsa_sample_tokens_ws    the same, with a workspace that lets a small
  *                           batch spread each row over several workgroups
  *   tsa_sample_tokens_workspace_bytes  its size
+ *   tsa_store_kv_quantized, tsa_load_kv_quantized  no counterpart: the store
+ *                           (kv_cache.py:122-191) into an 8-bit cache, and back
+ *   tsa_paged_decode_window  no counterpart: paged_attention_forward over part
+ *                           of the context, or over an 8-bit cache
+ *   tsa_paged_tree          no counterpart: the same for drafted tokens' trees
+ *   tsa_varlen_prefill_window  no counterpart: flash_attn_varlen_func with a
+ *                           sliding window and first tokens
  */
 #ifndef TSA_API_H
 #define TSA_API_H
@@ -69,6 +76,8 @@ enum tsa_dtype {
   TSA_F32 = 2,
   TSA_I32 = 3,
   TSA_I64 = 4,
+  TSA_E4M3 = 5, /* 8-bit caches: OCP e4m3 (no infinities, largest 448) */
+  TSA_I8 = 6,   /* 8-bit caches: two's complement, used from -127 to 127 */
 };
 
 /* A strided view of caller-owned device memory: element (i0, i1, ...) sits at
@@ -272,6 +281,73 @@ size_t tsa_sample_tokens_workspace_bytes(int64_t batch, int64_t vocab);
 int tsa_sample_tokens_ws(const tsa_view* out, const tsa_view* logits, const tsa_view* temperature,
                          const tsa_view* top_k, const tsa_view* top_p, const tsa_view* uniforms,
                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* An 8-bit paged cache. k_cache/v_cache (NB, Hkv, BS, D) hold codes, of dtype
+ * TSA_E4M3 or TSA_I8; k_scale/v_scale (NB, Hkv, BS) f32 a scale per row: a
+ * row's values are code * scale. The store takes k_src/v_src (Hkv, T, D)
+ * (bf16, f16 or f32) with tsa_store_kv_paged's addressing: scale = max|x| /
+ * 448 (e4m3) or 127 (int8), code = x / scale, both quotients rounded to f32
+ * and the code once more to its type, ties to even. A row of zeros has scale
+ * 0; a row holding a NaN or an infinity has scale NaN (and reads back as
+ * NaN). Tokens whose page is past the table or outside the pool are skipped.
+ * Each slot may be given once per call. */
+int tsa_store_kv_quantized(const tsa_view* k_src, const tsa_view* v_src, const tsa_view* k_cache,
+                           const tsa_view* v_cache, const tsa_view* k_scale, const tsa_view* v_scale,
+                           const tsa_view* block_tables, const tsa_view* cu_seqlens,
+                           const tsa_view* positions, void* stream);
+
+/* The inverse: k_out/v_out (T, Hkv, D) (bf16, f16 or f32) take code * scale of
+ * each token's row, in f32, rounded to their type; a token that no sequence holds, or whose
+ * page is past the table or outside the pool, reads as 0. */
+int tsa_load_kv_quantized(const tsa_view* k_out, const tsa_view* v_out, const tsa_view* k_cache,
+                          const tsa_view* v_cache, const tsa_view* k_scale, const tsa_view* v_scale,
+                          const tsa_view* block_tables, const tsa_view* cu_seqlens,
+                          const tsa_view* positions, void* stream);
+
+/* Bytes of workspace tsa_paged_decode_window (max_nodes 1) and tsa_paged_tree
+ * (window and sinks 0) need: the partial results of a (sequence, kv head)'s
+ * splits; 0 where nothing is split. */
+size_t tsa_paged_rows_workspace_bytes(int64_t num_seqs, int64_t max_nodes, int64_t num_heads,
+                                      int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks_per_seq,
+                                      int64_t block_size, int64_t window, int64_t sinks);
+
+/* tsa_paged_decode over part of the context: query s, at position
+ * seq_lens[s] - 1, sees the last `window` tokens (its own included; 0: all of
+ * them) and the first `sinks`. The caches are of query's dtype (k_scale and
+ * v_scale NULL) or 8-bit ones with their scales. Tokens that are not seen have
+ * no influence, whatever their rows hold; a token whose page id is outside the
+ * pool is not seen; lengths are taken within [0, the table's capacity]. A query
+ * that sees nothing (length 0) gives 0. The workspace (256-byte aligned) needs
+ * no initialisation; calls that share one must be ordered on one stream. */
+int tsa_paged_decode_window(const tsa_view* out, const tsa_view* query, const tsa_view* k_cache,
+                            const tsa_view* v_cache, const tsa_view* k_scale, const tsa_view* v_scale,
+                            const tsa_view* block_tables, const tsa_view* seq_lens, int64_t window,
+                            int64_t sinks, double softmax_scale, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* Attention of trees of drafted tokens. Sequence s's nodes are rows
+ * cu_nodes[s] .. cu_nodes[s + 1] of query/out (N, Hq, D), cu_nodes (B + 1)
+ * int32 non-decreasing; node i's keys and values are in the cache at position
+ * context_lens[s] + i. Node i sees the first context_lens[s] tokens and the
+ * nodes j whose bit is set in its row of tree_mask (N, words) int64: bit j %
+ * 64 of word j / 64 (a node sees itself only by its own bit). At most
+ * max_nodes rows a sequence are computed, and no more than the mask has bits;
+ * rows past those, and rows outside every sequence, are left as they were. A
+ * node that sees nothing gives 0. Page ids, lengths and the workspace as
+ * tsa_paged_decode_window's. */
+int tsa_paged_tree(const tsa_view* out, const tsa_view* query, const tsa_view* k_cache,
+                   const tsa_view* v_cache, const tsa_view* block_tables, const tsa_view* context_lens,
+                   const tsa_view* cu_nodes, const tsa_view* tree_mask, int64_t max_nodes,
+                   double softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* tsa_varlen_prefill, causal, over part of the keys: query i of a sequence
+ * sees the keys j <= i with j > i - window (window >= 1) or j < sinks. Keys
+ * that are not seen have no influence, whatever their rows hold; a query that
+ * sees none (its window past the last key, no first keys) gives 0. */
+int tsa_varlen_prefill_window(const tsa_view* out, const tsa_view* q, const tsa_view* k,
+                              const tsa_view* v, const tsa_view* cu_seqlens_q,
+                              const tsa_view* cu_seqlens_k, int64_t max_seqlen_q, int64_t max_seqlen_k,
+                              int64_t window, int64_t sinks, double softmax_scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -19,13 +19,15 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "libtsa.so"
 
 TSA_OK, TSA_ERR_INVALID, TSA_ERR_UNSUPPORTED, TSA_ERR_LAUNCH = 0, -1, -2, -3
-TSA_BF16, TSA_F16, TSA_F32, TSA_I32, TSA_I64 = 0, 1, 2, 3, 4
+TSA_BF16, TSA_F16, TSA_F32, TSA_I32, TSA_I64, TSA_E4M3, TSA_I8 = 0, 1, 2, 3, 4, 5, 6
 _DTYPES = {
     torch.bfloat16: TSA_BF16,
     torch.float16: TSA_F16,
     torch.float32: TSA_F32,
     torch.int32: TSA_I32,
     torch.int64: TSA_I64,
+    torch.float8_e4m3fn: TSA_E4M3,
+    torch.int8: TSA_I8,
 }
 
 
@@ -74,6 +76,15 @@ SIGNATURES = {
     "tsa_sample_tokens": (c_int, [_V, _V, _V, _V, _V, _V, c_void_p]),
     "tsa_sample_tokens_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "tsa_sample_tokens_ws": (c_int, [_V, _V, _V, _V, _V, _V, c_void_p, c_size_t, c_void_p]),
+    "tsa_store_kv_quantized": (c_int, [_V] * 9 + [c_void_p]),
+    "tsa_load_kv_quantized": (c_int, [_V] * 9 + [c_void_p]),
+    "tsa_paged_rows_workspace_bytes": (c_size_t, [c_int64] * 9),
+    "tsa_paged_decode_window": (
+        c_int,
+        [_V] * 8 + [c_int64, c_int64, c_double, c_void_p, c_size_t, c_void_p],
+    ),
+    "tsa_paged_tree": (c_int, [_V] * 8 + [c_int64, c_double, c_void_p, c_size_t, c_void_p]),
+    "tsa_varlen_prefill_window": (c_int, [_V] * 6 + [c_int64, c_int64, c_int64, c_int64, c_double, c_void_p]),
 }
 
 ABI_VERSION = 1
@@ -115,7 +126,7 @@ def host():
         except ImportError as e:
             raise RuntimeError("tinyserver_amd/_tsa_host.so is missing or does not load: build it first "
                                "(python -m tinyserver_amd._build or __graft_entry__.build())") from e
-        _entry.update({name: i for i, name in enumerate(_tsa_host.entries())})
+        _entry.update({name: i for i, name in enumerate((*_tsa_host.entries(), *_tsa_host.extra_entries()))})
         _host = _tsa_host
     return _host
 
@@ -164,6 +175,17 @@ def check(rc: int, what: str) -> None:
     if rc == TSA_ERR_UNSUPPORTED:
         raise NotImplementedError(f"{what}: {msg}")
     raise RuntimeError(f"{what}: {msg} (status {rc})")
+
+
+def launch(name: str, what: str, device: torch.device, *args) -> None:
+    """Call entry point ``name`` with ``args`` and the stream (torch's current one on ``device``), with ``device`` as
+    the current device: a kernel launched on a default stream goes to the current device, whosever its tensors are."""
+    if torch.cuda.current_device() == device.index:
+        rc = call(name, *args, stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            rc = call(name, *args, stream_of(device))
+    check(rc, what)
 
 
 _DEVICES: dict[int, torch.device] = {}

@@ -17,14 +17,20 @@
 
 namespace {
 
-enum Entry { kDecode, kDecodeStep, kNormRope, kNormRopeStore, kPrefill, kMixed, kSample, kSampleWs };
+enum Entry { kDecode, kDecodeStep, kNormRope, kNormRopeStore, kPrefill, kMixed, kSample, kSampleWs,
+             kStoreQuant, kLoadQuant, kDecodeWindow, kTree, kPrefillWindow };
 struct Shape { const char* name; int views, doubles, ints; };
 constexpr Shape kShapes[] = {
     {"tsa_paged_decode", 6, 1, 4},      {"tsa_paged_decode_step", 12, 2, 4}, {"tsa_qk_norm_rope", 8, 1, 1},
     {"tsa_qk_norm_rope_store", 14, 1, 1}, {"tsa_varlen_prefill", 6, 1, 4},   {"tsa_mixed_attention", 11, 2, 6},
     {"tsa_sample_tokens", 6, 0, 1},     {"tsa_sample_tokens_ws", 6, 0, 3},
+    {"tsa_store_kv_quantized", 9, 0, 1}, {"tsa_load_kv_quantized", 9, 0, 1}, {"tsa_paged_decode_window", 8, 1, 5},
+    {"tsa_paged_tree", 8, 1, 4},        {"tsa_varlen_prefill_window", 6, 1, 5},
 };
 constexpr int kEntries = sizeof(kShapes) / sizeof(kShapes[0]);
+// entries() lists the reference's path, the entry points before this one;
+// extra_entries() the others.
+constexpr int kExtra = kStoreQuant;
 constexpr int kMaxViews = 16, kMaxDoubles = 4, kMaxInts = 8;
 
 // A tensor's view, as _lib.view describes it. False with a Python error set
@@ -41,6 +47,8 @@ bool make_view(const at::Tensor& t, tsa_view& v) {
     case at::kFloat: v.dtype = TSA_F32; break;
     case at::kInt: v.dtype = TSA_I32; break;
     case at::kLong: v.dtype = TSA_I64; break;
+    case at::kFloat8_e4m3fn: v.dtype = TSA_E4M3; break;
+    case at::kChar: v.dtype = TSA_I8; break;
     default:
       PyErr_Format(PyExc_ValueError, "unsupported dtype %s", c10::toString(t.scalar_type()));
       return false;
@@ -76,6 +84,18 @@ int run(int e, const tsa_view* const* v, const double* d, const int64_t* i) {
                                  p(1), static_cast<size_t>(i[2]), i32(3), i32(4), p(5));
     case kSample:
       return tsa_sample_tokens(v[0], v[1], v[2], v[3], v[4], v[5], p(0));
+    case kStoreQuant:
+      return tsa_store_kv_quantized(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], p(0));
+    case kLoadQuant:
+      return tsa_load_kv_quantized(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], p(0));
+    case kDecodeWindow:
+      return tsa_paged_decode_window(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], i[0], i[1], d[0], p(2),
+                                     static_cast<size_t>(i[3]), p(4));
+    case kTree:
+      return tsa_paged_tree(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], i[0], d[0], p(1),
+                            static_cast<size_t>(i[2]), p(3));
+    case kPrefillWindow:
+      return tsa_varlen_prefill_window(v[0], v[1], v[2], v[3], v[4], v[5], i[0], i[1], i[2], i[3], d[0], p(4));
     default:
       return tsa_sample_tokens_ws(v[0], v[1], v[2], v[3], v[4], v[5], p(0), static_cast<size_t>(i[1]), p(2));
   }
@@ -145,17 +165,20 @@ PyObject* device_index(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// The entry points call() knows, in order.
-PyObject* entries(PyObject*, PyObject*) {
-  PyObject* t = PyTuple_New(kEntries);
-  for (int e = 0; t && e < kEntries; ++e) PyTuple_SET_ITEM(t, e, PyUnicode_FromString(kShapes[e].name));
+// The entry points call() knows, in order: entries(), then extra_entries().
+PyObject* names(int from, int to) {
+  PyObject* t = PyTuple_New(to - from);
+  for (int e = from; t && e < to; ++e) PyTuple_SET_ITEM(t, e - from, PyUnicode_FromString(kShapes[e].name));
   return t;
 }
+PyObject* entries(PyObject*, PyObject*) { return names(0, kExtra); }
+PyObject* extra_entries(PyObject*, PyObject*) { return names(kExtra, kEntries); }
 
 PyMethodDef kMethods[] = {
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call)), METH_FASTCALL, nullptr},
     {"device_index", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(device_index)), METH_FASTCALL, nullptr},
     {"entries", entries, METH_NOARGS, nullptr},
+    {"extra_entries", extra_entries, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tsa_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,164 @@
+// The 8-bit paged K/V cache (cache8.h): rows quantised as they are stored, and
+// read back.
+//
+// tsa_store_kv_quantized writes what tsa_store_kv_paged writes
+// (server/model/kernels/kv_cache.py:6-70 with qwen3.py:296-318's addressing),
+// in 8 bits; tsa_load_kv_quantized is its inverse. Both are copies with a row
+// maximum or a product between: bound by HBM for prompts, by the chain of
+// sequence search, block-table entry and row for a decode step's few tokens.
+#include "cache8.h"
+#include "kv_store.h"
+
+namespace tsa {
+
+struct Quant8Args {
+  const char* k_src; const char* v_src;  // store: (T, H, D) rows; load: not used
+  char* k_out; char* v_out;              // load: (T, H, D) rows
+  char* kc; char* vc;                    // codes (NB, H, BS, D)
+  float* ks; float* vs;                  // scales (NB, H, BS)
+  int64_t T, H, D, NB, BS;
+  int64_t kr_t, kr_h, kr_d, vr_t, vr_h, vr_d;  // element strides of the packed rows
+  int64_t kc_b, kc_h, kc_s, kc_d, vc_b, vc_h, vc_s, vc_d;
+  int64_t ks_b, ks_h, ks_s, vs_b, vs_h, vs_s;
+};
+
+// Any strides and head_dim: one wave per (token, kv head, K or V) row.
+template <typename T, typename C, bool STORE>
+__global__ __launch_bounds__(256) void quant8_rows(Quant8Args a, PagedAddr addr) {
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = 2 * a.T * a.H, waves = static_cast<int64_t>(gridDim.x) * 4;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6); r < rows; r += waves) {
+    const bool is_v = r & 1;
+    const int64_t t = (r >> 1) / a.H, h = (r >> 1) - t * a.H;
+    int64_t blk, slot;
+    const bool ok = addr.locate(t, a.BS, a.NB, blk, slot);
+    const int64_t row = is_v ? t * a.vr_t + h * a.vr_h : t * a.kr_t + h * a.kr_h, rd = is_v ? a.vr_d : a.kr_d;
+    C* const code = reinterpret_cast<C*>(is_v ? a.vc : a.kc) +
+                    (ok ? (is_v ? blk * a.vc_b + h * a.vc_h + slot * a.vc_s : blk * a.kc_b + h * a.kc_h + slot * a.kc_s)
+                        : 0);
+    const int64_t cd = is_v ? a.vc_d : a.kc_d;
+    float* const scale_p = (is_v ? a.vs : a.ks) +
+                           (ok ? (is_v ? blk * a.vs_b + h * a.vs_h + slot * a.vs_s
+                                       : blk * a.ks_b + h * a.ks_h + slot * a.ks_s)
+                               : 0);
+    if constexpr (STORE) {
+      if (!ok) continue;
+      const T* const src = reinterpret_cast<const T*>(is_v ? a.v_src : a.k_src) + row;
+      uint32_t top = 0;
+      for (int64_t d = lane; d < a.D; d += 64)
+        top = max(top, __builtin_bit_cast(uint32_t, to_float(src[d * rd])) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
+      const float scale = scale8<C>(top);
+      for (int64_t d = lane; d < a.D; d += 64)
+        code[d * cd] = __builtin_bit_cast(C, static_cast<uint8_t>(codes4<C>(quotient8<C>(to_float(src[d * rd]), scale), 0.f, 0.f, 0.f)));
+      if (lane == 0) *scale_p = scale;
+    } else {
+      T* const dst = reinterpret_cast<T*>(is_v ? a.v_out : a.k_out) + row;
+      const float scale = ok ? *scale_p : 0.f;
+      for (int64_t d = lane; d < a.D; d += 64)
+        dst[d * rd] = from_float<T>(ok ? product8(to_float(code[d * cd]), scale) : 0.f);
+    }
+  }
+}
+
+template <typename T, typename C, bool STORE>
+static int launch_quant8(const Quant8Args& a, const PagedAddr& addr, hipStream_t stream, const char* what) {
+  const int64_t wgs = (2 * a.T * a.H + 3) / 4;
+  quant8_rows<T, C, STORE><<<dim3(static_cast<uint32_t>(wgs < 65536 ? wgs : 65536)), dim3(256), 0, stream>>>(a, addr);
+  return check_launch(what);
+}
+
+// Rows (T, H, D) (store: the sources, passed as (H, T, D); load: the outputs), codes and scales.
+static int check_quant8(const tsa_view* k, const tsa_view* v, bool heads_first, const tsa_view* k_cache,
+                        const tsa_view* v_cache, const tsa_view* k_scale, const tsa_view* v_scale, Quant8Args& a) {
+  const char* const kn = heads_first ? "k_src" : "k_out";
+  const char* const vn = heads_first ? "v_src" : "v_out";
+  const int hd = heads_first ? 0 : 1, td = heads_first ? 1 : 0;
+  TSA_REQUIRE(view_ok(k, 3) && view_ok(v, 3), "%s and %s must be 3D tensors %s", kn, vn,
+              heads_first ? "(num_kv_heads, num_tokens, head_dim)" : "(num_tokens, num_kv_heads, head_dim)");
+  TSA_REQUIRE(view_ok(k_cache, 4) && view_ok(v_cache, 4),
+              "k_cache and v_cache must be 4D tensors (num_blocks, num_kv_heads, block_size, head_dim)");
+  TSA_REQUIRE(view_ok(k_scale, 3) && view_ok(v_scale, 3),
+              "k_scale and v_scale must be 3D tensors (num_blocks, num_kv_heads, block_size)");
+  for (int d = 0; d < 3; ++d) TSA_REQUIRE(k->size[d] == v->size[d], "%s and %s must have the same shape", kn, vn);
+  for (int d = 0; d < 4; ++d)
+    TSA_REQUIRE(k_cache->size[d] == v_cache->size[d], "k_cache and v_cache must have the same shape");
+  for (int d = 0; d < 3; ++d)
+    TSA_REQUIRE(k_scale->size[d] == k_cache->size[d] && v_scale->size[d] == k_cache->size[d],
+                "k_scale and v_scale must have the cache's shape but its head_dim");
+  TSA_REQUIRE(is_float_dtype(k->dtype) && v->dtype == k->dtype, "%s and %s must share one floating dtype (got %s/%s)",
+              kn, vn, dtype_name(k->dtype), dtype_name(v->dtype));
+  TSA_REQUIRE(is_cache8_dtype(k_cache->dtype) && v_cache->dtype == k_cache->dtype,
+              "k_cache and v_cache must share one 8-bit dtype, e4m3 or int8 (got %s/%s)", dtype_name(k_cache->dtype),
+              dtype_name(v_cache->dtype));
+  TSA_REQUIRE(k_scale->dtype == TSA_F32 && v_scale->dtype == TSA_F32, "k_scale and v_scale must be float32");
+  TSA_REQUIRE(k->size[hd] == k_cache->size[1], "%s has %lld kv heads but the cache has %lld", kn,
+              (long long)k->size[hd], (long long)k_cache->size[1]);
+  TSA_REQUIRE(k->size[2] == k_cache->size[3], "%s head_dim %lld != cache head_dim %lld", kn, (long long)k->size[2],
+              (long long)k_cache->size[3]);
+  TSA_REQUIRE(k_cache->size[2] > 0, "block_size must be positive");
+  a = Quant8Args{};
+  a.T = k->size[td]; a.H = k->size[hd]; a.D = k->size[2];
+  a.NB = k_cache->size[0]; a.BS = k_cache->size[2];
+  a.kr_t = k->stride[td]; a.kr_h = k->stride[hd]; a.kr_d = k->stride[2];
+  a.vr_t = v->stride[td]; a.vr_h = v->stride[hd]; a.vr_d = v->stride[2];
+  a.kc = static_cast<char*>(k_cache->data); a.vc = static_cast<char*>(v_cache->data);
+  a.ks = static_cast<float*>(k_scale->data); a.vs = static_cast<float*>(v_scale->data);
+  a.kc_b = k_cache->stride[0]; a.kc_h = k_cache->stride[1]; a.kc_s = k_cache->stride[2]; a.kc_d = k_cache->stride[3];
+  a.vc_b = v_cache->stride[0]; a.vc_h = v_cache->stride[1]; a.vc_s = v_cache->stride[2]; a.vc_d = v_cache->stride[3];
+  a.ks_b = k_scale->stride[0]; a.ks_h = k_scale->stride[1]; a.ks_s = k_scale->stride[2];
+  a.vs_b = v_scale->stride[0]; a.vs_h = v_scale->stride[1]; a.vs_s = v_scale->stride[2];
+  return TSA_OK;
+}
+
+template <bool STORE>
+static int dispatch_quant8(const Quant8Args& a, const PagedAddr& addr, int dt, int cache_dt, hipStream_t stream,
+                           const char* what) {
+  if (a.T == 0 || a.H == 0 || a.D == 0) return TSA_OK;
+  const bool e4m3 = cache_dt == TSA_E4M3;
+  switch (dt) {
+    case TSA_BF16:
+      return e4m3 ? launch_quant8<bf16_t, e4m3_t, STORE>(a, addr, stream, what)
+                  : launch_quant8<bf16_t, i8_t, STORE>(a, addr, stream, what);
+    case TSA_F16:
+      return e4m3 ? launch_quant8<f16_t, e4m3_t, STORE>(a, addr, stream, what)
+                  : launch_quant8<f16_t, i8_t, STORE>(a, addr, stream, what);
+    default:
+      return e4m3 ? launch_quant8<float, e4m3_t, STORE>(a, addr, stream, what)
+                  : launch_quant8<float, i8_t, STORE>(a, addr, stream, what);
+  }
+}
+
+}  // namespace tsa
+
+using namespace tsa;
+
+extern "C" int tsa_store_kv_quantized(const tsa_view* k_src, const tsa_view* v_src, const tsa_view* k_cache,
+                                      const tsa_view* v_cache, const tsa_view* k_scale, const tsa_view* v_scale,
+                                      const tsa_view* block_tables, const tsa_view* cu_seqlens,
+                                      const tsa_view* positions, void* stream) {
+  Quant8Args a;
+  if (int rc = check_quant8(k_src, v_src, true, k_cache, v_cache, k_scale, v_scale, a)) return rc;
+  a.k_src = static_cast<const char*>(k_src->data);
+  a.v_src = static_cast<const char*>(v_src->data);
+  PagedAddr addr;
+  if (int rc = make_paged_addr(block_tables, cu_seqlens, positions, a.T, addr)) return rc;
+  if (a.NB == 0) return TSA_OK;  // (no page to write)
+  return dispatch_quant8<true>(a, addr, k_src->dtype, k_cache->dtype, static_cast<hipStream_t>(stream),
+                               "tsa_store_kv_quantized");
+}
+
+extern "C" int tsa_load_kv_quantized(const tsa_view* k_out, const tsa_view* v_out, const tsa_view* k_cache,
+                                     const tsa_view* v_cache, const tsa_view* k_scale, const tsa_view* v_scale,
+                                     const tsa_view* block_tables, const tsa_view* cu_seqlens,
+                                     const tsa_view* positions, void* stream) {
+  Quant8Args a;
+  if (int rc = check_quant8(k_out, v_out, false, k_cache, v_cache, k_scale, v_scale, a)) return rc;
+  a.k_out = static_cast<char*>(k_out->data);
+  a.v_out = static_cast<char*>(v_out->data);
+  PagedAddr addr;
+  if (int rc = make_paged_addr(block_tables, cu_seqlens, positions, a.T, addr)) return rc;
+  return dispatch_quant8<false>(a, addr, k_out->dtype, k_cache->dtype, static_cast<hipStream_t>(stream),
+                                "tsa_load_kv_quantized");
+}

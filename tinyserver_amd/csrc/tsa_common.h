@@ -44,7 +44,10 @@ inline int check_launch(const char* what) {
 // ----------------------------------------------------------------- views --
 inline bool is_float_dtype(int dt) { return dt == TSA_BF16 || dt == TSA_F16 || dt == TSA_F32; }
 inline bool is_index_dtype(int dt) { return dt == TSA_I32 || dt == TSA_I64; }
-inline int dtype_bytes(int dt) { return dt == TSA_F32 || dt == TSA_I32 ? 4 : dt == TSA_I64 ? 8 : 2; }
+inline bool is_cache8_dtype(int dt) { return dt == TSA_E4M3 || dt == TSA_I8; }
+inline int dtype_bytes(int dt) {
+  return dt == TSA_F32 || dt == TSA_I32 ? 4 : dt == TSA_I64 ? 8 : is_cache8_dtype(dt) ? 1 : 2;
+}
 inline const char* dtype_name(int dt) {
   switch (dt) {
     case TSA_BF16: return "bf16";
@@ -52,6 +55,8 @@ inline const char* dtype_name(int dt) {
     case TSA_F32: return "f32";
     case TSA_I32: return "i32";
     case TSA_I64: return "i64";
+    case TSA_E4M3: return "e4m3";
+    case TSA_I8: return "i8";
   }
   return "?";
 }
@@ -60,7 +65,7 @@ inline const char* dtype_name(int dt) {
 // and non-negative sizes. Data may be NULL only for an empty view.
 inline bool view_ok(const tsa_view* v, int ndim) {
   if (!v || v->ndim != ndim) return false;
-  if (v->dtype < TSA_BF16 || v->dtype > TSA_I64) return false;
+  if (v->dtype < TSA_BF16 || v->dtype > TSA_I8) return false;
   int64_t n = 1;
   for (int d = 0; d < ndim; ++d) {
     if (v->size[d] < 0) return false;
