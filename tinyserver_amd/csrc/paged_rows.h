@@ -31,7 +31,9 @@ struct RowsArgs {
   int32_t words;      // trees: 32-bit words of a row's mask
   int32_t window;     // the last tokens a row sees (0: all)
   int32_t sinks;      // the first tokens that stay visible
+  int32_t S;          // splits of a unit's tokens
   float scale_log2;
+  float* part;        // their partials
 };
 
 constexpr float kNegInfR = -INFINITY;
@@ -72,5 +74,10 @@ int check_rows(const tsa_view* out, const tsa_view* query, const tsa_view* k_cac
                const tsa_view* k_scale, const tsa_view* v_scale, const tsa_view* block_tables, const tsa_view* lens,
                const tsa_view* cu_nodes, const tsa_view* tree_mask, int64_t max_nodes, int64_t window, int64_t sinks,
                double softmax_scale, RowsArgs& a);
+
+// paged_rows_unit.hip: the decode forms on the matrix cores. Splits of a unit of
+// at most max_tiles visible 16-token tiles, and the launch (a.S, a.part set).
+int rows_unit_splits(int64_t max_tiles, bool cache8);
+int rows_unit_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what);
 
 }  // namespace tsa
