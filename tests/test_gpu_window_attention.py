@@ -106,6 +106,26 @@ def test_decode_long(cache, hq, lens, page, window, sinks):
     check(_run_decode(case, page, window, sinks), ref, tol, f"{cache} {hq}/2, {lens}, {window}+{sinks}")
 
 
+@pytest.mark.parametrize("cache", [None, E4, I8])
+@pytest.mark.parametrize("hq,hkv,d,page,dtype,batch,longest,window,sinks", [
+    (16, 8, 128, 16, BF, 64, 2500, 0, 0),
+    (32, 8, 64, 32, F16, 48, 3000, 0, 0),
+    (16, 8, 128, 256, BF, 64, 3000, 1900, 40),
+    (40, 2, 128, 16, F16, 150, 2100, 1800, 5),
+    (8, 8, 128, 16, BF, 300, 1300, 0, 0),
+])
+def test_decode_many_tiles(cache, hq, hkv, d, page, dtype, batch, longest, window, sinks):
+    """Batches whose tables hold many tiles, of sequences that are short but for one: runs that cross units, empty
+    sequences, units of one tile, one that many waves share."""
+    g = torch.Generator().manual_seed(batch)
+    lens = (torch.rand(batch, generator=g) ** 3 * 150).long().tolist()
+    lens[batch // 3], lens[0], lens[-1] = longest, 0, 17
+    if cache is None and not window:
+        window = 1 << 20
+    case, ref, tol = _decode_case(lens, hq, hkv, d, page, dtype, window, sinks, cache)
+    check(_run_decode(case, page, window, sinks), ref, tol, f"{cache} {batch} x {hq}/{hkv} x {d}, {window}+{sinks}")
+
+
 def test_decode_scales_that_16_bits_do_not_hold():
     """Rows of values near 1e-6 and 1e5 in one 8-bit cache, with f16 queries."""
     lens = [300, 40]

@@ -31,12 +31,31 @@ struct RowsArgs {
   int32_t words;      // trees: 32-bit words of a row's mask
   int32_t window;     // the last tokens a row sees (0: all)
   int32_t sinks;      // the first tokens that stay visible
-  int32_t S;          // splits of a unit's tokens
+  int32_t S;          // splits of a unit's tokens (0: the stream)
+  int32_t NW;         // waves of the stream
+  // The matrix-core forms: page strides in bytes, and the tiles (16 tokens) of a
+  // page as a multiplier and a shift (tiles_of_page).
+  uint32_t k_page, v_page, ks_page, vs_page, page_mul, page_shift;
   float scale_log2;
   float* part;        // their partials
+  int32_t* pref;      // the stream: tile pairs before each sequence
 };
 
 constexpr float kNegInfR = -INFINITY;
+
+// tile / (BS / 16) for tiles below 2^23 (tables hold less than 2^27 tokens):
+// (tile * mul) >> (23 + shift) with shift = ceil(log2 d), mul = ceil(2^(23 +
+// shift) / d), whose error, less than d <= 2^shift in 2^(23 + shift), stays
+// below a unit of 1 / d for tiles below 2^23.
+__host__ __device__ __forceinline__ uint32_t page_of_tile(uint32_t tile, uint32_t mul, uint32_t shift) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(tile) * mul) >> (23 + shift));
+}
+inline void set_page_div(RowsArgs& a) {
+  const uint64_t d = static_cast<uint64_t>(a.BS) / 16;
+  a.page_shift = 0;
+  while ((uint64_t{1} << a.page_shift) < d) ++a.page_shift;
+  a.page_mul = static_cast<uint32_t>(((uint64_t{1} << (23 + a.page_shift)) + d - 1) / d);
+}
 
 // A sequence's tokens: ctx of the cache's, then the drafted nodes at positions
 // ctx .. ctx + nodes - 1; end is past the last that its block table holds. rows
@@ -75,9 +94,17 @@ int check_rows(const tsa_view* out, const tsa_view* query, const tsa_view* k_cac
                const tsa_view* cu_nodes, const tsa_view* tree_mask, int64_t max_nodes, int64_t window, int64_t sinks,
                double softmax_scale, RowsArgs& a);
 
-// paged_rows_unit.hip: the decode forms on the matrix cores. Splits of a unit of
-// at most max_tiles visible 16-token tiles, and the launch (a.S, a.part set).
-int rows_unit_splits(int64_t max_tiles, bool cache8);
+// The plan of a decode call on the matrix cores: splits of a unit (0: the
+// stream, of `waves` waves) and the workspace, part_bytes of partials and the
+// stream's prefix.
+struct DecodeRowsPlan {
+  int S, waves;
+  size_t part_bytes, total;
+};
+DecodeRowsPlan decode_rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, int64_t window,
+                                int64_t sinks, bool cache8);
+// paged_rows_unit.hip, paged_rows_stream.hip: the launches (a.S, a.NW, a.part, a.pref set).
 int rows_unit_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what);
+int rows_stream_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what);
 
 }  // namespace tsa

@@ -191,46 +191,24 @@ int check_rows(const tsa_view* out, const tsa_view* query, const tsa_view* k_cac
 }
 
 // The matrix-core forms: 16-bit queries, head_dim 64 or 128, pages of whole
-// 16-token tiles, unit-stride rows of 16-byte pieces whose offsets within a tile
-// fit 31 bits.
-static bool takes_mfma(const RowsArgs& a, const tsa_view* query, const tsa_view* k_cache, const tsa_view* v_cache) {
+// 16-token tiles, unit-stride rows of 16-byte pieces, and strides whose offsets
+// within a page fit 31 bits (a page's own 32). Fills what they need of a.
+static bool takes_mfma(RowsArgs& a, const tsa_view* query, const tsa_view* k_cache, const tsa_view* v_cache) {
   if ((query->dtype != TSA_BF16 && query->dtype != TSA_F16) || (a.D != 64 && a.D != 128) || a.BS % 16 || a.NB == 0)
     return false;
   if (!rows_vec16(query) || !rows_vec16(k_cache) || !rows_vec16(v_cache)) return false;
-  constexpr int64_t kMaxStride = int64_t{1} << 24;
-  if (a.kc_s < 0 || a.kc_s >= kMaxStride || a.vc_s < 0 || a.vc_s >= kMaxStride) return false;
+  const int64_t eb = dtype_bytes(k_cache->dtype);
+  auto fits = [&](int64_t page, int64_t slot, int64_t bytes) {
+    return page >= 0 && page < (int64_t{1} << 32) / bytes && slot >= 0 && slot < (int64_t{1} << 31) / bytes / a.BS;
+  };
+  if (!fits(a.kc_b, a.kc_s, eb) || !fits(a.vc_b, a.vc_s, eb)) return false;
+  if (a.ks && (!fits(a.ks_b, a.ks_s, 4) || !fits(a.vs_b, a.vs_s, 4))) return false;
+  a.k_page = static_cast<uint32_t>(a.kc_b * eb);
+  a.v_page = static_cast<uint32_t>(a.vc_b * eb);
+  a.ks_page = static_cast<uint32_t>(a.ks_b * 4);
+  a.vs_page = static_cast<uint32_t>(a.vs_b * 4);
+  set_page_div(a);
   return true;
-}
-
-// The plan of a decode call: a unit's splits and the bytes of their partials.
-struct RowsPlan {
-  int S;
-  size_t bytes;
-};
-static size_t part_bytes(int64_t units, int64_t S, int64_t rows, int64_t D) {
-  return S <= 1 ? 0 : static_cast<size_t>(units * S * rows * (D + 4)) * sizeof(float);
-}
-static RowsPlan decode_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, int64_t window, int64_t sinks,
-                            bool cache8) {
-  int64_t tiles = (cap + 15) / 16;
-  if (window > 0 && window < cap) {
-    const int64_t seen = ((sinks < cap ? sinks : cap) + 15) / 16 + (window + 15) / 16 + 1;
-    tiles = seen < tiles ? seen : tiles;
-  }
-  RowsPlan p{};
-  p.S = rows_unit_splits(tiles, cache8);
-  p.bytes = part_bytes(B * Hkv, p.S, Hq / Hkv, D);
-  return p;
-}
-
-static int bind_part(RowsArgs& a, const RowsPlan& p, void* workspace, size_t workspace_bytes) {
-  a.S = p.S;
-  if (p.bytes == 0) return TSA_OK;
-  TSA_REQUIRE(workspace != nullptr && workspace_bytes >= p.bytes, "workspace of %zu bytes is too small: %zu needed",
-              workspace_bytes, p.bytes);
-  TSA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
-  a.part = static_cast<float*>(workspace);
-  return TSA_OK;
 }
 
 static int dispatch_rows(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what) {
@@ -266,12 +244,18 @@ extern "C" int tsa_paged_decode_window(const tsa_view* out, const tsa_view* quer
                           window, sinks, softmax_scale, a))
     return rc;
   if (a.B > 0 && a.Hq > 0 && takes_mfma(a, query, k_cache, v_cache)) {
-    const RowsPlan p = decode_plan(a.B, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS, a.window, a.sinks, a.ks != nullptr);
-    const int64_t items = int64_t{a.B} * a.Hkv * ((a.G + 15) / 16);
-    if (items * p.S < (int64_t{1} << 23)) {  // (a launch's threads fit 32 bits)
-      if (int rc = bind_part(a, p, workspace, workspace_bytes)) return rc;
-      return rows_unit_launch(a, query->dtype, k_cache->dtype, static_cast<hipStream_t>(stream), "tsa_paged_decode_window");
-    }
+    const DecodeRowsPlan p = decode_rows_plan(a.B, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS, a.window, a.sinks,
+                                              a.ks != nullptr);
+    TSA_REQUIRE(p.total == 0 || (workspace != nullptr && workspace_bytes >= p.total),
+                "workspace of %zu bytes is too small: %zu needed", workspace_bytes, p.total);
+    TSA_REQUIRE(p.total == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
+    a.S = p.S;
+    a.NW = p.waves;
+    a.part = static_cast<float*>(workspace);
+    a.pref = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + p.part_bytes);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    return p.S > 0 ? rows_unit_launch(a, query->dtype, k_cache->dtype, st, "tsa_paged_decode_window")
+                   : rows_stream_launch(a, query->dtype, k_cache->dtype, st, "tsa_paged_decode_window");
   }
   return dispatch_rows(a, query->dtype, k_cache->dtype, static_cast<hipStream_t>(stream), "tsa_paged_decode_window");
 }
@@ -299,6 +283,7 @@ extern "C" size_t tsa_paged_rows_workspace_bytes(int64_t num_seqs, int64_t max_n
       max_blocks_per_seq * block_size >= (int64_t{1} << 27))
     return 0;  // (calls of such sizes are refused, or have nothing to do)
   const int64_t cap = max_blocks_per_seq * block_size;
-  // Either kind of cache: a 16-bit one has the smaller splits.
-  return decode_plan(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks, false).bytes;
+  const DecodeRowsPlan p16 = decode_rows_plan(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks, false);
+  const DecodeRowsPlan p8 = decode_rows_plan(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks, true);
+  return p16.total > p8.total ? p16.total : p8.total;  // for either kind of cache
 }

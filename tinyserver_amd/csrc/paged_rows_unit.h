@@ -126,9 +126,8 @@ __device__ __forceinline__ void rows_unit_wave(const RowsArgs& a, const int32_t*
 
   // Lane j: the split's tile j, its page and first slot.
   const int my_v = t0 + (lane & (kTiles - 1));
-  const uint32_t my_tok = 16u * static_cast<uint32_t>(ut.at(my_v));
-  const uint32_t my_lb = my_tok / static_cast<uint32_t>(a.BS);
-  const int my_slot = static_cast<int>(my_tok - my_lb * static_cast<uint32_t>(a.BS));
+  const uint32_t my_tile = static_cast<uint32_t>(ut.at(my_v)), my_lb = page_of_tile(my_tile, a.page_mul, a.page_shift);
+  const int my_slot = static_cast<int>(16u * my_tile - my_lb * static_cast<uint32_t>(a.BS));
   const int my_page = bt[s * a.bt_s0 + min(static_cast<int>(my_lb), a.max_blocks - 1) * a.bt_s1];
   const uint64_t ok64 = __ballot(my_v < ut.n && my_page >= 0 && my_page < a.NB);
 
@@ -150,15 +149,19 @@ __device__ __forceinline__ void rows_unit_wave(const RowsArgs& a, const int32_t*
   uint32_t vis[KT];      // bit i: token i of the tile is seen
   const char* const kbase = static_cast<const char*>(a.kc) + kvh * a.kc_h * eb;
   const char* const vbase = static_cast<const char*>(a.vc) + kvh * a.vc_h * eb;
+  const char* const ksbase = reinterpret_cast<const char*>(a.ks + kvh * a.ks_h);
+  const char* const vsbase = reinterpret_cast<const char*>(a.vs + kvh * a.vs_h);
   const uint32_t k_lane = static_cast<uint32_t>(c * static_cast<int>(a.kc_s) * eb + 16 * g);
   const uint32_t v_lane = static_cast<uint32_t>((4 * g) * static_cast<int>(a.vc_s) * eb + NU * eb * c);
+  const uint32_t ks_lane = static_cast<uint32_t>((4 * g + (c & 3)) * static_cast<int>(a.ks_s) * 4);
+  const uint32_t vs_lane = static_cast<uint32_t>((4 * g + (c & 3)) * static_cast<int>(a.vs_s) * 4);
 #pragma unroll
   for (int x = 0; x < KT; ++x) {
     const int j = vw + NW * x;
     vis[x] = 0;
     if (t0 + j < ut.n) {  // (uniform)
       const bool ok = (ok64 >> j) & 1;
-      const int64_t page = ok ? __builtin_amdgcn_readlane(my_page, j) : 0;
+      const uint32_t page = ok ? __builtin_amdgcn_readlane(my_page, j) : 0;
       const int slot0 = ok ? __builtin_amdgcn_readlane(my_slot, j) : 0;
       const int tok0 = 16 * ut.at(t0 + j), left = ut.L - tok0;
       uint32_t m16 = left >= 16 ? 0xFFFFu : (1u << left) - 1u;
@@ -168,15 +171,17 @@ __device__ __forceinline__ void rows_unit_wave(const RowsArgs& a, const int32_t*
         m16 &= in_window | (first >= 16 ? 0xFFFFu : first > 0 ? (1u << first) - 1u : 0u);
       }
       vis[x] = ok ? m16 : 0u;
-      const char* const kp = kbase + (page * a.kc_b + slot0 * a.kc_s) * eb;
-      const char* const vp = vbase + (page * a.vc_b + slot0 * a.vc_s) * eb;
+      const char* const kp = kbase + static_cast<uint64_t>(page) * a.k_page + slot0 * static_cast<int>(a.kc_s) * eb;
+      const char* const vp = vbase + static_cast<uint64_t>(page) * a.v_page + slot0 * static_cast<int>(a.vc_s) * eb;
 #pragma unroll
       for (int i = 0; i < KL; ++i) ko[x][i] = load_piece<NT, u32x4>(kp + k_lane + 64 * i);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) vo[x][r] = load_piece<NT, VP>(vp + r * a.vc_s * eb + v_lane);
+      for (int r = 0; r < 4; ++r) vo[x][r] = load_piece<NT, VP>(vp + r * static_cast<int>(a.vc_s) * eb + v_lane);
       if constexpr (kIs8<C>) {
-        ks[x] = a.ks[page * a.ks_b + kvh * a.ks_h + (slot0 + 4 * g + (c & 3)) * a.ks_s];
-        vs[x] = a.vs[page * a.vs_b + kvh * a.vs_h + (slot0 + 4 * g + (c & 3)) * a.vs_s];
+        ks[x] = *reinterpret_cast<const float*>(ksbase + static_cast<uint64_t>(page) * a.ks_page +
+                                                slot0 * static_cast<int>(a.ks_s) * 4 + ks_lane);
+        vs[x] = *reinterpret_cast<const float*>(vsbase + static_cast<uint64_t>(page) * a.vs_page +
+                                                slot0 * static_cast<int>(a.vs_s) * 4 + vs_lane);
       }
     } else {
 #pragma unroll

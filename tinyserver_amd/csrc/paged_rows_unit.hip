@@ -1,7 +1,24 @@
 // Instances and launch of the unit form (paged_rows_unit.h).
-#include "paged_rows_unit.h"
+#include "paged_rows_stream.h"
 
 namespace tsa {
+
+// Split calls of up to this many workgroups take the unit form.
+#ifndef TSA_ROWS_UNIT_MAX
+#define TSA_ROWS_UNIT_MAX 2048
+#endif
+constexpr int64_t kUnitMaxWorkgroups = TSA_ROWS_UNIT_MAX;
+#ifndef TSA_ROWS_STREAM_PER_CU
+#define TSA_ROWS_STREAM_PER_CU 1
+#endif
+// The stream's grid: a four-wave workgroup a CU.
+static int stream_workgroups() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
+    cus = 256;
+  return TSA_ROWS_STREAM_PER_CU * cus;
+}
 
 // Units of this many splits or more read K/V with non-temporal loads.
 constexpr int kRowsNtSplits = 16;
@@ -42,12 +59,30 @@ int rows_unit_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream
                               : launch_unit_d<f16_t, f16_t>(a, stream, what);
 }
 
-// Splits: one workgroup of eight waves where a unit's visible tiles fit it, else
-// workgroups of four.
-int rows_unit_splits(int64_t max_tiles, bool cache8) {
+// One workgroup of eight waves a unit where its visible tiles fit it, else
+// splits of four waves each, else the stream.
+DecodeRowsPlan decode_rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, int64_t window,
+                                int64_t sinks, bool cache8) {
+  int64_t tiles = (cap + 15) / 16;
+  if (window > 0 && window < cap) {
+    const int64_t seen = ((sinks < cap ? sinks : cap) + 15) / 16 + (window + 15) / 16 + 1;
+    tiles = seen < tiles ? seen : tiles;
+  }
   const int kt = cache8 ? kUnitTiles<i8_t> : kUnitTiles<bf16_t>;
-  if (max_tiles <= kUnitWavesOne * kt) return 1;
-  return static_cast<int>((max_tiles + kUnitWavesSplit * kt - 1) / (kUnitWavesSplit * kt));
+  const int64_t G = Hq / Hkv, items = B * Hkv * ((G + 15) / 16), rows = G < 16 ? G : 16;
+  const size_t slot = static_cast<size_t>(rows) * (D + 4) * sizeof(float);
+  auto align = [](size_t n) { return (n + 255) & ~size_t{255}; };
+  DecodeRowsPlan p{};
+  const int64_t S = tiles <= kUnitWavesOne * kt ? 1 : (tiles + kUnitWavesSplit * kt - 1) / (kUnitWavesSplit * kt);
+  if (S == 1 || items * S <= kUnitMaxWorkgroups || B > kStreamMaxSeqs) {
+    p.S = static_cast<int>(S);
+    p.total = p.part_bytes = S == 1 ? 0 : align(static_cast<size_t>(B * Hkv * S * G) * (D + 4) * sizeof(float));
+    return p;
+  }
+  p.waves = kStreamWaves * stream_workgroups();
+  p.part_bytes = align((static_cast<size_t>(items) + p.waves) * slot);
+  p.total = p.part_bytes + align((static_cast<size_t>(B) + 1) * sizeof(int32_t));
+  return p;
 }
 
 }  // namespace tsa
