@@ -33,6 +33,7 @@ struct RowsArgs {
   int32_t sinks;      // the first tokens that stay visible
   int32_t S;          // splits of a unit's tokens (0: the stream)
   int32_t NW;         // waves of the stream
+  int32_t RT, RB, per_split;  // trees: 32-row tiles of a workgroup, row blocks of a unit, 32-key blocks of a split
   // The matrix-core forms: page strides in bytes, and the tiles (16 tokens) of a
   // page as a multiplier and a shift (tiles_of_page).
   uint32_t k_page, v_page, ks_page, vs_page, page_mul, page_shift;
@@ -106,5 +107,12 @@ DecodeRowsPlan decode_rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
 // paged_rows_unit.hip, paged_rows_stream.hip: the launches (a.S, a.NW, a.part, a.pref set).
 int rows_unit_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what);
 int rows_stream_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what);
+// paged_rows_tree.hip: the plan of a tree call of at most T nodes a sequence, and the launch.
+struct TreeRowsPlan {
+  int RT, RB, S, per_split;
+  size_t bytes;
+};
+TreeRowsPlan tree_rows_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap);
+int rows_tree_launch(const RowsArgs& a, int dt, hipStream_t stream);
 
 }  // namespace tsa

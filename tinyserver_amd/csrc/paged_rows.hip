@@ -269,8 +269,17 @@ extern "C" int tsa_paged_tree(const tsa_view* out, const tsa_view* query, const 
   if (int rc = check_rows(out, query, k_cache, v_cache, nullptr, nullptr, block_tables, context_lens, cu_nodes,
                           tree_mask, max_nodes, 0, 0, softmax_scale, a))
     return rc;
-  (void)workspace;
-  (void)workspace_bytes;
+  if (a.B > 0 && a.Hq > 0 && a.T > 0 && a.N > 0 && a.scale_log2 > 0.f && takes_mfma(a, query, k_cache, v_cache)) {
+    const TreeRowsPlan p = tree_rows_plan(a.B, a.T, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS);
+    if (int64_t{a.B} * a.Hkv * p.S * p.RB < (int64_t{1} << 23)) {  // (a launch's threads fit 32 bits)
+      TSA_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes),
+                  "workspace of %zu bytes is too small: %zu needed", workspace_bytes, p.bytes);
+      TSA_REQUIRE(p.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
+      a.S = p.S; a.RT = p.RT; a.RB = p.RB; a.per_split = p.per_split;
+      a.part = static_cast<float*>(workspace);
+      return rows_tree_launch(a, query->dtype, static_cast<hipStream_t>(stream));
+    }
+  }
   return dispatch_rows(a, query->dtype, k_cache->dtype, static_cast<hipStream_t>(stream), "tsa_paged_tree");
 }
 
@@ -285,5 +294,8 @@ extern "C" size_t tsa_paged_rows_workspace_bytes(int64_t num_seqs, int64_t max_n
   const int64_t cap = max_blocks_per_seq * block_size;
   const DecodeRowsPlan p16 = decode_rows_plan(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks, false);
   const DecodeRowsPlan p8 = decode_rows_plan(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks, true);
-  return p16.total > p8.total ? p16.total : p8.total;  // for either kind of cache
+  const size_t decode = p16.total > p8.total ? p16.total : p8.total;  // for either kind of cache
+  if (window > 0 || sinks > 0) return decode;
+  const size_t tree = tree_rows_plan(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, cap).bytes;
+  return max_nodes > 1 ? tree : tree > decode ? tree : decode;
 }

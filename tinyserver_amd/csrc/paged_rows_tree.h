@@ -1,0 +1,304 @@
+// Attention of drafted tokens' trees on the matrix cores: the rows of a unit
+// (sequence, kv head) are its nodes' q-heads of that kv head, so every K/V byte
+// read serves nodes x heads rows.
+//
+// What bounds it: HBM for small trees (each K/V byte once), the matrix cores
+// and the exponentials beside them from some 200 rows a unit on. A workgroup of
+// four waves takes up to 32, 64 or 128 rows (the sequence's count decides): RT =
+// 1, 2 or 4 tiles of 32 rows and 4 / RT runs of keys, wave (rt, kg) row tile rt
+// over every (4 / RT)-th 32-key block. A unit's keys are split over workgroups,
+// whose partials a second launch merges. Row blocks of one unit and split go to
+// one XCD, one after the other, and share its L2.
+//
+// With lane (h, c) = (lane / 32, lane % 32), v_mfma_f32_32x32x16:
+//   S^T(32 keys x 32 rows) = K Q^T over D / 16 steps: lane (h, c) reads key c,
+//     dims 16 j + 8 h..+8, and holds row c's Q; element e of the result is the
+//     score of key 8 (e / 4) + 4 h + e % 4 for row c.
+//   O^T(dims x rows) += V^T P^T over two 16-key steps s: the P^T operand is the
+//     lane's own weights 8 s .. 8 s + 7, and V's operand is dim (D / 32) c + u of
+//     those same eight keys, from rows read 8 (4) bytes a lane. Lane (h, c)
+//     accumulates row c, so the softmax's scales are the lane's own.
+// K of the next block is asked for as soon as the scores have taken this
+// block's, V after the second product.
+//
+// A block of keys that every row sees (all of the context's but the last) takes
+// no mask. In the others each row has 32 bits: the context's tokens and its own
+// mask words' nodes. A weight of 0 times an infinity or NaN in V would be NaN, so
+// there V is tested, and elements that are not finite leave the product and
+// reach the rows that see them by a product of their own (flag_product).
+#pragma once
+
+#include "paged_rows_unit.h"
+
+namespace tsa {
+
+constexpr float kTreeRescale = 8.f;  // log2 units a maximum grows before it moves
+
+// Elements of a dword of T that are not finite: which (bit 0: low, 1: high).
+template <typename T> __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
+  constexpr uint32_t kExp = std::is_same<T, bf16_t>::value ? 0x7F80u : 0x7C00u;
+  return ((w & kExp) == kExp ? 1u : 0u) | (((w >> 16) & kExp) == kExp ? 2u : 0u);
+}
+// A 16-bit element as a flag of T: 0 (finite), 1 (+inf), 2^8 (-inf), 2^15 (NaN).
+// Sums of up to 32 of each are told apart.
+template <typename T> __device__ __forceinline__ uint32_t flag16(uint32_t x) {
+  constexpr bool bf = std::is_same<T, bf16_t>::value;
+  constexpr uint32_t kExp = bf ? 0x7F80u : 0x7C00u;
+  if ((x & kExp) != kExp) return 0;
+  if (x & (0x7FFFu ^ kExp)) return bf ? 0x4700u : 0x7800u;
+  return x & 0x8000u ? (bf ? 0x4380u : 0x5C00u) : (bf ? 0x3F80u : 0x3C00u);
+}
+// What a sum of flags adds to an output.
+__device__ __forceinline__ float flag_value(float n) {
+  const int k = static_cast<int>(n);
+  const bool nan = k >= 32768, pos = (k & 255) != 0, neg = ((k >> 8) & 127) != 0;
+  return nan || (pos && neg) ? __builtin_nanf("") : pos ? INFINITY : neg ? -INFINITY : 0.f;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void paged_rows_tree(
+    RowsArgs a, const int32_t* __restrict__ bt, const uint32_t* __restrict__ mask, float* __restrict__ part) {
+  constexpr int KJ = D / 16, NU = D / 32, PF = part_floats(D);
+  typedef typename VPiece<2 * NU>::type VP;
+  __shared__ __align__(16) float slots[4 * 32 * PF];
+  // ---- Which unit, split and row block.
+  const int id = blockIdx.x, k8 = id >> 3;
+  const int rb = k8 % a.RB, us = (k8 / a.RB) * 8 + (id & 7), U = a.B * a.Hkv;
+  if (us >= U * a.S) return;
+  const int sp = us / U, u = us - sp * U, s = u / a.Hkv, kvh = u - s * a.Hkv;
+  const SeqRange r = seq_of(a, s);
+  const int all = r.nodes * a.G, R = 32 * a.RT, row_first = rb * R, rows = min(all - row_first, R);
+  if (rows <= 0) return;
+  const int nblk = (r.end + 31) >> 5, b0 = sp * a.per_split, b1 = min(nblk, b0 + a.per_split);
+  if (b0 >= b1 && a.S > 1) return;  // (the merge takes the splits that have blocks)
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int RT = rows <= 32 ? 1 : rows <= 64 ? 2 : 4, KG = 4 / RT, rt = wave % RT, kg = wave / RT;
+
+  const int row = min(row_first + 32 * rt + c, all - 1);  // (past the last: it again, never stored)
+  const int node = row / a.G, head = kvh * a.G + row - node * a.G;
+  const int64_t prow = r.row0 + node;
+  const uint32_t* const my_mask = mask + prow * a.mask_s;
+  u32x4 q[KJ];
+  {
+    const T* const qp = static_cast<const T*>(a.q) + prow * a.q_sr + head * a.q_sh + 8 * h;
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) q[j] = *reinterpret_cast<const u32x4*>(qp + 16 * j);
+  }
+  const float cs = a.scale_log2;  // > 0 here
+  float m = kNegInfR, l = 0.f;
+  f32x16 acc[NU];
+#pragma unroll
+  for (int x = 0; x < NU; ++x)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[x][e] = 0.f;
+
+  const int mine = b0 + kg < b1 ? (b1 - b0 - kg + KG - 1) / KG : 0;  // this wave's blocks
+  if (32 * rt < rows && mine > 0) {
+    // Lane 2 i + half: the page and first slot of that half of the wave's
+    // block i0 + i, for 32 blocks at a time.
+    int my_page = 0, my_slot = 0;
+    uint64_t ok64 = 0;
+    auto lookup = [&](int i0) __attribute__((always_inline)) {
+      const int blk = b0 + kg + KG * (i0 + (lane >> 1));
+      const uint32_t tile = static_cast<uint32_t>(2 * blk + (lane & 1)), lb = page_of_tile(tile, a.page_mul, a.page_shift);
+      my_slot = static_cast<int>(16u * tile - lb * static_cast<uint32_t>(a.BS));
+      const bool in = static_cast<int>(16u * tile) < r.end;
+      my_page = bt[s * a.bt_s0 + min(static_cast<int>(lb), a.max_blocks - 1) * a.bt_s1];
+      ok64 = __ballot(in && my_page >= 0 && my_page < a.NB);
+    };
+    const char* const kb = static_cast<const char*>(a.kc) + kvh * a.kc_h * 2;
+    const char* const vb = static_cast<const char*>(a.vc) + kvh * a.vc_h * 2;
+    const uint32_t k_slot = static_cast<uint32_t>(a.kc_s) * 2, v_slot = static_cast<uint32_t>(a.vc_s) * 2;
+    const uint32_t k_lane = static_cast<uint32_t>(c & 15) * k_slot + 16u * h;
+    const uint32_t v_lane = 4u * h * v_slot + 2u * NU * c;
+    u32x4 kr[KJ];
+    VP vr[16];
+    // Rows of pages outside the pool, and of halves past the end, are row 0 of
+    // page 0 (and masked).
+    auto load_k = [&](int i) __attribute__((always_inline)) {
+      const int x = 2 * (i & 31);
+      const char* p[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const bool ok = (ok64 >> (x + y)) & 1;
+        const uint32_t page = ok ? __builtin_amdgcn_readlane(my_page, x + y) : 0;
+        const uint32_t slot = ok ? __builtin_amdgcn_readlane(my_slot, x + y) : 0;
+        p[y] = kb + static_cast<uint64_t>(page) * a.k_page + slot * k_slot;
+      }
+      const char* const kp = (c < 16 ? p[0] : p[1]) + k_lane;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) kr[j] = *reinterpret_cast<const u32x4*>(kp + 32 * j);
+    };
+    auto load_v = [&](int i) __attribute__((always_inline)) {
+      const int x = 2 * (i & 31);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const bool ok = (ok64 >> (x + y)) & 1;
+        const uint32_t page = ok ? __builtin_amdgcn_readlane(my_page, x + y) : 0;
+        const uint32_t slot = ok ? __builtin_amdgcn_readlane(my_slot, x + y) : 0;
+        const char* const p = vb + static_cast<uint64_t>(page) * a.v_page + slot * v_slot;
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          vr[8 * y + t] = *reinterpret_cast<const VP*>(p + ((t & 3) + 8 * (t >> 2)) * v_slot + v_lane);
+      }
+    };
+    lookup(0);
+    load_k(0);
+    load_v(0);
+    for (int i = 0; i < mine; ++i) {
+      const int blk = b0 + kg + KG * i;
+      const uint32_t okb = static_cast<uint32_t>(ok64 >> (2 * (i & 31))) & 3u;
+      const uint64_t ok_cur = ok64;
+      const int page_cur = my_page, slot_cur = my_slot;
+      (void)ok_cur; (void)page_cur; (void)slot_cur;
+      f32x16 sc;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) sc = mfma_k16x32<T>(kr[j], q[j], sc);
+      const bool more = i + 1 < mine;
+      if (((i + 1) & 31) == 0 && more) lookup(i + 1);
+      load_k(more ? i + 1 : i);  // (the last block's again: unconditional, so that the waits count it)
+      uint32_t vis = ~0u;
+      if (okb != 3u || 32 * blk + 32 > r.ctx) {  // (uniform) some key that some row does not see
+        auto below = [](int n) { return n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u; };
+        const uint32_t there = below(r.end - 32 * blk) & ((okb & 1 ? 0xFFFFu : 0u) | (okb & 2 ? 0xFFFF0000u : 0u));
+        const int j0 = 32 * blk - r.ctx, w = j0 >> 5, sh = j0 & 31;
+        const uint32_t lo = w >= 0 && w < a.words ? my_mask[w] : 0u;
+        const uint32_t hi = w + 1 >= 0 && w + 1 < a.words ? my_mask[w + 1] : 0u;
+        const uint32_t nodes = sh ? (lo >> sh) | (hi << (32 - sh)) : lo;
+        vis = (below(r.ctx - 32 * blk) | nodes) & there;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!((vis >> (8 * (e >> 2) + 4 * h + (e & 3))) & 1)) sc[e] = kNegInfR;
+        bool bad = false;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (!((there >> (8 * (e >> 2) + 4 * h + (e & 3))) & 1)) vr[e] = VP{};  // unread rows
+#pragma unroll
+          for (int x = 0; x < NU / 2; ++x) bad |= nonfinite2<T>(word_of(vr[e], x)) != 0;
+        }
+        if (__any(bad)) {
+          // acc += for each row and dim, the infinities and NaN of the keys the
+          // row sees: P is 1 where it sees a key, V a flag where it is not
+          // finite; those elements then leave V.
+          constexpr uint32_t one = std::is_same<T, bf16_t>::value ? 0x3F80u : 0x3C00u;
+          u32x4 sees[2];
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const uint32_t b = vis >> (8 * (e >> 2) + 4 * h + (e & 3));
+            sees[e >> 3][(e & 7) >> 1] = (b & 1 ? one : 0u) | (b & 2 ? one << 16 : 0u);
+          }
+#pragma unroll
+          for (int x = 0; x < NU; ++x) {
+            f32x16 n;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) n[e] = 0.f;
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+              u32x4 f;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t w0 = word_of(vr[8 * s2 + 2 * k], x >> 1), w1 = word_of(vr[8 * s2 + 2 * k + 1], x >> 1);
+                f[k] = flag16<T>((x & 1 ? w0 >> 16 : w0) & 0xFFFFu) | flag16<T>((x & 1 ? w1 >> 16 : w1) & 0xFFFFu) << 16;
+              }
+              n = mfma_k16x32<T>(f, sees[s2], n);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[x][e] += flag_value(n[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            uint32_t w[NU / 2];
+#pragma unroll
+            for (int x = 0; x < NU / 2; ++x) {
+              w[x] = word_of(vr[e], x);
+              const uint32_t nf = nonfinite2<T>(w[x]);
+              w[x] &= (nf & 1 ? 0xFFFF0000u : ~0u) & (nf & 2 ? 0xFFFFu : ~0u);
+            }
+            if constexpr (NU == 4) vr[e] = u32x2{w[0], w[NU / 2 - 1]};
+            else vr[e] = w[0];
+          }
+        }
+      }
+      float mx = kNegInfR;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+      const float mt = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * cs;
+      if (__any(mt > m + kTreeRescale)) {
+        const float mn = fmaxf(m, mt), alpha = mn == kNegInfR ? 1.f : fast_exp2(m - mn);
+        l *= alpha;
+#pragma unroll
+        for (int x = 0; x < NU; ++x)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[x][e] *= alpha;
+        m = mn;
+      }
+      const float mu = m == kNegInfR ? 0.f : m;
+      u32x4 pop[2];
+      {
+        float p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          p[e] = fast_exp2(fmaf(sc[e], cs, -mu));
+          l += p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) pop[e >> 3][(e & 7) >> 1] = pack2<T>(p[e], p[e + 1]);
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int x = 0; x < NU; ++x) {
+          u32x4 w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = v_pair<T, T>(vr[8 * s2 + 2 * k], vr[8 * s2 + 2 * k + 1], x);
+          acc[x] = mfma_k16x32<T>(w, pop[s2], acc[x]);
+        }
+      load_v(more ? i + 1 : i);
+    }
+    l += __builtin_bit_cast(float, xor_lane32<32>(__builtin_bit_cast(uint32_t, l), lane));
+  }
+  // ---- The waves' partials to LDS, then the runs of keys together.
+  float* const slot = slots + (wave * 32 + c) * PF;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int i = 8 * (e >> 2) + 4 * h + (e & 3);
+    if constexpr (NU == 4) *reinterpret_cast<f32x4*>(slot + 4 * i) = f32x4{acc[0][e], acc[1][e], acc[2][e], acc[NU - 1][e]};
+    else *reinterpret_cast<f32x2*>(slot + 2 * i) = f32x2{acc[0][e], acc[1][e]};
+  }
+  if (h == 0) {
+    slot[D] = m;
+    slot[D + 1] = l;
+  }
+  __syncthreads();
+  for (int idx = tid; idx < rows * (D / 2); idx += 256) {
+    const int rr = idx / (D / 2), d = 2 * (idx - rr * (D / 2));
+    float M = kNegInfR, den = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int g = 0; g < KG; ++g) {
+      const float* const x = slots + (((rr >> 5) + RT * g) * 32 + (rr & 31)) * PF;
+      const f32x2 v = *reinterpret_cast<const f32x2*>(x + d), ml = *reinterpret_cast<const f32x2*>(x + D);
+      const float mn = fmaxf(M, ml[0]), mu = mn == kNegInfR ? 0.f : mn;
+      const float c_old = fast_exp2(M - mu), c_new = fast_exp2(ml[0] - mu);
+      o0 = fmaf(v[0], c_new, o0 * c_old);
+      o1 = fmaf(v[1], c_new, o1 * c_old);
+      den = fmaf(ml[1], c_new, den * c_old);
+      M = mn;
+    }
+    const int gr = row_first + rr;
+    if (a.S == 1) {
+      const int nd = gr / a.G;
+      T* const out = static_cast<T*>(a.out) + (r.row0 + nd) * a.o_sr + (kvh * a.G + gr - nd * a.G) * a.o_sh;
+      out[d * a.o_sd] = from_float<T>(den == 0.f ? 0.f : o0 / den);
+      out[(d + 1) * a.o_sd] = from_float<T>(den == 0.f ? 0.f : o1 / den);
+    } else {
+      float* const out = part + ((static_cast<int64_t>(u) * a.S + sp) * (a.T * a.G) + gr) * PF;
+      *reinterpret_cast<f32x2*>(out + d) = f32x2{o0, o1};
+      if (d == 0) *reinterpret_cast<f32x2*>(out + D) = f32x2{M, den};
+    }
+  }
+}
+
+}  // namespace tsa

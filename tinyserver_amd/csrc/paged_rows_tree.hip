@@ -1,0 +1,47 @@
+// Instances, plan and launch of the tree kernel (paged_rows_tree.h).
+#include "paged_rows_tree.h"
+
+namespace tsa {
+
+#ifndef TSA_TREE_WGS
+#define TSA_TREE_WGS 1024
+#endif
+#ifndef TSA_TREE_MIN_SPLIT
+#define TSA_TREE_MIN_SPLIT 16
+#endif
+
+TreeRowsPlan tree_rows_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap) {
+  TreeRowsPlan p{};
+  const int64_t rows = T * (Hq / Hkv), blocks = (cap + 31) / 32;
+  p.RT = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  p.RB = static_cast<int>((rows + 32 * p.RT - 1) / (32 * p.RT));
+  const int64_t wgs = B * Hkv * p.RB;
+  int64_t S = (TSA_TREE_WGS + wgs - 1) / wgs;
+  const int64_t most = (blocks + TSA_TREE_MIN_SPLIT - 1) / TSA_TREE_MIN_SPLIT;
+  S = S < most ? S : most;
+  S = S < 1 ? 1 : S;
+  const int64_t per = ((blocks + S - 1) / S + 3) / 4 * 4;
+  p.per_split = static_cast<int>(per < 4 ? 4 : per);
+  p.S = static_cast<int>((blocks + p.per_split - 1) / p.per_split);
+  if (p.S < 1) p.S = 1;
+  p.bytes = p.S == 1 ? 0 : static_cast<size_t>(B * Hkv * p.S) * static_cast<size_t>(rows) * (D + 4) * sizeof(float);
+  return p;
+}
+
+template <typename T, int D>
+static int launch_tree(const RowsArgs& a, hipStream_t stream) {
+  const int64_t us = int64_t{a.B} * a.Hkv * a.S;
+  paged_rows_tree<T, D><<<dim3(static_cast<uint32_t>((us + 7) / 8 * 8 * a.RB)), dim3(256), 0, stream>>>(a, a.bt, a.mask, a.part);
+  if (int rc = check_launch("tsa_paged_tree")) return rc;
+  if (a.S == 1) return TSA_OK;
+  constexpr int RW = 64 / (D / 4);
+  paged_rows_merge<T, D><<<dim3(a.B * a.Hkv, (a.T * a.G + RW - 1) / RW), dim3(256), 0, stream>>>(a, a.lens, a.part, a.per_split);
+  return check_launch("tsa_paged_tree");
+}
+
+int rows_tree_launch(const RowsArgs& a, int dt, hipStream_t stream) {
+  if (dt == TSA_BF16) return a.D == 128 ? launch_tree<bf16_t, 128>(a, stream) : launch_tree<bf16_t, 64>(a, stream);
+  return a.D == 128 ? launch_tree<f16_t, 128>(a, stream) : launch_tree<f16_t, 64>(a, stream);
+}
+
+}  // namespace tsa
