@@ -1,5 +1,6 @@
-// Instances, plan and launch of the tree kernel (paged_rows_tree.h).
-#include "paged_rows_tree.h"
+// Instances, plan and launch of the tree kernels (paged_rows_tree.h,
+// paged_rows_tree_lds.h).
+#include "paged_rows_tree_lds.h"
 
 namespace tsa {
 
@@ -19,6 +20,8 @@ TreeRowsPlan tree_rows_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64
   int64_t S = (TSA_TREE_WGS + wgs - 1) / wgs;
   const int64_t most = (blocks + TSA_TREE_MIN_SPLIT - 1) / TSA_TREE_MIN_SPLIT;
   S = S < most ? S : most;
+  const int64_t least = (blocks + kTreeMaxSplit - 1) / kTreeMaxSplit;
+  S = S < least ? least : S;
   S = S < 1 ? 1 : S;
   const int64_t per = ((blocks + S - 1) / S + 3) / 4 * 4;
   p.per_split = static_cast<int>(per < 4 ? 4 : per);
@@ -27,11 +30,15 @@ TreeRowsPlan tree_rows_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64
   p.bytes = p.S == 1 ? 0 : static_cast<size_t>(B * Hkv * p.S) * static_cast<size_t>(rows) * (D + 4) * sizeof(float);
   return p;
 }
+static_assert(kTreeMaxSplit % 4 == 0, "a split rounded up to four blocks still fits its table");
 
 template <typename T, int D>
 static int launch_tree(const RowsArgs& a, hipStream_t stream) {
   const int64_t us = int64_t{a.B} * a.Hkv * a.S;
-  paged_rows_tree<T, D><<<dim3(static_cast<uint32_t>((us + 7) / 8 * 8 * a.RB)), dim3(256), 0, stream>>>(a, a.bt, a.mask, a.part);
+  const dim3 grid(static_cast<uint32_t>((us + 7) / 8 * 8 * a.RB));
+  if (a.RT == 1) paged_rows_tree<T, D><<<grid, dim3(256), 0, stream>>>(a, a.bt, a.mask, a.part);
+  else if (a.RT == 2) paged_rows_tree_lds<T, D, 2><<<grid, dim3(128), 0, stream>>>(a, a.bt, a.mask, a.part);
+  else paged_rows_tree_lds<T, D, 4><<<grid, dim3(256), 0, stream>>>(a, a.bt, a.mask, a.part);
   if (int rc = check_launch("tsa_paged_tree")) return rc;
   if (a.S == 1) return TSA_OK;
   constexpr int RW = 64 / (D / 4);
