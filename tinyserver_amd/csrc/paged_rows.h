@@ -33,6 +33,7 @@ struct RowsArgs {
   int32_t sinks;      // the first tokens that stay visible
   int32_t S;          // splits of a unit's tokens (0: the stream)
   int32_t NW;         // waves of the stream
+  int32_t out8;       // output rows are unit-stride, in 8-byte pieces
   int32_t RT, RB, per_split;  // trees: 32-row tiles of a workgroup, row blocks of a unit, 32-key blocks of a split
   // The matrix-core forms: page strides in bytes, and the tiles (16 tokens) of a
   // page as a multiplier and a shift (tiles_of_page).

@@ -193,7 +193,7 @@ int check_rows(const tsa_view* out, const tsa_view* query, const tsa_view* k_cac
 // The matrix-core forms: 16-bit queries, head_dim 64 or 128, pages of whole
 // 16-token tiles, unit-stride rows of 16-byte pieces, and strides whose offsets
 // within a page fit 31 bits (a page's own 32). Fills what they need of a.
-static bool takes_mfma(RowsArgs& a, const tsa_view* query, const tsa_view* k_cache, const tsa_view* v_cache) {
+static bool takes_mfma(RowsArgs& a, const tsa_view* out, const tsa_view* query, const tsa_view* k_cache, const tsa_view* v_cache) {
   if ((query->dtype != TSA_BF16 && query->dtype != TSA_F16) || (a.D != 64 && a.D != 128) || a.BS % 16 || a.NB == 0)
     return false;
   if (!rows_vec16(query) || !rows_vec16(k_cache) || !rows_vec16(v_cache)) return false;
@@ -207,6 +207,7 @@ static bool takes_mfma(RowsArgs& a, const tsa_view* query, const tsa_view* k_cac
   a.v_page = static_cast<uint32_t>(a.vc_b * eb);
   a.ks_page = static_cast<uint32_t>(a.ks_b * 4);
   a.vs_page = static_cast<uint32_t>(a.vs_b * 4);
+  a.out8 = a.o_sd == 1 && a.o_sr % 4 == 0 && a.o_sh % 4 == 0 && reinterpret_cast<uintptr_t>(out->data) % 8 == 0;
   set_page_div(a);
   return true;
 }
@@ -243,7 +244,7 @@ extern "C" int tsa_paged_decode_window(const tsa_view* out, const tsa_view* quer
   if (int rc = check_rows(out, query, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens, nullptr, nullptr, 0,
                           window, sinks, softmax_scale, a))
     return rc;
-  if (a.B > 0 && a.Hq > 0 && takes_mfma(a, query, k_cache, v_cache)) {
+  if (a.B > 0 && a.Hq > 0 && takes_mfma(a, out, query, k_cache, v_cache)) {
     const DecodeRowsPlan p = decode_rows_plan(a.B, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS, a.window, a.sinks,
                                               a.ks != nullptr);
     TSA_REQUIRE(p.total == 0 || (workspace != nullptr && workspace_bytes >= p.total),
@@ -269,7 +270,7 @@ extern "C" int tsa_paged_tree(const tsa_view* out, const tsa_view* query, const 
   if (int rc = check_rows(out, query, k_cache, v_cache, nullptr, nullptr, block_tables, context_lens, cu_nodes,
                           tree_mask, max_nodes, 0, 0, softmax_scale, a))
     return rc;
-  if (a.B > 0 && a.Hq > 0 && a.T > 0 && a.N > 0 && a.scale_log2 > 0.f && takes_mfma(a, query, k_cache, v_cache)) {
+  if (a.B > 0 && a.Hq > 0 && a.T > 0 && a.N > 0 && a.scale_log2 > 0.f && takes_mfma(a, out, query, k_cache, v_cache)) {
     const TreeRowsPlan p = tree_rows_plan(a.B, a.T, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS);
     if (int64_t{a.B} * a.Hkv * p.S * p.RB < (int64_t{1} << 23)) {  // (a launch's threads fit 32 bits)
       TSA_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes),

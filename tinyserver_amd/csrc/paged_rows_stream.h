@@ -439,8 +439,16 @@ __global__ __launch_bounds__(256) void paged_rows_stream_merge(RowsArgs a, const
     take(x[D], x[D + 1], *reinterpret_cast<const f32x4*>(x + d));
   }
   T* const out = static_cast<T*>(a.out) + s * a.o_sr + (kvh * a.G + g0 + row) * a.o_sh;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  if (a.out8) {
+    u32x2 w;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[(d + e) * a.o_sd] = from_float<T>(den == 0.f ? 0.f : o[e] / den);
+    for (int i = 0; i < 2; ++i) w[i] = den == 0.f ? 0u : pack2<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
+    *reinterpret_cast<u32x2*>(out + d) = w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[(d + e) * a.o_sd] = from_float<T>(den == 0.f ? 0.f : o[e] * inv);
+  }
 }
 
 }  // namespace tsa

@@ -5,7 +5,7 @@
 namespace tsa {
 
 #ifndef TSA_TREE_WGS
-#define TSA_TREE_WGS 1024
+#define TSA_TREE_WGS 512
 #endif
 #ifndef TSA_TREE_MIN_SPLIT
 #define TSA_TREE_MIN_SPLIT 16
@@ -41,8 +41,7 @@ static int launch_tree(const RowsArgs& a, hipStream_t stream) {
   else paged_rows_tree_lds<T, D, 4><<<grid, dim3(256), 0, stream>>>(a, a.bt, a.mask, a.part);
   if (int rc = check_launch("tsa_paged_tree")) return rc;
   if (a.S == 1) return TSA_OK;
-  constexpr int RW = 64 / (D / 4);
-  paged_rows_merge<T, D><<<dim3(a.B * a.Hkv, (a.T * a.G + RW - 1) / RW), dim3(256), 0, stream>>>(a, a.lens, a.part, a.per_split);
+  launch_rows_merge<T, D>(a, a.T * a.G, a.per_split, stream);
   return check_launch("tsa_paged_tree");
 }
 

@@ -362,8 +362,18 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll
     for (int x = 0; x < NU; ++x)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        out[(32 * x + 8 * (e >> 2) + 4 * h + (e & 3)) * a.o_sd] = from_float<T>(l == 0.f ? 0.f : acc[x][e] * inv);
+      for (int e = 0; e < 16; e += 4) {
+        const int d = 32 * x + 8 * (e >> 2) + 4 * h;
+        u32x2 w = {pack2<T>(acc[x][e] * inv, acc[x][e + 1] * inv), pack2<T>(acc[x][e + 2] * inv, acc[x][e + 3] * inv)};
+        if (l == 0.f) w = u32x2{0, 0};
+        if (a.out8) {
+          *reinterpret_cast<u32x2*>(out + d) = w;
+        } else {
+          uint16_t* const o16 = reinterpret_cast<uint16_t*>(out);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o16[(d + i) * a.o_sd] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+        }
+      }
   } else {
     float* const out = part + ((static_cast<int64_t>(u) * a.S + sp) * (a.T * a.G) + row) * PF;
 #pragma unroll

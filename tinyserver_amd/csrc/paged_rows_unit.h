@@ -323,15 +323,17 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   }
 }
 
-// Outputs from the partials of a unit's splits, in order of the splits: a wave
-// takes a quarter of them in batches whose loads are issued together (past the
-// last: repeated and dropped), 4 dims a lane, 64 / (D / 4) rows a workgroup;
-// then the quarters in order. Grid: units x row groups.
-template <typename T, int D>
+// Outputs from the partials of a unit's splits, 4 dims a lane, 64 / (D / 4) rows
+// a wave. Few rows with many splits (SHARE): the four waves of a workgroup take
+// the same rows, a quarter of the splits each, then the quarters in order; else
+// each wave takes rows of its own and all their splits. Splits go in batches
+// whose loads are issued together (past the last: repeated and dropped). Grid:
+// units x row groups.
+template <typename T, int D, bool SHARE>
 __global__ __launch_bounds__(256) void paged_rows_merge(RowsArgs a, const int32_t* __restrict__ lens,
                                                         const float* __restrict__ part, int tiles_per_split) {
-  constexpr int LR = D / 4, RW = 64 / LR, PF = part_floats(D);
-  __shared__ float red[4][RW][D + 2];
+  constexpr int LR = D / 4, RW = 64 / LR, PF = part_floats(D), kBatch = SHARE ? 8 : 4;
+  __shared__ __align__(16) float red[SHARE ? 4 : 1][RW][PF];
   const int u = blockIdx.x, s = u / a.Hkv, kvh = u - s * a.Hkv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int n;  // splits with tiles
@@ -348,14 +350,17 @@ __global__ __launch_bounds__(256) void paged_rows_merge(RowsArgs a, const int32_
     nrows = a.G;
   }
   const int all_rows = a.T * a.G;
-  const int row = static_cast<int>(blockIdx.y) * RW + lane / LR, d = 4 * (lane % LR);
-  if (static_cast<int>(blockIdx.y) * RW >= nrows) return;
+  const int group = SHARE ? static_cast<int>(blockIdx.y) : 4 * static_cast<int>(blockIdx.y) + wave;
+  const int row = group * RW + lane / LR, d = 4 * (lane % LR);
+  if (group * RW >= nrows) return;
   const int rr = min(row, nrows - 1);
-  const int per = (n + 3) / 4, first = min(n, wave * per), last = min(n, first + per);
+  const int per = SHARE ? (n + 3) / 4 : n;
+  const int first = SHARE ? min(n, wave * per) : 0, last = SHARE ? min(n, first + per) : n;
   const float* const base = part + (static_cast<int64_t>(u) * a.S * all_rows + rr) * PF;
   const int64_t step = static_cast<int64_t>(all_rows) * PF;
-  float M = kNegInfR, den = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  auto take = [&](float m, float l, const float (&x)[4]) {
+  float M = kNegInfR, den = 0.f;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto take = [&](float m, float l, f32x4 x) {
     const float mn = fmaxf(M, m), mu = mn == kNegInfR ? 0.f : mn;
     const float c_old = fast_exp2(M - mu), c_new = fast_exp2(m - mu);
 #pragma unroll
@@ -363,42 +368,59 @@ __global__ __launch_bounds__(256) void paged_rows_merge(RowsArgs a, const int32_
     den = fmaf(l, c_new, den * c_old);
     M = mn;
   };
-  for (int sp = first; sp < last; sp += 8) {
-    f32x4 po[8];
-    f32x2 ml[8];
+  for (int sp = first; sp < last; sp += kBatch) {
+    f32x4 po[kBatch];
+    f32x2 ml[kBatch];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < kBatch; ++k) {
       const float* const x = base + min(sp + k, last - 1) * step;
       po[k] = *reinterpret_cast<const f32x4*>(x + d);
       ml[k] = *reinterpret_cast<const f32x2*>(x + D);
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (sp + k < last) {
-        const float x[4] = {po[k][0], po[k][1], po[k][2], po[k][3]};
-        take(ml[k][0], ml[k][1], x);
-      }
+    for (int k = 0; k < kBatch; ++k)
+      if (sp + k < last) take(ml[k][0], ml[k][1], po[k]);
   }
-  float* const mine = red[wave][lane / LR];
+  if constexpr (SHARE) {
+    float* const mine = red[wave][lane / LR];
+    *reinterpret_cast<f32x4*>(mine + d) = o;
+    if (d == 0) {
+      mine[D] = M;
+      mine[D + 1] = den;
+    }
+    __syncthreads();
+    if (wave > 0) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) mine[d + i] = o[i];
-  if (d == 0) {
-    mine[D] = M;
-    mine[D + 1] = den;
+    for (int w = 1; w < 4; ++w) {
+      const float* const x = red[w][lane / LR];
+      take(x[D], x[D + 1], *reinterpret_cast<const f32x4*>(x + d));
+    }
   }
-  __syncthreads();
-  if (wave > 0 || row >= nrows) return;
-#pragma unroll
-  for (int w = 1; w < 4; ++w) {
-    const float* const x = red[w][lane / LR];
-    const float v[4] = {x[d], x[d + 1], x[d + 2], x[d + 3]};
-    take(x[D], x[D + 1], v);
-  }
+  if (row >= nrows) return;
   const int node = row / a.G;
   T* const out = static_cast<T*>(a.out) + (row0 + node) * a.o_sr + (kvh * a.G + row - node * a.G) * a.o_sh;
-  const float r = den == 0.f ? 0.f : 1.f;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  if (a.out8) {
+    u32x2 w;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) out[(d + i) * a.o_sd] = from_float<T>(r == 0.f ? 0.f : o[i] / den);
+    for (int i = 0; i < 2; ++i) w[i] = den == 0.f ? 0u : pack2<T>(o[2 * i] * inv, o[2 * i + 1] * inv);
+    *reinterpret_cast<u32x2*>(out + d) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[(d + i) * a.o_sd] = from_float<T>(den == 0.f ? 0.f : o[i] * inv);
+  }
+}
+
+// Splits from which the waves of the merge share rows.
+constexpr int kMergeShare = 6;
+template <typename T, int D>
+inline void launch_rows_merge(const RowsArgs& a, int rows, int tiles_per_split, hipStream_t stream) {
+  constexpr int RW = 64 / (D / 4);
+  const int groups = (rows + RW - 1) / RW;
+  if (a.S >= kMergeShare)
+    paged_rows_merge<T, D, true><<<dim3(a.B * a.Hkv, groups), dim3(256), 0, stream>>>(a, a.lens, a.part, tiles_per_split);
+  else
+    paged_rows_merge<T, D, false><<<dim3(a.B * a.Hkv, (groups + 3) / 4), dim3(256), 0, stream>>>(a, a.lens, a.part, tiles_per_split);
 }
 
 }  // namespace tsa

@@ -38,9 +38,7 @@ static int launch_unit(const RowsArgs& a, hipStream_t stream, const char* what) 
   else
     paged_rows_unit<T, C, D, kUnitWavesSplit, false><<<grid, threads, kUnitWavesSplit * row_bytes, stream>>>(a, a.bt, a.lens, a.part);
   if (int rc = check_launch(what)) return rc;
-  constexpr int RW = 64 / (D / 4);
-  paged_rows_merge<T, D><<<dim3(a.B * a.Hkv, (a.G + RW - 1) / RW), dim3(256), 0, stream>>>(
-      a, a.lens, a.part, kUnitWavesSplit * kUnitTiles<C>);
+  launch_rows_merge<T, D>(a, a.G, kUnitWavesSplit * kUnitTiles<C>, stream);
   return check_launch(what);
 }
 
