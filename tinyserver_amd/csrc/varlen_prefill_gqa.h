@@ -7,6 +7,7 @@
 #pragma once
 
 #include <cmath>
+#include <type_traits>
 
 #include "tsa_common.h"
 
@@ -26,6 +27,43 @@ struct PrefillArgs {
   int32_t causal;
   float scale_log2;
 };
+
+// With a sliding window and first tokens (tsa_varlen_prefill_window): query i
+// sees the keys j <= i with j > i - window or j < sinks. The kernels that take
+// both argument blocks tell them apart by this type (kWindow<Args>).
+struct PrefillWindowArgs : PrefillArgs {
+  int32_t window;  // at least 1
+  int32_t sinks;
+};
+template <typename Args> constexpr bool kWindow = std::is_same<Args, PrefillWindowArgs>::value;
+
+// The key blocks (of 32) that queries [q0, q1) see: `first` blocks of the first
+// tokens, then `count - first` from block w0 on, where the first query's window
+// starts, to the causal end. Block v of this list is block at(v) of the keys.
+struct WindowBlocks {
+  int first, skip, count, end;  // end: past the last key of the last block
+  __device__ __forceinline__ int at(int v) const { return v < first ? v : v + skip; }
+};
+__device__ __forceinline__ WindowBlocks window_blocks(const PrefillWindowArgs& a, int q0, int q1, int k_len) {
+  WindowBlocks b;
+  const int w0 = (q0 + 1 > a.window ? q0 + 1 - a.window : 0) >> 5;
+  const int near = ((min(k_len, q1) + 31) >> 5) - w0, sinks = (min(a.sinks, k_len) + 31) >> 5;
+  b.first = min(sinks, w0);
+  b.skip = w0 - b.first;
+  b.count = b.first + max(near, 0);
+  b.end = near > 0 ? 32 * (w0 + near) : 32 * b.first;
+  return b;
+}
+// Whether the 32 queries from q on see all of the 32 keys from k on (none past
+// k_len).
+__device__ __forceinline__ bool window_sees_all(const PrefillWindowArgs& a, int q, int k, int k_len) {
+  return k + 31 <= q && k + 32 <= k_len && (k >= q + 32 - a.window || k + 32 <= a.sinks);
+}
+// The keys k + i, i < 32, that query q sees, as bits.
+__device__ __forceinline__ uint32_t window_bits(const PrefillWindowArgs& a, int q, int k, int k_len) {
+  auto below = [](int n) { return n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u; };
+  return below(min(q + 1, k_len) - k) & (~below(q + 1 - a.window - k) | below(a.sinks - k));
+}
 
 // varlen_prefill_f32.hip: the float32 kernel, and the calls it takes (of those
 // prefill_prepare marks mfma).
@@ -47,6 +85,11 @@ __device__ __forceinline__ void seq_range(const int32_t* cu, int64_t stride, int
   start = s0;
   len = s1 - s0;
 }
+
+// varlen_prefill_window.h: one row, over the keys it sees.
+template <typename T>
+__device__ void prefill_window_row(const PrefillWindowArgs& a, int64_t qi, int64_t qq, int h, int64_t k_start,
+                                   int64_t k_len);
 
 // The work-item plan: up to kPlanItems item descriptors of a workgroup (6
 // int32 each), computed kPlanItems at a time, and the level table (items
@@ -96,8 +139,16 @@ constexpr int gqa_smem_bytes() {
 // QS > 1: an item is 32 QS queries, and the workgroup's NW waves take NW / QS
 // q-heads (the group) of QS blocks of 32 queries each, wave w head w % (NW /
 // QS) of block w / (NW / QS).
-template <typename T, int D, int NW, int QS = 1>
-__device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* __restrict__ cu_q,
+// With PrefillWindowArgs an item's blocks are those that its queries see
+// (window_blocks). Its masked blocks -- at the diagonal, at the window's low end,
+// at the first tokens' end -- may hold infinities or NaN in rows of V that a
+// query does not see, and 0 times those is NaN: a wave whose sums are not all
+// finite at an item's end computes its 32 rows again one by one
+// (prefill_window_row), over visible keys alone, in place of storing them. (A
+// test of V in those blocks instead took 16 prompts of 128-2048 tokens, window
+// 512, 32/8 heads, from 381 to 402 us.)
+template <typename T, int D, int NW, int QS = 1, typename Args = PrefillArgs>
+__device__ __forceinline__ void prefill_gqa_body(Args a, const int32_t* __restrict__ cu_q,
                                                  const int32_t* __restrict__ cu_k, char* smem, int wg_base) {
   constexpr int KJ = D / 16;              // 16-dim steps of the QK reduction
   constexpr int NU = D / 32;              // 32-dim column tiles of the output
@@ -168,6 +219,20 @@ __device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* _
     int64_t q_start;
     const T* kb;
     const T* vb;
+    WindowBlocks win;  // (window) the blocks; k_start: the sequence's first key
+    int64_t k_start;
+  };
+  // (window) The item's blocks, in place of the causal range.
+  auto set_window = [&](Item& it, int q_last) __attribute__((always_inline)) {
+    if constexpr (kWindow<Args>) {
+      it.win = window_blocks(a, it.q0, q_last, it.k_len);
+      it.nblk = it.win.count;
+      it.kfull = min(it.k_len, it.win.end);
+    }
+  };
+  auto block_at = [&](const Item& it, int v) __attribute__((always_inline)) {
+    if constexpr (kWindow<Args>) return it.win.at(v);
+    else return v;
   };
   // Item i -> its level (the smallest Q with items_above(Q) <= i), then the
   // sequence of rank (i - items_above(Q)) / Hkv among those with nqb > Q.
@@ -208,6 +273,8 @@ __device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* _
     it.nblk = (kend + 31) / 32;
     it.jm = a.causal ? min(it.k_len / 32, Q * QS + my_blk) : it.k_len / 32;
     it.kfull = min(it.k_len, it.nblk * 32);
+    set_window(it, q_last);
+    if constexpr (kWindow<Args>) it.k_start = ks;
     it.kb = static_cast<const T*>(a.k) + ks * a.k_st + it.kvh * a.k_sh;
     it.vb = static_cast<const T*>(a.v) + ks * a.v_st + it.kvh * a.v_sh;
   };
@@ -282,6 +349,8 @@ __device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* _
     it.nblk = (kend + 31) / 32;
     it.jm = a.causal ? min(it.k_len / 32, Q * QS + my_blk) : it.k_len / 32;
     it.kfull = min(it.k_len, it.nblk * 32);
+    set_window(it, q_last);
+    if constexpr (kWindow<Args>) it.k_start = ks;
     it.kb = static_cast<const T*>(a.k) + ks * a.k_st + it.kvh * a.k_sh;
     it.vb = static_cast<const T*>(a.v) + ks * a.v_st + it.kvh * a.v_sh;
   };
@@ -337,7 +406,7 @@ __device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* _
   };
   // This wave's loads of block blk of item `it` (K if k_wave) into slot `slot`.
   auto load_block = [&](const Item& it, int blk, int slot) __attribute__((always_inline)) {
-    const int key0 = min(blk, it.nblk - 1) * 32 + row0w;
+    const int key0 = block_at(it, min(blk, it.nblk - 1)) * 32 + row0w;
     const int lds0 = (k_wave ? 0 : VOFF) + slot * BLKB + row0w * RB;
     const char* gbase = reinterpret_cast<const char*>(k_wave ? it.kb : it.vb);
     if (key0 + IPW * RPI <= it.k_len) {
@@ -390,6 +459,11 @@ __device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* _
   auto load_step_c = [&](const Item& it, int j, auto S) __attribute__((always_inline)) {
     constexpr int s = decltype(S)::value;
     const int lds0 = (k_wave ? s * BLKB : VOFF + ((s + NB - 1) % NB) * BLKB) + row0w * RB;
+    if constexpr (kWindow<Args>) {  // (the blocks are two runs: their place is computed)
+      const int v = j + A + (k_wave ? 1 : 0);
+      rk = v < it.nblk ? 32 * it.win.at(v) + row0w : it.kfull;
+      rp = reinterpret_cast<const char*>(k_wave ? it.kb : it.vb) + rk * st_b;
+    }
     if (rk + IPW * RPI <= it.kfull) {
 #pragma unroll
       for (int i = 0; i < IPW; ++i) dma(rp, doffs[i], lds0 + i * 1024);
@@ -443,7 +517,17 @@ __device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* _
   // Keys past k_len, and (causal) keys after the query, only occur in a
   // sequence's last block or on the diagonal: a wave-uniform branch.
   auto mask_block = [&](const Item& it, f32x16& sc, int blk) {
-    const int kb0 = blk * 32;
+    const int kb0 = block_at(it, blk) * 32;
+    if constexpr (kWindow<Args>) {
+      const int qw = it.q0 + 32 * my_blk;
+      if (!window_sees_all(a, qw, kb0, it.k_len)) {
+        const uint32_t bits = window_bits(a, qw + c, kb0, it.k_len) >> (4 * h);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!(bits & (1u << (8 * (e >> 2) + (e & 3))))) sc[e] = kNegInfP;
+      }
+      return;
+    }
     if (blk >= it.jm) {
       const int qq = it.q0 + 32 * my_blk + c;
 #pragma unroll
@@ -590,7 +674,8 @@ __device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* _
   // which keeps a wave's writes within two-way bank conflicts.
   char* const ost = smem + OOFF + wave * kOutStage;
   auto store_out = [&](const Item& it) {
-    const float rl = 1.f / (l + __shfl_xor(l, 32, 64));  // 1 / query c's denominator
+    const float den = l + __shfl_xor(l, 32, 64);
+    const float rl = kWindow<Args> && den == 0.f ? 0.f : 1.f / den;  // 1 / query c's denominator (window: nothing seen, 0)
     T* const obase = static_cast<T*>(a.out) + it.q_start * a.o_st + (it.kvh * HG + my_head) * a.o_sh;
     const int wsw = (c >> 2) & 3;
 #pragma unroll
@@ -703,7 +788,7 @@ __device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* _
       rescale(block_max(sca));
       softmax_exp(sca);
       vread(j % NB);
-    }
+      }
     // The next item's blocks go to slots 0 .. A: every wave must have read
     // X's last V block (whichever slot it is in) before they are issued.
     lds_barrier();
@@ -711,8 +796,25 @@ __device__ __forceinline__ void prefill_gqa_body(PrefillArgs a, const int32_t* _
     // (QS > 1: the item's last block can lie wholly after an earlier query block,
     // whose wave leaves it out: its weights there are 0, but 0 times an infinity
     // or NaN in V is NaN. So a bad V row reaches queries of its own 32 alone.)
-    if (X.nblk > 0 && !(QS > 1 && a.causal && 32 * j > X.q0 + 32 * my_blk)) pv();
-    store_out(X);
+    if constexpr (kWindow<Args>) {
+      if (X.nblk > 0) pv();
+      float sum = 0.f * l;  // NaN where anything is not finite
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum = fmaf(acc[u][e], 0.f, sum);
+      if (__any(sum != 0.f)) {  // (uniform)
+        const int qw = X.q0 + 32 * my_blk, last = min(X.q_len, qw + 32);
+#pragma unroll 1
+        for (int qq = qw; qq < last; ++qq)
+          prefill_window_row<T>(a, X.q_start + qq, qq, X.kvh * HG + my_head, X.k_start, X.k_len);
+      } else {
+        store_out(X);
+      }
+    } else {
+      if (X.nblk > 0 && !(QS > 1 && a.causal && 32 * j > X.q0 + 32 * my_blk)) pv();
+      store_out(X);
+    }
     X = Y;
     idx = nidx;
   }
@@ -729,8 +831,31 @@ int prefill_prepare(const tsa_view* out, const tsa_view* q, const tsa_view* k, c
                     int64_t max_seqlen_k, int32_t causal, double softmax_scale, PrefillArgs& a, bool& mfma);
 int prefill_launch(PrefillArgs& a, bool mfma, int dtype, int64_t max_seqlen_q, hipStream_t stream);
 bool prefill_takes_gqa4(const PrefillArgs& a, bool mfma);
-// varlen_prefill_w64.hip: its launch (bf16 or f16) and its sequence limit.
+// The LDS-staged kernels keep 32 rows of K/V byte offsets in 32 bits, and
+// per-sequence query-block counts in 16 bits (every sequence's length is at
+// most total_q). Both need a positive scale (the masked-score sentinel).
+constexpr int64_t kMaxStride = int64_t{1} << 24;
+// varlen_prefill_w64 and its windowed form: head_dim 128, groups of a multiple of
+// 4 q-heads, its per-sequence tile counts in LDS, 16-bit tile counts.
 constexpr int kW64MaxSeqsHost = 2048;
+inline bool prefill_takes_w64(const PrefillArgs& a) {
+  return a.D == 128 && a.G % 4 == 0 && a.scale_log2 > 0.f && a.q_st < kMaxStride && a.k_st < kMaxStride &&
+         a.v_st < kMaxStride && a.nseq <= kW64MaxSeqsHost && a.total_q <= int64_t{65535} * 64 &&
+         a.Hkv * (a.G / 4) < 32768;
+}
+inline bool prefill_takes_gqa(const PrefillArgs& a) {
+  return (a.G == 2 || a.G == 4 || a.G == 8) && a.scale_log2 > 0.f && a.k_st < kMaxStride && a.v_st < kMaxStride &&
+         a.nseq <= max_persist_seqs(a.G) && a.total_q <= int64_t{65535} * 32;
+}
+// Groups of two q-heads: whether items are pairs of query blocks (QS = 2). The
+// sides of both bounds are measured where the launch takes them.
+constexpr int64_t kPairMeanLen = 384;
+constexpr int64_t kPairItems = 352;
+inline bool prefill_pairs(const PrefillArgs& a) {
+  return a.G == 2 && a.total_q >= kPairMeanLen * a.nseq && a.total_q * a.Hkv >= kPairItems * 32;
+}
+// varlen_prefill_w64.hip: the launches (bf16 or f16).
+int prefill_w64_window_launch(const PrefillWindowArgs& a, bool bf16, hipStream_t stream);
 int prefill_w64_launch(const PrefillArgs& a, bool bf16, hipStream_t stream);
 bool prefill_w64_enabled();
 

@@ -1,0 +1,183 @@
+// Prefill attention for GQA groups that the LDS-staged kernel does not take:
+// four q-heads a workgroup, 32 queries a wave, operands straight from global
+// memory, 16x16x32 tiles. Args: PrefillArgs, or PrefillWindowArgs for a sliding
+// window with first tokens.
+#pragma once
+
+#include "varlen_prefill_gqa.h"
+
+namespace tsa {
+
+template <typename T, int D, typename Args>
+__global__ __launch_bounds__(256) void varlen_prefill_mfma(Args a) {
+  constexpr int KJ = D / 32;
+  const int qb = a.nqb - 1 - static_cast<int>(blockIdx.x);  // heaviest blocks first
+  const int b = blockIdx.y;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int h = blockIdx.z * 4 + wave;
+  int64_t q_start, q_len, k_start, k_len;
+  seq_range(a.cu_q, a.cuq_s, b, a.total_q, q_start, q_len);
+  seq_range(a.cu_k, a.cuk_s, b, a.total_k, k_start, k_len);
+  const int64_t row0 = static_cast<int64_t>(qb) * 32;
+  if (row0 >= q_len || h >= a.Hq) return;
+  const int kvh = h / a.G;
+
+  const T* qb_ptr = static_cast<const T*>(a.q) + q_start * a.q_st + h * a.q_sh;
+  const T* kb_ptr = static_cast<const T*>(a.k) + k_start * a.k_st + kvh * a.k_sh;
+  const T* vb_ptr = static_cast<const T*>(a.v) + k_start * a.v_st + kvh * a.v_sh;
+  const bool v_lane = 8 * c < D;
+
+  // Q^T operands of the two 16-row subtiles.
+  u32x4 qop[2][KJ];
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs) {
+    const int64_t row = row0 + 16 * qs + c;
+#pragma unroll
+    for (int j = 0; j < KJ; ++j)
+      qop[qs][j] = row < q_len ? *reinterpret_cast<const u32x4*>(qb_ptr + row * a.q_st + 8 * (g + 4 * j))
+                               : u32x4{0, 0, 0, 0};
+  }
+
+  float m[2] = {kNegInfP, kNegInfP};  // running max of query (16 qs + c), log2 domain
+  float l[2] = {0.f, 0.f};            // lane share of its denominator (fp32 p)
+  f32x4 acc[2][8];
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+    for (int u = 0; u < 8; ++u) acc[qs][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // The 32-key blocks from 0 to kend, or (window) those of the two runs.
+  int64_t kend = a.causal ? (k_len < row0 + 32 ? k_len : row0 + 32) : k_len;
+  WindowBlocks win{};
+  if constexpr (kWindow<Args>) {
+    win = window_blocks(a, static_cast<int>(row0), static_cast<int>(q_len < row0 + 32 ? q_len : row0 + 32),
+                        static_cast<int>(k_len));
+    kend = 32 * static_cast<int64_t>(win.count);
+  }
+  for (int64_t kv0 = 0; kv0 < kend; kv0 += 32) {
+    const int64_t kb0 = kWindow<Args> ? 32 * static_cast<int64_t>(win.at(static_cast<int>(kv0 >> 5))) : kv0;
+    u32x4 kop[2][KJ];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const int64_t key = kb0 + 16 * ks + c;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+        kop[ks][j] = key < k_len ? *reinterpret_cast<const u32x4*>(kb_ptr + key * a.k_st + 8 * (g + 4 * j))
+                                 : u32x4{0, 0, 0, 0};
+    }
+    u32x4 vrow[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t key = kb0 + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
+      vrow[e] = (v_lane && key < k_len) ? *reinterpret_cast<const u32x4*>(vb_ptr + key * a.v_st + 8 * c)
+                                        : u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs) {
+      const int64_t qq = row0 + 16 * qs + c;
+      float sv[2][4];
+      float tmax = kNegInfP;
+      uint32_t seen = 0;
+      if constexpr (kWindow<Args>)
+        seen = window_bits(a, static_cast<int>(qq), static_cast<int>(kb0), static_cast<int>(k_len)) >> (4 * g);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        f32x4 sc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) sc = mfma_k32<T>(kop[ks][j], qop[qs][j], sc);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int64_t kk = kb0 + 16 * ks + 4 * g + r;
+          bool ok = kk < k_len && (!a.causal || kk <= qq);
+          if constexpr (kWindow<Args>) ok = seen & (1u << (16 * ks + r));
+          sv[ks][r] = ok ? sc[r] * a.scale_log2 : kNegInfP;
+          tmax = fmaxf(tmax, sv[ks][r]);
+        }
+      }
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 16, 64));
+      tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64));
+      const float m_new = fmaxf(m[qs], tmax);
+      const bool fin = m_new != kNegInfP;
+      if (__any(m_new > m[qs])) {
+        const float alpha = fin ? fast_exp2(m[qs] - m_new) : 1.f;
+        l[qs] *= alpha;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float ar = __shfl(alpha, 4 * g + r, 64);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) acc[qs][u][r] *= ar;
+        }
+        m[qs] = m_new;
+      }
+      float p[2][4];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          p[ks][r] = fin ? fast_exp2(sv[ks][r] - m[qs]) : 0.f;
+          l[qs] += p[ks][r];
+        }
+      const u32x4 pop = u32x4{pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]), pack2<T>(p[1][0], p[1][1]),
+                              pack2<T>(p[1][2], p[1][3])};
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int w = u >> 1;
+        u32x4 bop;
+        if (u & 1) {
+          bop[0] = pack_hi(vrow[0][w], vrow[1][w]);
+          bop[1] = pack_hi(vrow[2][w], vrow[3][w]);
+          bop[2] = pack_hi(vrow[4][w], vrow[5][w]);
+          bop[3] = pack_hi(vrow[6][w], vrow[7][w]);
+        } else {
+          bop[0] = pack_lo(vrow[0][w], vrow[1][w]);
+          bop[1] = pack_lo(vrow[2][w], vrow[3][w]);
+          bop[2] = pack_lo(vrow[4][w], vrow[5][w]);
+          bop[3] = pack_lo(vrow[6][w], vrow[7][w]);
+        }
+        acc[qs][u] = mfma_k32<T>(pop, bop, acc[qs][u]);  // O[query 16qs+4g+r][dim 8c+u]
+      }
+    }
+  }
+
+  if constexpr (kWindow<Args>) {
+    // Sums that are not finite: a key that a query does not see may have held
+    // an infinity or NaN. Then the rows one by one, over the keys each sees.
+    float sum = 0.f;
+#pragma unroll
+    for (int qs = 0; qs < 2; ++qs)
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum = fmaf(acc[qs][u][r], 0.f, sum);
+    if (__any(sum != 0.f)) {
+#pragma unroll 1
+      for (int64_t qq = row0; qq < q_len && qq < row0 + 32; ++qq)
+        prefill_window_row<T>(a, q_start + qq, qq, h, k_start, k_len);
+      return;
+    }
+  }
+  T* ob_ptr = static_cast<T*>(a.out) + q_start * a.o_st + h * a.o_sh;
+#pragma unroll
+  for (int qs = 0; qs < 2; ++qs) {
+    float lt = l[qs];
+    lt += __shfl_xor(lt, 16, 64);
+    lt += __shfl_xor(lt, 32, 64);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float lr = __shfl(lt, 4 * g + r, 64);
+      const int64_t row = row0 + 16 * qs + 4 * g + r;
+      if (row < q_len && v_lane) {
+        T* op = ob_ptr + row * a.o_st + 8 * c;
+        float vals[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) vals[u] = kWindow<Args> && lr == 0.f ? 0.f : acc[qs][u][r] / lr;
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack2<T>(vals[2 * i], vals[2 * i + 1]);
+        *reinterpret_cast<u32x4*>(op) = w;
+      }
+    }
+  }
+}
+
+}  // namespace tsa

@@ -37,6 +37,11 @@
 // K/V blocks and each item's Q go from global memory straight into LDS
 // (global_load_lds_dwordx4); the loads of block step s (K(s + 1), V(s)) run
 // kW64A steps ahead through kW64Slots slots.
+//
+// With PrefillWindowArgs (a sliding window and first tokens) an item's blocks are
+// those that its 64 queries see (window_blocks), and a wave whose outputs are
+// not all finite computes its rows again over visible keys alone, as in
+// prefill_gqa_body.
 #pragma once
 
 #include <type_traits>
@@ -125,8 +130,8 @@ __device__ __forceinline__ void scale_agpr2(f32x4& x, float a0, float a1) {
   in_agpr(x);
 }
 
-template <typename T>
-__device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* __restrict__ cu_q,
+template <typename T, typename Args = PrefillArgs>
+__device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restrict__ cu_q,
                                                  const int32_t* __restrict__ cu_k, char* smem) {
   constexpr int KJ = 8, NU = 4, CPR = 16, RB = 256, BLKB = 32 * RB;
   constexpr int NB = kW64Slots, A = kW64A;
@@ -184,6 +189,13 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
     const T* kb;
     const T* vb;
     T* ob;
+    WindowBlocks win;  // (window) the blocks; the rest: for rows computed again
+    int64_t q_start, k_start;
+    int head;
+  };
+  auto block_at = [&](const Item& it, int v) __attribute__((always_inline)) {
+    if constexpr (kWindow<Args>) return it.win.at(v);
+    else return v;
   };
   auto fill_item = [&](Item& it, int b, int hh, int Q, int64_t qs, int64_t ql, int64_t ks, int64_t kl) {
     const int kvh = hh / HG, hg = hh - kvh * HG;
@@ -200,6 +212,14 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
     it.kb = static_cast<const T*>(a.k) + ks * a.k_st + kvh * a.k_sh;
     it.vb = static_cast<const T*>(a.v) + ks * a.v_st + kvh * a.v_sh;
     it.ob = static_cast<T*>(a.out) + qs * a.o_st + head * a.o_sh;
+    if constexpr (kWindow<Args>) {
+      it.win = window_blocks(a, it.q0, q_last, it.k_len);
+      it.nblk = it.win.count;
+      it.kfull = min(it.k_len, it.win.end);
+      it.q_start = qs;
+      it.k_start = ks;
+      it.head = head;
+    }
     (void)b;
   };
   // Item i -> level Q (the smallest with items_above(Q) <= i), then the
@@ -315,7 +335,7 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
 #pragma unroll
   for (int i = 0; i < IPW; ++i) doffs[i] = doff[i] + static_cast<uint32_t>(i * RPI * st_b);
   auto load_block = [&](const Item& it, int blk, int slot) __attribute__((always_inline)) {
-    const int key0 = min(blk, it.nblk - 1) * 32 + row0w;
+    const int key0 = block_at(it, min(blk, it.nblk - 1)) * 32 + row0w;
     const int lds0 = (k_wave ? 0 : VOFF) + slot * BLKB + row0w * RB;
     const char* gbase = reinterpret_cast<const char*>(k_wave ? it.kb : it.vb);
     if (key0 + IPW * RPI <= it.k_len) {
@@ -351,6 +371,11 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
     constexpr int s = decltype(S)::value;
     constexpr int kslot = (s + A + 1) % NB, vslot = (s + A) % NB;
     const int lds0 = (k_wave ? kslot * BLKB : VOFF + vslot * BLKB) + row0w * RB;
+    if constexpr (kWindow<Args>) {  // (the blocks are two runs: their place is computed)
+      const int v = j + A + (k_wave ? 1 : 0);
+      rk = v < it.nblk ? 32 * it.win.at(v) + row0w : it.kfull;
+      rp = reinterpret_cast<const char*>(k_wave ? it.kb : it.vb) + rk * st_b;
+    }
     if (rk + IPW * RPI <= it.kfull) {
 #pragma unroll
       for (int i = 0; i < IPW; ++i) dma16_sv(rp, doffs[i], smem_lds + lds0 + i * 1024);
@@ -467,7 +492,19 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
   // With base = 32 blk + 4h the key is base + ke(e), ke(e) = 8(e/4) + e%4 a
   // compile-time constant, so one per-lane bound serves all 16 scores: score
   // e is kept iff ke(e) < min(k_len - base, query - base + 1).
+  // With a window the row's 32 bits say it instead (window_bits).
+  auto needs_mask = [&](const Item& it, int t, int blk) __attribute__((always_inline)) {
+    if constexpr (kWindow<Args>) return !window_sees_all(a, it.q0 + 32 * t, 32 * it.win.at(blk), it.k_len);
+    else return blk >= it.jm;
+  };
   auto mask_scores = [&](const Item& it, int t, int blk, int e0, int e1) __attribute__((always_inline)) {
+    if constexpr (kWindow<Args>) {
+      const uint32_t bits = window_bits(a, it.q0 + 32 * t + c, 32 * it.win.at(blk), it.k_len) >> (4 * h);
+#pragma unroll
+      for (int e = e0; e < e1; ++e)
+        if (!(bits & (1u << (8 * (e >> 2) + (e & 3))))) sc[t][e] = kNegInfP;
+      return;
+    }
     const int base = blk * 32 + 4 * h;
     int bound = it.k_len - base;
     if (a.causal) bound = min(bound, it.q0 + 32 * t + c - base + 1);
@@ -556,7 +593,7 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
       }
       // Blocks from jm on may hold keys past k_len or (causal) past the
       // query: a uniform branch, rarely taken.
-      if (g == 10 && do_qk && mblk >= it.jm) {
+      if (g == 10 && do_qk && needs_mask(it, o, mblk)) {
         xdl_to_valu_nops();
         mask_scores(it, o, mblk, 0, 16);
       }
@@ -620,6 +657,7 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
     char* pend_p[4];
     bool pend_ok[4];
     bool pend_full = true, have = false;
+    float finite = 0.f;  // (window) NaN where a sum is not finite
     auto flush = [&]() __attribute__((always_inline)) {
       if (pend_full) {
 #pragma unroll
@@ -633,7 +671,9 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const float l0 = __shfl(lacc[t][0], c & 15, 64), l1 = __shfl(lacc[t][1], c & 15, 64);
-      const float rl = 1.f / (c < 16 ? l0 : l1);  // 1 / query c's denominator
+      const float den = c < 16 ? l0 : l1;
+      const float rl = kWindow<Args> && den == 0.f ? 0.f : 1.f / den;  // 1 / query c's denominator (window: nothing seen, 0)
+      if constexpr (kWindow<Args>) finite = fmaf(den, 0.f, finite);
       const int rbase = it.q0 + 32 * t;
       const bool full = rbase + 32 <= it.q_len;
       char* rowp[4];
@@ -651,6 +691,10 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const int u = 2 * half + uu;
+            if constexpr (kWindow<Args>) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) finite = fmaf(acc[t][u][4 * g + i], 0.f, finite);
+            }
             const u32x2 w = {pack2<T>(acc[t][u][4 * g] * rl, acc[t][u][4 * g + 1] * rl),
                              pack2<T>(acc[t][u][4 * g + 2] * rl, acc[t][u][4 * g + 3] * rl)};
             *reinterpret_cast<u32x2*>(ost + c * 128 + 16 * ((4 * uu + g) ^ (c & 7)) + 8 * h) = w;
@@ -673,6 +717,15 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
       }
     }
     flush();
+    if constexpr (kWindow<Args>) {
+      if (__any(finite != 0.f)) {  // (uniform)
+        wait_vmcnt<0>();  // those stores first
+        const int last = min(it.q_len, it.q0 + 64);
+#pragma unroll 1
+        for (int qq = it.q0; qq < last; ++qq)
+          prefill_window_row<T>(a, it.q_start + qq, qq, it.head, it.k_start, it.k_len);
+      }
+    }
   };
 
   // ---- The item loop. At an item's end, after its last barrier, the next
@@ -711,7 +764,7 @@ __device__ __forceinline__ void prefill_w64_body(PrefillArgs a, const int32_t* _
 #pragma unroll
       for (int jj = 0; jj < KJ; ++jj) qk1(0, jj);
       xdl_to_valu_nops();
-      if (X.jm == 0) mask_scores(X, 0, 0, 0, 16);
+      if (needs_mask(X, 0, 0)) mask_scores(X, 0, 0, 0, 16);
 #pragma unroll
       for (int part = 0; part < 4; ++part) max_part(0, part);
       max_end(0);

@@ -4,6 +4,7 @@
 
 #include "tsa_common.h"
 #include "varlen_prefill_w64.h"
+#include "varlen_prefill_window.h"
 
 namespace tsa {
 
@@ -25,6 +26,23 @@ int prefill_w64_launch(const PrefillArgs& a, bool bf16, hipStream_t stream) {
   if (bf16) varlen_prefill_w64<bf16_t><<<dim3(cus), dim3(256), 0, stream>>>(a, a.cu_q, a.cu_k);
   else varlen_prefill_w64<f16_t><<<dim3(cus), dim3(256), 0, stream>>>(a, a.cu_q, a.cu_k);
   return check_launch("tsa_varlen_prefill");
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void varlen_window_w64(
+    PrefillWindowArgs a, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k) {
+  __shared__ __align__(16) char smem[w64_smem_bytes()];
+  prefill_w64_body<T>(a, cu_q, cu_k, smem);
+}
+
+int prefill_w64_window_launch(const PrefillWindowArgs& a, bool bf16, hipStream_t stream) {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
+    cus = 256;
+  if (bf16) varlen_window_w64<bf16_t><<<dim3(cus), dim3(256), 0, stream>>>(a, a.cu_q, a.cu_k);
+  else varlen_window_w64<f16_t><<<dim3(cus), dim3(256), 0, stream>>>(a, a.cu_q, a.cu_k);
+  return check_launch("tsa_varlen_prefill_window");
 }
 
 // TSA_PREFILL_W64=0 in the environment routes calls to varlen_prefill_gqa

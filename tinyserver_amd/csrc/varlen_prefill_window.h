@@ -1,14 +1,9 @@
-// What windowed prefill adds to the prefill's argument block, and one row of it.
+// Windowed prefill (PrefillWindowArgs in varlen_prefill_gqa.h): one row, by one wave.
 #pragma once
 
 #include "varlen_prefill_gqa.h"
 
 namespace tsa {
-
-struct PrefillWindowArgs : PrefillArgs {
-  int32_t window;  // keys j > i - window are seen by query i (at least 1), and
-  int32_t sinks;   // keys j < sinks
-};
 
 // Row qi of q/out (query qq of its sequence), q-head h, over the sequence's
 // keys [k_start, k_start + k_len), by one wave: any strides, head_dim up to

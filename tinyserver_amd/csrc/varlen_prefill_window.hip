@@ -1,9 +1,66 @@
 // Varlen prefill attention with a sliding window and first tokens that stay
 // visible: query i of a sequence sees the keys j <= i with j > i - window or
 // j < sinks (top-left positions, as tsa_varlen_prefill's causal mask).
+//
+// varlen_window_w64   bf16/f16, head_dim 128, GQA group 4 (12, 16, ...): 64
+//                     queries a wave (prefill_w64_body), and
+// varlen_window_gqa   head_dim 64 or group 2 or 8: the LDS-staged persistent
+//                     kernel (prefill_gqa_body), both over the blocks of the
+//                     window and of the first keys;
+// varlen_prefill_mfma other groups;
+// varlen_window_generic  float32, other head_dims, strides and scales: one wave
+//                     per (query, q-head), VALU.
+#include "varlen_prefill_mfma.h"
 #include "varlen_prefill_window.h"
 
 namespace tsa {
+
+template <typename T, int D, int NW, int QS>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void varlen_window_gqa(
+    PrefillWindowArgs a, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k) {
+  __shared__ __align__(16) char smem[gqa_smem_bytes<D, NW>()];
+  prefill_gqa_body<T, D, NW, QS>(a, cu_q, cu_k, smem, 0);
+}
+
+// As many workgroups as fit on the device at once.
+template <typename T, int D, int NW, int QS = 1>
+static int launch_window_gqa(const PrefillWindowArgs& a, hipStream_t stream) {
+  int per_cu = 0, dev = 0, cus = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, varlen_window_gqa<T, D, NW, QS>, 64 * NW, 0) != hipSuccess ||
+      per_cu <= 0)
+    per_cu = 1;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
+    cus = 256;
+  varlen_window_gqa<T, D, NW, QS><<<dim3(per_cu * cus), dim3(64 * NW), 0, stream>>>(a, a.cu_q, a.cu_k);
+  return check_launch("tsa_varlen_prefill_window");
+}
+
+template <typename T>
+static int launch_window_mfma(PrefillWindowArgs& a, int64_t max_seqlen_q, hipStream_t stream) {
+  // Groups of eight keep the eight waves of the LDS-staged kernel, which stage
+  // each K/V block once for all of them: 16 prompts of 128-2048 tokens, 64/8
+  // heads, window 128 / 512: 296 / 460 us against 398 / 551 with 64 queries a
+  // wave (one of 16384, window 4096: 1892 against 1900). Groups of four take 64
+  // queries a wave: 229 / 364 -> 197 / 279.
+  if (prefill_takes_w64(a) && a.G != 8)
+    return prefill_w64_window_launch(a, std::is_same<T, bf16_t>::value, stream);
+  if (prefill_takes_gqa(a)) {
+    if (a.D == 128) {
+      if (prefill_pairs(a)) return launch_window_gqa<T, 128, 4, 2>(a, stream);
+      if (a.G == 2) return launch_window_gqa<T, 128, 2>(a, stream);
+      return a.G == 4 ? launch_window_gqa<T, 128, 4>(a, stream) : launch_window_gqa<T, 128, 8>(a, stream);
+    }
+    if (a.G == 2) return launch_window_gqa<T, 64, 2>(a, stream);
+    return a.G == 4 ? launch_window_gqa<T, 64, 4>(a, stream) : launch_window_gqa<T, 64, 8>(a, stream);
+  }
+  a.nqb = static_cast<int32_t>((max_seqlen_q + 31) / 32);
+  if (a.nqb == 0) return TSA_OK;
+  const dim3 grid(a.nqb, a.nseq, (a.Hq + 3) / 4);
+  if (a.D == 128) varlen_prefill_mfma<T, 128><<<grid, dim3(256), 0, stream>>>(a);
+  else varlen_prefill_mfma<T, 64><<<grid, dim3(256), 0, stream>>>(a);
+  return check_launch("tsa_varlen_prefill_window");
+}
 
 // Any strides and head_dim up to 512: one wave per (query row, q-head).
 template <typename T>
@@ -53,6 +110,9 @@ extern "C" int tsa_varlen_prefill_window(const tsa_view* out, const tsa_view* q,
   a.sinks = static_cast<int32_t>(sinks < kMost ? sinks : kMost);
   if (a.nseq == 0 || a.Hq == 0 || a.D == 0 || a.total_q == 0) return TSA_OK;
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (mfma && a.scale_log2 > 0.f && a.nseq < 65536 && q->dtype != TSA_F32)
+    return q->dtype == TSA_BF16 ? launch_window_mfma<bf16_t>(a, max_seqlen_q, st)
+                                : launch_window_mfma<f16_t>(a, max_seqlen_q, st);
   switch (q->dtype) {
     case TSA_BF16: return launch_window<bf16_t>(a, st);
     case TSA_F16: return launch_window<f16_t>(a, st);
