@@ -62,6 +62,175 @@ __global__ __launch_bounds__(256) void quant8_rows(Quant8Args a, PagedAddr addr)
   }
 }
 
+// 16-bit rows of 64 or 128 dims in 16-byte pieces: D / 8 lanes a row, 8 elements
+// a lane, so that a wave's stores of one head's tokens are whole lines. A
+// workgroup takes 256 / (D / 8) tokens and `heads` kv heads of each, kBatch at a
+// time, K and V together, with all of a batch's loads in flight; a token's
+// place is looked up once. The sequences' starts go to LDS first, so the search
+// is one round trip to memory and not one for each of its steps.
+//
+// A quotient is x times the scale's reciprocal, corrected twice by its fma
+// residual: with the correctly rounded reciprocal that is the correctly rounded
+// x / scale (Markstein's theorem: one step from a quotient within a unit in the
+// last place; the first step gives that one). Residuals below the normal range
+// would lose bits, so rows of scales under 2^-80 divide.
+constexpr int kQuant8Batch = 4;
+constexpr int kQuant8LdsSeqs = 2048;
+
+struct LdsCu {
+  const int32_t* cu;  // [nseq + 1] in LDS
+  __device__ __forceinline__ bool locate(const PagedAddr& a, int64_t t, int64_t BS, int64_t NB, int64_t& blk,
+                                         int64_t& slot) const {
+    int lo = 0, hi = static_cast<int>(a.nseq);  // the last s with cu[s] <= t is in [lo, hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (cu[mid] <= t) lo = mid; else hi = mid;
+    }
+    const int64_t t0 = cu[lo];
+    if (t < t0 || t >= cu[lo + 1]) return false;
+    int64_t p;
+    if (a.pos_kind == 2) p = static_cast<const int64_t*>(a.pos)[t * a.pos_stride];
+    else if (a.pos_kind == 1) p = static_cast<const int32_t*>(a.pos)[t * a.pos_stride];
+    else p = t - t0;
+    if (p < 0 || p >= a.max_blocks * BS) return false;
+    // (positions within a table fit 32 bits here: checked by the caller)
+    const uint32_t lb = static_cast<uint32_t>(p) / static_cast<uint32_t>(BS);
+    blk = a.bt[lo * a.bt_s0 + lb * a.bt_s1];
+    slot = static_cast<uint32_t>(p) - lb * static_cast<uint32_t>(BS);
+    return blk >= 0 && blk < NB;
+  }
+};
+
+template <typename C> __device__ __forceinline__ void quotients8(const float (&x)[8], float scale, float (&q)[8]) {
+  if (scale > 0x1p-80f) {
+    const float r = 1.f / scale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float y = x[i] * r;
+      y = fmaf(fmaf(-y, scale, x[i]), r, y);
+      y = fmaf(fmaf(-y, scale, x[i]), r, y);
+      q[i] = fminf(fmaxf(y, -kLargest8<C>), kLargest8<C>);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = quotient8<C>(x[i], scale);
+  }
+}
+
+template <typename T, typename C, int D, bool STORE>
+__global__ __launch_bounds__(256) void quant8_vec(Quant8Args a, PagedAddr addr, int heads) {
+  constexpr int LG = D / 8, TOK = 256 / LG;
+  __shared__ int32_t cu_s[kQuant8LdsSeqs + 1];
+  const int tid = threadIdx.x, c = tid % LG;
+  for (int i = tid; i <= addr.nseq; i += 256) cu_s[i] = addr.cu[i * addr.cu_stride];
+  __syncthreads();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * TOK + tid / LG, tt = t < a.T ? t : a.T - 1;
+  int64_t blk = 0, slot = 0;
+  const bool found = LdsCu{cu_s}.locate(addr, tt, a.BS, a.NB, blk, slot), ok = found && t < a.T;
+  if (!found) blk = slot = 0;
+  const int h0 = static_cast<int>(blockIdx.y) * heads, h1 = min(h0 + heads, static_cast<int>(a.H));
+  const int64_t kc = blk * a.kc_b + slot * a.kc_s + 8 * c, vc = blk * a.vc_b + slot * a.vc_s + 8 * c;
+  const int64_t ks = blk * a.ks_b + slot * a.ks_s, vs = blk * a.vs_b + slot * a.vs_s;
+  for (int h = h0; h < h1; h += kQuant8Batch) {
+    if constexpr (STORE) {
+      u32x4 x[kQuant8Batch][2];
+#pragma unroll
+      for (int i = 0; i < kQuant8Batch; ++i) {
+        const int hh = min(h + i, h1 - 1);
+        x[i][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(a.k_src) + tt * a.kr_t + hh * a.kr_h + 8 * c);
+        x[i][1] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(a.v_src) + tt * a.vr_t + hh * a.vr_h + 8 * c);
+      }
+#pragma unroll
+      for (int i = 0; i < kQuant8Batch; ++i) {
+        if (h + i >= h1) break;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float f[8], q[8];
+          uint32_t top = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            f[2 * k] = lo_f<T>(x[i][y][k]);
+            f[2 * k + 1] = hi_f<T>(x[i][y][k]);
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top = max(top, __builtin_bit_cast(uint32_t, f[k]) & 0x7FFFFFFFu);
+          const int lane = tid & 63;  // (every lane takes part: tokens past the last repeat it)
+          top = max(top, xor_lane32<1>(top, lane));
+          top = max(top, xor_lane32<2>(top, lane));
+          top = max(top, xor_lane32<4>(top, lane));
+          if constexpr (LG == 16) top = max(top, xor_lane32<8>(top, lane));
+          const float scale = scale8<C>(top);
+          quotients8<C>(f, scale, q);
+          if (ok) {
+            const u32x2 w = {codes4<C>(q[0], q[1], q[2], q[3]), codes4<C>(q[4], q[5], q[6], q[7])};
+            *reinterpret_cast<u32x2*>((y ? a.vc + vc + (h + i) * a.vc_h : a.kc + kc + (h + i) * a.kc_h)) = w;
+            if (c == 0) (y ? a.vs[vs + (h + i) * a.vs_h] : a.ks[ks + (h + i) * a.ks_h]) = scale;
+          }
+        }
+      }
+    } else {
+      u32x2 w[kQuant8Batch][2];
+      float sc[kQuant8Batch][2];
+#pragma unroll
+      for (int i = 0; i < kQuant8Batch; ++i) {  // (a token without a page reads page 0's first row, and drops it)
+        const int hh = min(h + i, h1 - 1);
+        w[i][0] = w[i][1] = u32x2{0, 0};
+        sc[i][0] = sc[i][1] = 0.f;
+        if (a.NB > 0) {
+          w[i][0] = *reinterpret_cast<const u32x2*>(a.kc + kc + hh * a.kc_h);
+          w[i][1] = *reinterpret_cast<const u32x2*>(a.vc + vc + hh * a.vc_h);
+          sc[i][0] = a.ks[ks + hh * a.ks_h];
+          sc[i][1] = a.vs[vs + hh * a.vs_h];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kQuant8Batch; ++i) {
+        if (h + i >= h1 || t >= a.T) break;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          u32x4 out;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float v[4];
+            values4<C>(w[i][y][k], v);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              out[2 * k + e] = found ? pack2<T>(product8(v[2 * e], sc[i][y]), product8(v[2 * e + 1], sc[i][y])) : 0u;
+          }
+          T* const dst = y ? reinterpret_cast<T*>(a.v_out) + t * a.vr_t + (h + i) * a.vr_h
+                           : reinterpret_cast<T*>(a.k_out) + t * a.kr_t + (h + i) * a.kr_h;
+          *reinterpret_cast<u32x4*>(dst + 8 * c) = out;
+        }
+      }
+    }
+  }
+}
+
+// Whether the calls' rows are what quant8_vec takes.
+static bool quant8_takes_vec(const Quant8Args& a, const PagedAddr& addr, const tsa_view* k, const tsa_view* v,
+                             const tsa_view* k_cache, const tsa_view* v_cache) {
+  if ((k->dtype != TSA_BF16 && k->dtype != TSA_F16) || (a.D != 64 && a.D != 128)) return false;
+  if (!rows_vec16(k) || !rows_vec16(v) || addr.nseq < 1 || addr.nseq > kQuant8LdsSeqs) return false;
+  if (addr.max_blocks >= (int64_t{1} << 31) / a.BS || a.T >= (int64_t{1} << 31)) return false;
+  for (const tsa_view* x : {k_cache, v_cache}) {
+    if (x->stride[3] != 1 || reinterpret_cast<uintptr_t>(x->data) % 8) return false;
+    for (int d = 0; d < 3; ++d)
+      if (x->size[d] > 1 && x->stride[d] % 8) return false;
+  }
+  return a.H < 65536;
+}
+
+template <typename T, typename C, bool STORE>
+static int launch_quant8_vec(const Quant8Args& a, const PagedAddr& addr, hipStream_t stream, const char* what) {
+  // Prompts: eight heads a workgroup, so a token is looked up once for them.
+  // Few tokens: one head each, for more workgroups.
+  const int tok = 256 / static_cast<int>(a.D / 8), heads = a.T >= 2048 ? 8 : 1;
+  const dim3 grid(static_cast<uint32_t>((a.T + tok - 1) / tok), static_cast<uint32_t>((a.H + heads - 1) / heads));
+  if (a.D == 128) quant8_vec<T, C, 128, STORE><<<grid, dim3(256), 0, stream>>>(a, addr, heads);
+  else quant8_vec<T, C, 64, STORE><<<grid, dim3(256), 0, stream>>>(a, addr, heads);
+  return check_launch(what);
+}
+
 template <typename T, typename C, bool STORE>
 static int launch_quant8(const Quant8Args& a, const PagedAddr& addr, hipStream_t stream, const char* what) {
   const int64_t wgs = (2 * a.T * a.H + 3) / 4;
@@ -113,10 +282,16 @@ static int check_quant8(const tsa_view* k, const tsa_view* v, bool heads_first, 
 }
 
 template <bool STORE>
-static int dispatch_quant8(const Quant8Args& a, const PagedAddr& addr, int dt, int cache_dt, hipStream_t stream,
-                           const char* what) {
+static int dispatch_quant8(const Quant8Args& a, const PagedAddr& addr, bool vec, int dt, int cache_dt,
+                           hipStream_t stream, const char* what) {
   if (a.T == 0 || a.H == 0 || a.D == 0) return TSA_OK;
   const bool e4m3 = cache_dt == TSA_E4M3;
+  if (vec && dt == TSA_BF16)
+    return e4m3 ? launch_quant8_vec<bf16_t, e4m3_t, STORE>(a, addr, stream, what)
+                : launch_quant8_vec<bf16_t, i8_t, STORE>(a, addr, stream, what);
+  if (vec)
+    return e4m3 ? launch_quant8_vec<f16_t, e4m3_t, STORE>(a, addr, stream, what)
+                : launch_quant8_vec<f16_t, i8_t, STORE>(a, addr, stream, what);
   switch (dt) {
     case TSA_BF16:
       return e4m3 ? launch_quant8<bf16_t, e4m3_t, STORE>(a, addr, stream, what)
@@ -145,8 +320,8 @@ extern "C" int tsa_store_kv_quantized(const tsa_view* k_src, const tsa_view* v_s
   PagedAddr addr;
   if (int rc = make_paged_addr(block_tables, cu_seqlens, positions, a.T, addr)) return rc;
   if (a.NB == 0) return TSA_OK;  // (no page to write)
-  return dispatch_quant8<true>(a, addr, k_src->dtype, k_cache->dtype, static_cast<hipStream_t>(stream),
-                               "tsa_store_kv_quantized");
+  return dispatch_quant8<true>(a, addr, quant8_takes_vec(a, addr, k_src, v_src, k_cache, v_cache), k_src->dtype,
+                               k_cache->dtype, static_cast<hipStream_t>(stream), "tsa_store_kv_quantized");
 }
 
 extern "C" int tsa_load_kv_quantized(const tsa_view* k_out, const tsa_view* v_out, const tsa_view* k_cache,
@@ -159,6 +334,6 @@ extern "C" int tsa_load_kv_quantized(const tsa_view* k_out, const tsa_view* v_ou
   a.v_out = static_cast<char*>(v_out->data);
   PagedAddr addr;
   if (int rc = make_paged_addr(block_tables, cu_seqlens, positions, a.T, addr)) return rc;
-  return dispatch_quant8<false>(a, addr, k_out->dtype, k_cache->dtype, static_cast<hipStream_t>(stream),
-                                "tsa_load_kv_quantized");
+  return dispatch_quant8<false>(a, addr, quant8_takes_vec(a, addr, k_out, v_out, k_cache, v_cache), k_out->dtype,
+                                k_cache->dtype, static_cast<hipStream_t>(stream), "tsa_load_kv_quantized");
 }
