@@ -74,12 +74,13 @@ __global__ __launch_bounds__(256) void quant8_rows(Quant8Args a, PagedAddr addr)
 // x / scale (Markstein's theorem: one step from a quotient within a unit in the
 // last place; the first step gives that one). Residuals below the normal range
 // would lose bits, so rows of scales under 2^-80 divide.
-constexpr int kQuant8Batch = 4;
+constexpr int kQuant8Batch = 2;
 constexpr int kQuant8LdsSeqs = 2048;
 
 struct LdsCu {
   const int32_t* cu;  // [nseq + 1] in LDS
-  __device__ __forceinline__ bool locate(const PagedAddr& a, int64_t t, int64_t BS, int64_t NB, int64_t& blk,
+  // pos: the token's given position, where there are any.
+  __device__ __forceinline__ bool locate(const PagedAddr& a, int64_t t, int64_t pos, int64_t BS, int64_t NB, int64_t& blk,
                                          int64_t& slot) const {
     int lo = 0, hi = static_cast<int>(a.nseq);  // the last s with cu[s] <= t is in [lo, hi)
     while (hi - lo > 1) {
@@ -88,10 +89,7 @@ struct LdsCu {
     }
     const int64_t t0 = cu[lo];
     if (t < t0 || t >= cu[lo + 1]) return false;
-    int64_t p;
-    if (a.pos_kind == 2) p = static_cast<const int64_t*>(a.pos)[t * a.pos_stride];
-    else if (a.pos_kind == 1) p = static_cast<const int32_t*>(a.pos)[t * a.pos_stride];
-    else p = t - t0;
+    const int64_t p = a.pos_kind ? pos : t - t0;
     if (p < 0 || p >= a.max_blocks * BS) return false;
     // (positions within a table fit 32 bits here: checked by the caller)
     const uint32_t lb = static_cast<uint32_t>(p) / static_cast<uint32_t>(BS);
@@ -122,24 +120,32 @@ __global__ __launch_bounds__(256) void quant8_vec(Quant8Args a, PagedAddr addr, 
   constexpr int LG = D / 8, TOK = 256 / LG;
   __shared__ int32_t cu_s[kQuant8LdsSeqs + 1];
   const int tid = threadIdx.x, c = tid % LG;
-  for (int i = tid; i <= addr.nseq; i += 256) cu_s[i] = addr.cu[i * addr.cu_stride];
-  __syncthreads();
   const int64_t t = static_cast<int64_t>(blockIdx.x) * TOK + tid / LG, tt = t < a.T ? t : a.T - 1;
-  int64_t blk = 0, slot = 0;
-  const bool found = LdsCu{cu_s}.locate(addr, tt, a.BS, a.NB, blk, slot), ok = found && t < a.T;
-  if (!found) blk = slot = 0;
   const int h0 = static_cast<int>(blockIdx.y) * heads, h1 = min(h0 + heads, static_cast<int>(a.H));
+  // (store) The first batch's rows and the position are asked for before the search.
+  u32x4 x[kQuant8Batch][2];
+  auto fetch = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kQuant8Batch; ++i) {
+      const int hh = min(h + i, h1 - 1);
+      x[i][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(a.k_src) + tt * a.kr_t + hh * a.kr_h + 8 * c);
+      x[i][1] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(a.v_src) + tt * a.vr_t + hh * a.vr_h + 8 * c);
+    }
+  };
+  int64_t pos = 0;
+  if (addr.pos_kind == 2) pos = static_cast<const int64_t*>(addr.pos)[tt * addr.pos_stride];
+  else if (addr.pos_kind == 1) pos = static_cast<const int32_t*>(addr.pos)[tt * addr.pos_stride];
+  for (int i = tid; i <= addr.nseq; i += 256) cu_s[i] = addr.cu[i * addr.cu_stride];
+  if constexpr (STORE) fetch(h0);
+  lds_barrier();
+  int64_t blk = 0, slot = 0;
+  const bool found = LdsCu{cu_s}.locate(addr, tt, pos, a.BS, a.NB, blk, slot), ok = found && t < a.T;
+  if (!found) blk = slot = 0;
   const int64_t kc = blk * a.kc_b + slot * a.kc_s + 8 * c, vc = blk * a.vc_b + slot * a.vc_s + 8 * c;
   const int64_t ks = blk * a.ks_b + slot * a.ks_s, vs = blk * a.vs_b + slot * a.vs_s;
   for (int h = h0; h < h1; h += kQuant8Batch) {
     if constexpr (STORE) {
-      u32x4 x[kQuant8Batch][2];
-#pragma unroll
-      for (int i = 0; i < kQuant8Batch; ++i) {
-        const int hh = min(h + i, h1 - 1);
-        x[i][0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(a.k_src) + tt * a.kr_t + hh * a.kr_h + 8 * c);
-        x[i][1] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(a.v_src) + tt * a.vr_t + hh * a.vr_h + 8 * c);
-      }
+      if (h > h0) fetch(h);
 #pragma unroll
       for (int i = 0; i < kQuant8Batch; ++i) {
         if (h + i >= h1) break;
@@ -222,9 +228,10 @@ static bool quant8_takes_vec(const Quant8Args& a, const PagedAddr& addr, const t
 
 template <typename T, typename C, bool STORE>
 static int launch_quant8_vec(const Quant8Args& a, const PagedAddr& addr, hipStream_t stream, const char* what) {
-  // Prompts: eight heads a workgroup, so a token is looked up once for them.
-  // Few tokens: one head each, for more workgroups.
-  const int tok = 256 / static_cast<int>(a.D / 8), heads = a.T >= 2048 ? 8 : 1;
+  // Prompts: two heads a workgroup share a token's lookup (the 16 prompts' store
+  // and the 8 prefixes' load: 24.7 and 25.1 us; eight heads 25.3 and 26.9, one
+  // 26.3 and 29.5). Few tokens: one head each, for more workgroups.
+  const int tok = 256 / static_cast<int>(a.D / 8), heads = a.T >= 2048 ? 2 : 1;
   const dim3 grid(static_cast<uint32_t>((a.T + tok - 1) / tok), static_cast<uint32_t>((a.H + heads - 1) / heads));
   if (a.D == 128) quant8_vec<T, C, 128, STORE><<<grid, dim3(256), 0, stream>>>(a, addr, heads);
   else quant8_vec<T, C, 64, STORE><<<grid, dim3(256), 0, stream>>>(a, addr, heads);
