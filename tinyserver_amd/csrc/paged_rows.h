@@ -104,7 +104,7 @@ struct DecodeRowsPlan {
   size_t part_bytes, total;
 };
 DecodeRowsPlan decode_rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, int64_t window,
-                                int64_t sinks, bool cache8);
+                                int64_t sinks);
 // paged_rows_unit.hip, paged_rows_stream.hip: the launches (a.S, a.NW, a.part, a.pref set).
 int rows_unit_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what);
 int rows_stream_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what);

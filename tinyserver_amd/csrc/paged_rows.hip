@@ -245,8 +245,7 @@ extern "C" int tsa_paged_decode_window(const tsa_view* out, const tsa_view* quer
                           window, sinks, softmax_scale, a))
     return rc;
   if (a.B > 0 && a.Hq > 0 && takes_mfma(a, out, query, k_cache, v_cache)) {
-    const DecodeRowsPlan p = decode_rows_plan(a.B, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS, a.window, a.sinks,
-                                              a.ks != nullptr);
+    const DecodeRowsPlan p = decode_rows_plan(a.B, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS, a.window, a.sinks);
     TSA_REQUIRE(p.total == 0 || (workspace != nullptr && workspace_bytes >= p.total),
                 "workspace of %zu bytes is too small: %zu needed", workspace_bytes, p.total);
     TSA_REQUIRE(p.total == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
@@ -293,9 +292,7 @@ extern "C" size_t tsa_paged_rows_workspace_bytes(int64_t num_seqs, int64_t max_n
       max_blocks_per_seq * block_size >= (int64_t{1} << 27))
     return 0;  // (calls of such sizes are refused, or have nothing to do)
   const int64_t cap = max_blocks_per_seq * block_size;
-  const DecodeRowsPlan p16 = decode_rows_plan(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks, false);
-  const DecodeRowsPlan p8 = decode_rows_plan(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks, true);
-  const size_t decode = p16.total > p8.total ? p16.total : p8.total;  // for either kind of cache
+  const size_t decode = decode_rows_plan(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks).total;
   if (window > 0 || sinks > 0) return decode;
   const size_t tree = tree_rows_plan(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, cap).bytes;
   return max_nodes > 1 ? tree : tree > decode ? tree : decode;

@@ -38,7 +38,7 @@ static int launch_unit(const RowsArgs& a, hipStream_t stream, const char* what) 
   else
     paged_rows_unit<T, C, D, kUnitWavesSplit, false><<<grid, threads, kUnitWavesSplit * row_bytes, stream>>>(a, a.bt, a.lens, a.part);
   if (int rc = check_launch(what)) return rc;
-  launch_rows_merge<T, D>(a, a.G, kUnitWavesSplit * kUnitTiles<C>, stream);
+  launch_rows_merge<T, D>(a, a.G, kUnitWavesSplit * kUnitTiles, stream);
   return check_launch(what);
 }
 
@@ -60,18 +60,17 @@ int rows_unit_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream
 // One workgroup of eight waves a unit where its visible tiles fit it, else
 // splits of four waves each, else the stream.
 DecodeRowsPlan decode_rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, int64_t window,
-                                int64_t sinks, bool cache8) {
+                                int64_t sinks) {
   int64_t tiles = (cap + 15) / 16;
   if (window > 0 && window < cap) {
     const int64_t seen = ((sinks < cap ? sinks : cap) + 15) / 16 + (window + 15) / 16 + 1;
     tiles = seen < tiles ? seen : tiles;
   }
-  const int kt = cache8 ? kUnitTiles<i8_t> : kUnitTiles<bf16_t>;
   const int64_t G = Hq / Hkv, items = B * Hkv * ((G + 15) / 16), rows = G < 16 ? G : 16;
   const size_t slot = static_cast<size_t>(rows) * (D + 4) * sizeof(float);
   auto align = [](size_t n) { return (n + 255) & ~size_t{255}; };
   DecodeRowsPlan p{};
-  const int64_t S = tiles <= kUnitWavesOne * kt ? 1 : (tiles + kUnitWavesSplit * kt - 1) / (kUnitWavesSplit * kt);
+  const int64_t S = tiles <= kUnitWavesOne * kUnitTiles ? 1 : (tiles + kUnitWavesSplit * kUnitTiles - 1) / (kUnitWavesSplit * kUnitTiles);
   if (S == 1 || items * S <= kUnitMaxWorkgroups || B > kStreamMaxSeqs) {
     p.S = static_cast<int>(S);
     p.total = p.part_bytes = S == 1 ? 0 : align(static_cast<size_t>(B * Hkv * S * G) * (D + 4) * sizeof(float));
