@@ -306,7 +306,8 @@ int tsa_load_kv_quantized(const tsa_view* k_out, const tsa_view* v_out, const ts
 
 /* Bytes of workspace tsa_paged_decode_window (max_nodes 1) and tsa_paged_tree
  * (window and sinks 0) need: the partial results of a (sequence, kv head)'s
- * splits; 0 where nothing is split. */
+ * splits; 0 where nothing is split. A tree's max_nodes is the lesser of the
+ * call's and its mask's bits. Of the current device. */
 size_t tsa_paged_rows_workspace_bytes(int64_t num_seqs, int64_t max_nodes, int64_t num_heads,
                                       int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks_per_seq,
                                       int64_t block_size, int64_t window, int64_t sinks);
@@ -318,7 +319,8 @@ size_t tsa_paged_rows_workspace_bytes(int64_t num_seqs, int64_t max_nodes, int64
  * no influence, whatever their rows hold; a token whose page id is outside the
  * pool is not seen; lengths are taken within [0, the table's capacity]. A query
  * that sees nothing (length 0) gives 0. The workspace (256-byte aligned) needs
- * no initialisation; calls that share one must be ordered on one stream. */
+ * no initialisation; calls that share one must be ordered on one stream. out
+ * may not overlap an input. */
 int tsa_paged_decode_window(const tsa_view* out, const tsa_view* query, const tsa_view* k_cache,
                             const tsa_view* v_cache, const tsa_view* k_scale, const tsa_view* v_scale,
                             const tsa_view* block_tables, const tsa_view* seq_lens, int64_t window,

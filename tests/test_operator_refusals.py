@@ -151,3 +151,20 @@ def test_argument_counts_of_the_extension():
     assert rc == INVALID and b"multiple" in _lib.load().tsa_last_error()
     rc = _lib.call("tsa_paged_decode", q, q, kc, kc, bt, sl, 0.1, 0, 0, 0, 0)  # the 16-bit decode takes no 8-bit cache
     assert rc == INVALID and b"floating" in _lib.load().tsa_last_error()
+
+
+@pytest.mark.parametrize("shape", [
+    (65535, 1, 65535, 65535, 128, 1 << 20, 64, 0, 0),
+    (65535, 1, 65535, 1, 512, (1 << 27) - 1, 1, 0, 0),
+    (65535, 1 << 40, 65535, 1, 128, 1 << 20, 64, 0, 0),
+    (1, 1 << 30, 64, 8, 128, 1 << 26, 1, 0, 0),
+    (4097, 1, 32, 8, 128, 1024, 16, 0, 0),
+    (8193, 1, 32, 8, 128, 1024, 16, 1000, 70000),
+])
+def test_workspace_of_large_calls(shape):
+    """Sizes stay within what the sequences of one launch need, however large the batch and the table."""
+    size = _lib.load().tsa_paged_rows_workspace_bytes(*shape)
+    b, _, hq, hkv, d = shape[:5]
+    g = min(hq // hkv, 16)
+    units = min(1 << 22, min(b, 4096) * hkv * -(-(hq // hkv) // 16)) + 65536
+    assert 0 <= size <= max(units * g, 1 << 22) * (d + 4) * 4 + (1 << 20)

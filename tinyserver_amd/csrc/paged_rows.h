@@ -96,7 +96,8 @@ int check_rows(const tsa_view* out, const tsa_view* query, const tsa_view* k_cac
                const tsa_view* cu_nodes, const tsa_view* tree_mask, int64_t max_nodes, int64_t window, int64_t sinks,
                double softmax_scale, RowsArgs& a);
 
-// The plan of a decode call on the matrix cores: splits of a unit (0: the
+constexpr int kRowsMaxSeqs = 4096;  // sequences of one decode launch (the stream's prefix is in LDS)
+// The plan of a decode launch on the matrix cores: splits of a unit (0: the
 // stream, of `waves` waves) and the workspace, part_bytes of partials and the
 // stream's prefix.
 struct DecodeRowsPlan {
@@ -108,7 +109,8 @@ DecodeRowsPlan decode_rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
 // paged_rows_unit.hip, paged_rows_stream.hip: the launches (a.S, a.NW, a.part, a.pref set).
 int rows_unit_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what);
 int rows_stream_launch(const RowsArgs& a, int dt, int cache_dt, hipStream_t stream, const char* what);
-// paged_rows_tree.hip: the plan of a tree call of at most T nodes a sequence, and the launch.
+// paged_rows_tree.hip: the plan of a tree call of at most T nodes a sequence (S 0: too
+// many workgroups or rows for it), and the launch.
 struct TreeRowsPlan {
   int RT, RB, S, per_split;
   size_t bytes;

@@ -1,5 +1,7 @@
 // Attention of a few query rows per sequence over the paged cache
-// (paged_rows.h): windowed decode, decode over 8-bit caches, draft trees.
+// (paged_rows.h): windowed decode, decode over 8-bit caches, draft trees. The
+// entry points, and the form for what the matrix-core ones do not take
+// (paged_rows_unit.h, paged_rows_stream.h; paged_rows_tree.h, paged_rows_tree_lds.h).
 #include "paged_rows.h"
 
 namespace tsa {
@@ -190,6 +192,24 @@ int check_rows(const tsa_view* out, const tsa_view* query, const tsa_view* k_cac
   return TSA_OK;
 }
 
+// Sequences of one launch: within the stream's prefix, 2^22 workgroups, and
+// 2^30 tile pairs (its prefix is 32 bits).
+static int64_t decode_rows_chunk(int64_t B, int64_t Hq, int64_t Hkv, int64_t cap) {
+  const int64_t units = Hkv * ((Hq / Hkv + 15) / 16), pairs = (cap + 31) / 32 + 1;
+  int64_t n = kRowsMaxSeqs < B ? kRowsMaxSeqs : B;
+  n = n < (int64_t{1} << 22) / units ? n : (int64_t{1} << 22) / units;
+  n = n < (int64_t{1} << 30) / pairs ? n : (int64_t{1} << 30) / pairs;
+  return n < 1 ? 1 : n;
+}
+// The workspace of a decode call: of its full chunks and of the last one.
+static size_t decode_rows_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, int64_t window,
+                                int64_t sinks) {
+  const int64_t chunk = decode_rows_chunk(B, Hq, Hkv, cap);
+  const size_t full = decode_rows_plan(chunk, Hq, Hkv, D, cap, window, sinks).total;
+  const size_t last = B % chunk ? decode_rows_plan(B % chunk, Hq, Hkv, D, cap, window, sinks).total : 0;
+  return full > last ? full : last;
+}
+
 // The matrix-core forms: 16-bit queries, head_dim 64 or 128, pages of whole
 // 16-token tiles, unit-stride rows of 16-byte pieces, and strides whose offsets
 // within a page fit 31 bits (a page's own 32). Fills what they need of a.
@@ -245,17 +265,29 @@ extern "C" int tsa_paged_decode_window(const tsa_view* out, const tsa_view* quer
                           window, sinks, softmax_scale, a))
     return rc;
   if (a.B > 0 && a.Hq > 0 && takes_mfma(a, out, query, k_cache, v_cache)) {
-    const DecodeRowsPlan p = decode_rows_plan(a.B, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS, a.window, a.sinks);
-    TSA_REQUIRE(p.total == 0 || (workspace != nullptr && workspace_bytes >= p.total),
-                "workspace of %zu bytes is too small: %zu needed", workspace_bytes, p.total);
-    TSA_REQUIRE(p.total == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
-    a.S = p.S;
-    a.NW = p.waves;
-    a.part = static_cast<float*>(workspace);
-    a.pref = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + p.part_bytes);
+    const int64_t cap = int64_t{a.max_blocks} * a.BS, chunk = decode_rows_chunk(a.B, a.Hq, a.Hkv, cap);
+    const size_t need = decode_rows_bytes(a.B, a.Hq, a.Hkv, a.D, cap, a.window, a.sinks);
+    TSA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need),
+                "workspace of %zu bytes is too small: %zu needed", workspace_bytes, need);
+    TSA_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    return p.S > 0 ? rows_unit_launch(a, query->dtype, k_cache->dtype, st, "tsa_paged_decode_window")
-                   : rows_stream_launch(a, query->dtype, k_cache->dtype, st, "tsa_paged_decode_window");
+    for (int64_t b = 0; b < block_tables->size[0]; b += chunk) {  // (one chunk, but for batches past its limits)
+      RowsArgs c = a;
+      c.B = static_cast<int32_t>(block_tables->size[0] - b < chunk ? block_tables->size[0] - b : chunk);
+      c.q = static_cast<const char*>(a.q) + b * a.q_sr * dtype_bytes(query->dtype);
+      c.out = static_cast<char*>(a.out) + b * a.o_sr * dtype_bytes(query->dtype);
+      c.bt = a.bt + b * a.bt_s0;
+      c.lens = a.lens + b * a.len_s;
+      const DecodeRowsPlan p = decode_rows_plan(c.B, a.Hq, a.Hkv, a.D, cap, a.window, a.sinks);
+      c.S = p.S;
+      c.NW = p.waves;
+      c.part = static_cast<float*>(workspace);
+      c.pref = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + p.part_bytes);
+      if (int rc = p.S > 0 ? rows_unit_launch(c, query->dtype, k_cache->dtype, st, "tsa_paged_decode_window")
+                           : rows_stream_launch(c, query->dtype, k_cache->dtype, st, "tsa_paged_decode_window"))
+        return rc;
+    }
+    return TSA_OK;
   }
   return dispatch_rows(a, query->dtype, k_cache->dtype, static_cast<hipStream_t>(stream), "tsa_paged_decode_window");
 }
@@ -271,7 +303,7 @@ extern "C" int tsa_paged_tree(const tsa_view* out, const tsa_view* query, const 
     return rc;
   if (a.B > 0 && a.Hq > 0 && a.T > 0 && a.N > 0 && a.scale_log2 > 0.f && takes_mfma(a, out, query, k_cache, v_cache)) {
     const TreeRowsPlan p = tree_rows_plan(a.B, a.T, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS);
-    if (int64_t{a.B} * a.Hkv * p.S * p.RB < (int64_t{1} << 23)) {  // (a launch's threads fit 32 bits)
+    if (p.S > 0) {
       TSA_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes),
                   "workspace of %zu bytes is too small: %zu needed", workspace_bytes, p.bytes);
       TSA_REQUIRE(p.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
@@ -292,8 +324,9 @@ extern "C" size_t tsa_paged_rows_workspace_bytes(int64_t num_seqs, int64_t max_n
       max_blocks_per_seq * block_size >= (int64_t{1} << 27))
     return 0;  // (calls of such sizes are refused, or have nothing to do)
   const int64_t cap = max_blocks_per_seq * block_size;
-  const size_t decode = decode_rows_plan(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks).total;
+  const size_t decode = decode_rows_bytes(num_seqs, num_heads, num_kv_heads, head_dim, cap, window, sinks);
   if (window > 0 || sinks > 0) return decode;
+  max_nodes = max_nodes < 65536 ? max_nodes : 65536;  // (the widest mask's)
   const size_t tree = tree_rows_plan(num_seqs, max_nodes, num_heads, num_kv_heads, head_dim, cap).bytes;
   return max_nodes > 1 ? tree : tree > decode ? tree : decode;
 }

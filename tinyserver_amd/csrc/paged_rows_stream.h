@@ -22,7 +22,6 @@
 namespace tsa {
 
 constexpr int kStreamWaves = 4;
-constexpr int kStreamMaxSeqs = 4096;  // tile-pair prefix in LDS
 
 struct StreamCur {
   int s, k, n, t;  // sequence, unit of the sequence (kv head x group), its pairs, the pair

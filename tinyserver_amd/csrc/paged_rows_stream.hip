@@ -3,16 +3,15 @@
 
 namespace tsa {
 
-#ifndef TSA_ROWS_RING8
-#define TSA_ROWS_RING8 3
-#endif
-#ifndef TSA_ROWS_RING16
-#define TSA_ROWS_RING16 2
-#endif
+// Tile pairs a wave keeps in registers. e4m3, 64 x 512-4096 / 32 x 32768 tokens:
+// three 64.0 / 348 us, four 66.4 / 351, six 69.4 / 353; bf16, window 1024 + 4 of
+// 64: two 51.8, three 55.0, four 54.5, five 59.1 (more have to land before the
+// first is computed).
+constexpr int kRing8 = 3, kRing16 = 2;
 
 template <typename T, typename C, int D>
 static int launch_stream(const RowsArgs& a, hipStream_t stream, const char* what) {
-  constexpr int RING = kIs8<C> ? TSA_ROWS_RING8 : TSA_ROWS_RING16;
+  constexpr int RING = kIs8<C> ? kRing8 : kRing16;
   const int groups = (a.G + 15) / 16, units = a.Hkv * groups, rows = a.G < 16 ? a.G : 16;
   paged_rows_stream<T, C, D, RING><<<dim3(a.NW / kStreamWaves), dim3(64 * kStreamWaves), (2 * a.B + 1) * sizeof(int32_t), stream>>>(
       a, a.bt, a.lens, a.part, a.pref);

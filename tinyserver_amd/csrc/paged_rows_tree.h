@@ -149,9 +149,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
     for (int i = 0; i < mine; ++i) {
       const int blk = b0 + kg + KG * i;
       const uint32_t okb = static_cast<uint32_t>(ok64 >> (2 * (i & 31))) & 3u;
-      const uint64_t ok_cur = ok64;
-      const int page_cur = my_page, slot_cur = my_slot;
-      (void)ok_cur; (void)page_cur; (void)slot_cur;
       f32x16 sc;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = 0.f;

@@ -3,21 +3,21 @@
 
 namespace tsa {
 
-// Split calls of up to this many workgroups take the unit form.
-#ifndef TSA_ROWS_UNIT_MAX
-#define TSA_ROWS_UNIT_MAX 2048
-#endif
-constexpr int64_t kUnitMaxWorkgroups = TSA_ROWS_UNIT_MAX;
-#ifndef TSA_ROWS_STREAM_PER_CU
-#define TSA_ROWS_STREAM_PER_CU 1
-#endif
-// The stream's grid: a four-wave workgroup a CU.
+// Split calls of up to this many workgroups take the unit form. Both sides, 32/8
+// heads, e4m3 / bf16, us, unit form against stream: 16 x 256-1024 tokens (512
+// workgroups) 10.9 / 14.4 against 14.5 / 17.2; 16 x 512-2048 (1024) 17.2 / 20.6
+// against 18.4 / 22.3; 64 x 256-1024 (2048) 23.6 / 31.2 against 26.2 / 33.5; 16 x
+// 1024-4096 (2048) 26.3 / 37.4 against 26.7 / 36.1; 4 x 8192-32768 (4096) 47.5 /
+// 72 against 40 / 60.
+constexpr int64_t kUnitMaxWorkgroups = 2048;
+// The stream's grid: a four-wave workgroup a CU (two a CU, e4m3, 64 x 512-4096
+// tokens: 68.5 us against 64.0; 32 x 32768: 361 against 348).
 static int stream_workgroups() {
   int dev = 0, cus = 0;
   if (hipGetDevice(&dev) != hipSuccess ||
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
     cus = 256;
-  return TSA_ROWS_STREAM_PER_CU * cus;
+  return cus;
 }
 
 // Units of this many splits or more read K/V with non-temporal loads.
@@ -71,7 +71,7 @@ DecodeRowsPlan decode_rows_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
   auto align = [](size_t n) { return (n + 255) & ~size_t{255}; };
   DecodeRowsPlan p{};
   const int64_t S = tiles <= kUnitWavesOne * kUnitTiles ? 1 : (tiles + kUnitWavesSplit * kUnitTiles - 1) / (kUnitWavesSplit * kUnitTiles);
-  if (S == 1 || items * S <= kUnitMaxWorkgroups || B > kStreamMaxSeqs) {
+  if (S == 1 || items * S <= kUnitMaxWorkgroups) {
     p.S = static_cast<int>(S);
     p.total = p.part_bytes = S == 1 ? 0 : align(static_cast<size_t>(B * Hkv * S * G) * (D + 4) * sizeof(float));
     return p;

@@ -25,7 +25,8 @@ def _workspace(dev: torch.device, *shape) -> torch.Tensor | None:
     if n is None:
         if len(_WS_BYTES) >= 4096:
             _WS_BYTES.clear()
-        n = _WS_BYTES[key] = int(_lib.load().tsa_paged_rows_workspace_bytes(*shape))
+        with torch.cuda.device(dev):  # (the stream's waves are those of the device's CUs)
+            n = _WS_BYTES[key] = int(_lib.load().tsa_paged_rows_workspace_bytes(*shape))
     return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
 
 
