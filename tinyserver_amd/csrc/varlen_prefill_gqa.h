@@ -74,6 +74,12 @@ int prefill_f32_launch(const PrefillArgs& a, hipStream_t stream);
 constexpr int max_persist_seqs(int nw) { return nw == 2 ? 1024 : 2048; }
 
 constexpr float kNegInfP = -INFINITY;
+// x if bit i of bits is set, else -inf: two instructions (v_bfe_i32, v_bfi_b32),
+// where a compare and a select take three and a wait for vcc.
+__device__ __forceinline__ float masked_score(float x, uint32_t bits, int i) {
+  const uint32_t keep = static_cast<uint32_t>(static_cast<int32_t>(bits << (31 - i)) >> 31);
+  return __uint_as_float((keep & __float_as_uint(x)) | (~keep & 0xFF800000u));
+}
 
 // [start, end) of sequence b in a packed tensor of n tokens; out-of-range
 // cu_seqlens entries are clamped so a malformed table cannot read past it.

@@ -59,6 +59,7 @@ constexpr int w64_smem_bytes() {
   return 2 * kW64Slots * 8192 + 4 * kW64QArea + 4 * kW64OutStage + kW64MaxSeqs * 2 + kPlanItems * 6 * 4 +
          kPlanLevels * 4;
 }
+constexpr int w64_window_smem_bytes() { return w64_smem_bytes() + 512; }
 
 // Register homes. The output accumulators (2 x 64 fp32 per lane) live in
 // AGPRs, where the P.V MFMAs (builtins) accumulate them; Q lives in AGPRs
@@ -149,6 +150,10 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
   uint16_t* const nqt_s = reinterpret_cast<uint16_t*>(smem + COFF);
   int32_t* const plan_s = reinterpret_cast<int32_t*>(smem + PLOFF);
   int32_t* const lev_s = reinterpret_cast<int32_t*>(smem + LVOFF);
+  // (window) this wave's rounds whose rows are computed again, a bit each (the
+  // last bit: all rounds from kRedo - 1 on).
+  constexpr int kRedo = 1024;
+  static_assert(w64_window_smem_bytes() == w64_smem_bytes() + 4 * kRedo / 8, "LDS layout and its size agree");
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -156,6 +161,10 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
   const int HG = a.G / 4;      // q-head groups per kv head
   const int HH = a.Hkv * HG;   // items per (sequence, query tile)
   const float cs = a.scale_log2;  // > 0 on this path
+  uint32_t* const redo_s = reinterpret_cast<uint32_t*>(smem + w64_smem_bytes()) + wave * (kRedo / 32);
+  if constexpr (kWindow<Args>) {
+    if (lane < kRedo / 32) redo_s[lane] = 0;
+  }
 
   // ---- Work items (64-query tile, sequence, kv head, head group), heaviest
   // tiles first: level Q holds tile Q of every sequence that has one, in
@@ -189,9 +198,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     const T* kb;
     const T* vb;
     T* ob;
-    WindowBlocks win;  // (window) the blocks; the rest: for rows computed again
-    int64_t q_start, k_start;
-    int head;
+    WindowBlocks win;  // (window) the blocks
   };
   auto block_at = [&](const Item& it, int v) __attribute__((always_inline)) {
     if constexpr (kWindow<Args>) return it.win.at(v);
@@ -216,15 +223,12 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
       it.win = window_blocks(a, it.q0, q_last, it.k_len);
       it.nblk = it.win.count;
       it.kfull = min(it.k_len, it.win.end);
-      it.q_start = qs;
-      it.k_start = ks;
-      it.head = head;
     }
     (void)b;
   };
   // Item i -> level Q (the smallest with items_above(Q) <= i), then the
   // sequence of rank (i - items_above(Q)) / HH among those with nqt > Q.
-  auto resolve = [&](int i, Item& it) {
+  auto locate = [&](int i, auto use) __attribute__((always_inline)) {
     int lo = 0, hi = qt_max - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -251,7 +255,12 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     int64_t qs, ql, ks, kl;
     seq_range(cu_q, a.cuq_s, b, a.total_q, qs, ql);
     seq_range(cu_k, a.cuk_s, b, a.total_k, ks, kl);
-    fill_item(it, b, hh, Q, qs, ql, ks, kl);
+    use(b, hh, Q, qs, ql, ks, kl);
+  };
+  auto resolve = [&](int i, Item& it) {
+    locate(i, [&](int b, int hh, int Q, int64_t qs, int64_t ql, int64_t ks, int64_t kl) __attribute__((always_inline)) {
+      fill_item(it, b, hh, Q, qs, ql, ks, kl);
+    });
   };
   // The item plan (as varlen_prefill_gqa's): for at most kPlanSeqs sequences
   // and kPlanLevels tile levels, wave 0 resolves kPlanItems rounds at a
@@ -502,7 +511,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
       const uint32_t bits = window_bits(a, it.q0 + 32 * t + c, 32 * it.win.at(blk), it.k_len) >> (4 * h);
 #pragma unroll
       for (int e = e0; e < e1; ++e)
-        if (!(bits & (1u << (8 * (e >> 2) + (e & 3))))) sc[t][e] = kNegInfP;
+        sc[t][e] = masked_score(sc[t][e], bits, 8 * (e >> 2) + (e & 3));
       return;
     }
     const int base = blk * 32 + 4 * h;
@@ -649,7 +658,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
   // stores follow one round later. Rows past q_len are not stored. The stores
   // are non-temporal: the output is not read again here, and allocating it
   // in L2 evicts K/V lines that later items re-read (measured 4% slower).
-  auto store_out = [&](const Item& it) {
+  auto store_out = [&](const Item& it, [[maybe_unused]] int k) {  // (k: its round)
     xdl_to_valu_nops();  // the last P.V MFMAs wrote the accumulators
     char* const ost = smem + OOFF + wave * kW64OutStage;
     const int rr = lane >> 3, ch = lane & 7;  // read-back: rows rr + 8i, chunk ch
@@ -718,13 +727,8 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     }
     flush();
     if constexpr (kWindow<Args>) {
-      if (__any(finite != 0.f)) {  // (uniform)
-        wait_vmcnt<0>();  // those stores first
-        const int last = min(it.q_len, it.q0 + 64);
-#pragma unroll 1
-        for (int qq = it.q0; qq < last; ++qq)
-          prefill_window_row<T>(a, it.q_start + qq, qq, it.head, it.k_start, it.k_len);
-      }
+      const int r = min(k, kRedo - 1);
+      if (__any(finite != 0.f) && lane == 0) redo_s[r >> 5] |= 1u << (r & 31);
     }
   };
 
@@ -810,11 +814,22 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
         lsum1(1, s2);
       }
     }
-    store_out(X);
+    store_out(X, round - 1);
     X = Y;
     idx = nidx;
   }
   wait_loads(integral_constant<int, 0>{});
+  if constexpr (kWindow<Args>) {  // (that wait was for the outputs' stores too)
+#pragma unroll 1
+    for (int k = 0; item_of(k) < n_items; ++k) {
+      if (!((__builtin_amdgcn_readfirstlane(redo_s[min(k, kRedo - 1) >> 5]) >> (min(k, kRedo - 1) & 31)) & 1)) continue;
+      locate(item_of(k), [&](int, int hh, int Q, int64_t qs, int64_t ql, int64_t ks, int64_t kl) {
+        const int head = hh / HG * a.G + hh % HG * 4 + wave, last = min(static_cast<int>(ql), 64 * Q + 64);
+#pragma unroll 1
+        for (int qq = 64 * Q; qq < last; ++qq) prefill_window_row<T>(a, qs + qq, qq, head, ks, kl);
+      });
+    }
+  }
   (void)kQLoads;
 }
 

@@ -31,7 +31,7 @@ int prefill_w64_launch(const PrefillArgs& a, bool bf16, hipStream_t stream) {
 template <typename T>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void varlen_window_w64(
     PrefillWindowArgs a, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k) {
-  __shared__ __align__(16) char smem[w64_smem_bytes()];
+  __shared__ __align__(16) char smem[w64_window_smem_bytes()];
   prefill_w64_body<T>(a, cu_q, cu_k, smem);
 }
 
