@@ -39,9 +39,16 @@
 // kW64A steps ahead through kW64Slots slots.
 //
 // With PrefillWindowArgs (a sliding window and first tokens) an item's blocks are
-// those that its 64 queries see (window_blocks), and a wave whose outputs are
-// not all finite computes its rows again over visible keys alone, as in
-// prefill_gqa_body.
+// those that its 64 queries see (window_blocks). The next item's Q is loaded
+// during this one's blocks (peek_q): windowed items are alike, so without it the
+// workgroups all load Q at once between items (16 prompts of 2048 tokens, 32/8
+// heads, window 32 / 512: 252 / 441 us without, 226 / 425 with). An item whose
+// outputs are not all finite is marked, and its rows are computed again over
+// visible keys alone after the item loop (inlined at the item's end that cost 50
+// spilled registers: 16 prompts of 128-2048 tokens, window 512 + 4, 294 us against
+// 261). At window 512 an item of 19 blocks takes 58k cycles: 43k the blocks (five
+// masked half-iterations 1.2k more than the others), 3k the first scores, 6k the
+// output.
 #pragma once
 
 #include <type_traits>
@@ -310,7 +317,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
   };
   auto resolve_round = [&](int k, int i, Item& it) {
     if (planned) {
-      if (k % kPlanItems == 0) make_plan(k);
+      if (k % kPlanItems == 0 && (!kWindow<Args> || k == 0)) make_plan(k);  // (window: peek_q made the later ones)
       const int32_t* const e = plan_s + 6 * (k % kPlanItems);
       const int w0 = __builtin_amdgcn_readfirstlane(e[0]);
       const int Q = __builtin_amdgcn_readfirstlane(e[1]);
@@ -424,6 +431,35 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     }
   };
   constexpr int kQLoads = 2 * KJ;
+  // (window) The next item's Q, while this one's blocks are computed: its rows are
+  // in registers by then, and a windowed call's items are alike, so its
+  // workgroups, all at the same place, would ask for Q at once and wait for it
+  // (12-15k of the 62k cycles of an item of 19 blocks). Part p of 8: rows 8p ..
+  // 8p + 7, as dma_q lays them out. rows: the last row, from the item's first.
+  struct NextQ {
+    const char* p;
+    int last;  // < 0: not known yet (calls without a plan)
+  };
+  auto peek_q = [&](int k) __attribute__((always_inline)) {
+    NextQ n{nullptr, -1};
+    const int i = item_of(k);
+    if (!planned || i >= n_items) return n;
+    if (k % kPlanItems == 0) make_plan(k);
+    const int32_t* const e = plan_s + 6 * (k % kPlanItems);
+    const int hh = __builtin_amdgcn_readfirstlane(e[0]) >> 16, q0 = 64 * __builtin_amdgcn_readfirstlane(e[1]);
+    const int64_t qs = __builtin_amdgcn_readfirstlane(e[2]);
+    const int kvh = hh / HG, head = kvh * a.G + (hh - kvh * HG) * 4 + wave;
+    n.p = static_cast<const char*>(a.q) + ((qs + q0) * a.q_st + head * a.q_sh) * static_cast<int64_t>(sizeof(T));
+    n.last = __builtin_amdgcn_readfirstlane(e[3]) - 1 - q0;
+    return n;
+  };
+  auto dma_q_part = [&](const NextQ& n, int p) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t row = static_cast<uint32_t>(min(8 * p + 4 * u + lrow, n.last));
+      dma16_sv(n.p, row * static_cast<uint32_t>(qst_b) + (q_cpart ^ (16u * ((2 * p + u) & 3))), q_lds + 2048 * p + 1024 * u);
+    }
+  };
   auto wait_loads = [&](auto n) { wait_vmcnt<decltype(n)::value>(); };
 
   // K operands of the block in slot ks: lane (h, c) reads key c, dims
@@ -548,6 +584,8 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
   // accumulators are scaled by 2^(m_old - m_new). Until a tile's first key,
   // l and the accumulators are zero and only m moves.
   auto rescale_check = [&](int t) __attribute__((always_inline)) {
+    // (window: rows meet their first key at different blocks, and have nothing to scale there)
+    if constexpr (kWindow<Args>) m[t] = m[t] == kNegInfP ? mt[t] : m[t];
     if (__any(mt[t] > m[t] + kRescale)) {
       const float m_new = fmaxf(m[t], mt[t]);
       if (!__all(m[t] == kNegInfP)) {
@@ -631,16 +669,23 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
   // last iteration the K(j + 1) read and QK0(j+1) are not used (the slot
   // holds a clamped copy of the last block). S is the slot phase j % NB, a
   // compile-time constant.
-  auto iter = [&](const Item& it, int j, auto S) __attribute__((always_inline)) {
+  // (window) A part of the next item's Q goes out with step j + A for j < 8: from
+  // iteration A to 8 just A parts are behind step j's loads.
+  auto iter = [&](const Item& it, int j, auto S, [[maybe_unused]] const NextQ& nq) __attribute__((always_inline)) {
     // Step j has landed for every wave: wait for this wave's loads of it,
     // meet the others, then issue step j + A (its slots were last read in
     // iteration j + A - NB < j, before this barrier).
     const bool issue = j + A < it.nblk;
-    if (issue) wait_loads(std::integral_constant<int, kInFlight>{});
+    if (kWindow<Args> && issue && nq.last >= 0 && j >= A && j <= 8)
+      wait_loads(std::integral_constant<int, kInFlight + 2 * A>{});
+    else if (issue) wait_loads(std::integral_constant<int, kInFlight>{});
     else wait_loads(std::integral_constant<int, 0>{});
     lds_barrier();
     constexpr int s = decltype(S)::value;
     if (issue) load_step_c(it, j, S);
+    if constexpr (kWindow<Args>) {
+      if (nq.last >= 0 && j < 8) dma_q_part(nq, j);
+    }
     half(it, 0, j, std::integral_constant<int, (s + 1) % NB>{}, std::integral_constant<int, -1>{}, true);
     half(it, 1, j + 1, std::integral_constant<int, -1>{}, S, true);
   };
@@ -666,7 +711,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     char* pend_p[4];
     bool pend_ok[4];
     bool pend_full = true, have = false;
-    float finite = 0.f;  // (window) NaN where a sum is not finite
+    float finite[4] = {0.f, 0.f, 0.f, 0.f};  // (window) NaN where a sum is not finite
     auto flush = [&]() __attribute__((always_inline)) {
       if (pend_full) {
 #pragma unroll
@@ -682,7 +727,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
       const float l0 = __shfl(lacc[t][0], c & 15, 64), l1 = __shfl(lacc[t][1], c & 15, 64);
       const float den = c < 16 ? l0 : l1;
       const float rl = kWindow<Args> && den == 0.f ? 0.f : 1.f / den;  // 1 / query c's denominator (window: nothing seen, 0)
-      if constexpr (kWindow<Args>) finite = fmaf(den, 0.f, finite);
+      if constexpr (kWindow<Args>) finite[t] = fmaf(den, 0.f, finite[t]);
       const int rbase = it.q0 + 32 * t;
       const bool full = rbase + 32 <= it.q_len;
       char* rowp[4];
@@ -702,7 +747,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
             const int u = 2 * half + uu;
             if constexpr (kWindow<Args>) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) finite = fmaf(acc[t][u][4 * g + i], 0.f, finite);
+              for (int i = 0; i < 4; ++i) finite[i] = fmaf(acc[t][u][4 * g + i], 0.f, finite[i]);
             }
             const u32x2 w = {pack2<T>(acc[t][u][4 * g] * rl, acc[t][u][4 * g + 1] * rl),
                              pack2<T>(acc[t][u][4 * g + 2] * rl, acc[t][u][4 * g + 3] * rl)};
@@ -728,7 +773,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     flush();
     if constexpr (kWindow<Args>) {
       const int r = min(k, kRedo - 1);
-      if (__any(finite != 0.f) && lane == 0) redo_s[r >> 5] |= 1u << (r & 31);
+      if (__any((finite[0] + finite[1]) + (finite[2] + finite[3]) != 0.f) && lane == 0) redo_s[r >> 5] |= 1u << (r & 31);
     }
   };
 
@@ -775,6 +820,8 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     }
     loop_loads_start(X);
     const int n = X.nblk;
+    NextQ nq{nullptr, -1};
+    if constexpr (kWindow<Args>) nq = peek_q(round + 1);
     // P1(-1) V(-1) of the first iteration adds zeros.
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
@@ -784,13 +831,13 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     }
     // Iterations 0 .. n-1, unrolled by slot phase.
     for (int j = 0; j < n;) {
-      iter(X, j, integral_constant<int, 0>{});
+      iter(X, j, integral_constant<int, 0>{}, nq);
       if (++j == n) break;
-      iter(X, j, integral_constant<int, 1>{});
+      iter(X, j, integral_constant<int, 1>{}, nq);
       if (++j == n) break;
-      iter(X, j, integral_constant<int, 2>{});
+      iter(X, j, integral_constant<int, 2>{}, nq);
       if (++j == n) break;
-      iter(X, j, integral_constant<int, 3>{});
+      iter(X, j, integral_constant<int, 3>{}, nq);
       ++j;
     }
     // Every wave has read X's last K/V block (in H0 of the last iteration)
@@ -801,7 +848,12 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     Item Y;
     if (nidx < n_items) {
       resolve_round(round, nidx, Y);
-      dma_q(Y);
+      if (kWindow<Args> && nq.last >= 0) {
+#pragma unroll 1
+        for (int p = min(n, 8); p < 8; ++p) dma_q_part(nq, p);
+      } else {
+        dma_q(Y);
+      }
       load_head(Y);
     }
     // X's last P.V of tile 1 (V(n-1) and P1(n-1) are in registers), then

@@ -40,9 +40,10 @@ template <typename T>
 static int launch_window_mfma(PrefillWindowArgs& a, int64_t max_seqlen_q, hipStream_t stream) {
   // Groups of eight keep the eight waves of the LDS-staged kernel, which stage
   // each K/V block once for all of them: 16 prompts of 128-2048 tokens, 64/8
-  // heads, window 128 / 512: 296 / 460 us against 398 / 551 with 64 queries a
-  // wave (one of 16384, window 4096: 1892 against 1900). Groups of four take 64
-  // queries a wave: 229 / 364 -> 197 / 279.
+  // heads, window 128 / 512: 293 / 460 us against 309 / 477 with 64 queries a
+  // wave (four of 100-700: 34 / 35 against 35 / 39; one of 16384: 275 / 443
+  // against 242 / 422, window 4096 + 16: 1892 against 1874). Groups of four take
+  // 64 queries a wave: 228 / 364 -> 164 / 262.
   if (prefill_takes_w64(a) && a.G != 8)
     return prefill_w64_window_launch(a, std::is_same<T, bf16_t>::value, stream);
   if (prefill_takes_gqa(a)) {
