@@ -5,8 +5,8 @@
 namespace tsa {
 
 // Workgroups a call's units are split into, at least, where there are tokens for
-// it (64 sequences of 512-4096 tokens, 32 nodes, 32/8 heads: 512 159 us, 1024 187,
-// 2048 190; 8 of 8192 with 64 nodes, 64/8 heads: 173, 192, 238; 256 are alike), and
+// it (64 sequences of 512-4096 tokens, 16 nodes, 32/8 heads: 512 138 us, 768 161;
+// 32 nodes: 156, 183; 8 of 8192 with 64 nodes, 64/8 heads: 169, 181; 256 are as 512), and
 // the least blocks of a split (one sequence of 300 tokens: 16 14.9 us, 4 18.1).
 constexpr int64_t kTreeWorkgroups = 512, kTreeMinSplit = 16;
 

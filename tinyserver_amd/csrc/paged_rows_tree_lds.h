@@ -12,8 +12,8 @@
 // prefill_gqa_body's; the rows, the pages, the masks and what is written differ.
 // The pipeline takes the blocks that every row sees whole; those from the
 // context's end on (or from a page outside the pool) follow one at a time.
-// At up to 256 registers two waves share a SIMD, so one's exponentials run
-// under the other's products.
+// Of four waves, two workgroups give a SIMD two waves of up to 256 registers, and
+// one's exponentials run under the other's products.
 #pragma once
 
 #include "paged_rows_tree.h"
@@ -21,20 +21,23 @@
 namespace tsa {
 
 constexpr int kTreeMaxSplit = 256;  // 32-key blocks of a split: its page table in LDS
-template <int NW> constexpr int kTreeSlots = NW == 2 ? 2 : 4;
-template <int D, int NW> constexpr int tree_lds_bytes() { return 2 * kTreeSlots<NW> * 32 * 2 * D + kTreeMaxSplit * 8 + 16; }
+// K/V slots: two workgroups fit a CU, which is what the plan's 512 give it, with
+// three blocks each in flight (64 sequences of 512-4096 tokens, 16 nodes, 32/8
+// heads: four 138 us, two, with four workgroups to a CU, 155).
+constexpr int kTreeSlots = 4;
+template <int D> constexpr int tree_lds_bytes() { return 2 * kTreeSlots * 32 * 2 * D + kTreeMaxSplit * 8 + 16; }
 
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void paged_rows_tree_lds(
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 2 ? 1 : 2))) void paged_rows_tree_lds(
     RowsArgs a, const int32_t* __restrict__ bt, const uint32_t* __restrict__ mask, float* __restrict__ part) {
   constexpr int KJ = D / 16, NU = D / 32, CPR = D / 8, RB = 2 * D, BLKB = 32 * RB, PF = part_floats(D);
-  constexpr int NB = kTreeSlots<NW>, A = NB - 1;
+  constexpr int NB = kTreeSlots, A = NB - 1;
   constexpr int RPI = 1024 / RB;            // rows of a 1 KB load instruction
   constexpr int IPW = 2 * (32 / RPI) / NW;  // load instructions of a wave and block
   constexpr int IPH = 16 / RPI;             // load instructions of a 16-row half
   constexpr int VOFF = NB * BLKB, TOFF = 2 * NB * BLKB;
   constexpr int kInFlight = (A - 1) * IPW;
-  __shared__ __align__(16) char smem[tree_lds_bytes<D, NW>()];
+  __shared__ __align__(16) char smem[tree_lds_bytes<D>()];
   int32_t* const tab = reinterpret_cast<int32_t*>(smem + TOFF);  // page id of each half of the split's blocks, -1: none
   int32_t* const first_bad = tab + 2 * kTreeMaxSplit;            // the first block with such a half
 
@@ -317,17 +320,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       lds_barrier();  // iteration 0's loads overwrite K(0)'s slot
       full(0, integral_constant<int, 0>{}, std::false_type{});
       for (int j = 1; j < n1;) {
-        full(j, integral_constant<int, 1 % NB>{}, std::true_type{});
+        full(j, integral_constant<int, 1>{}, std::true_type{});
         if (++j == n1) break;
-        full(j, integral_constant<int, 2 % NB>{}, std::true_type{});
+        full(j, integral_constant<int, 2>{}, std::true_type{});
+        if (++j == n1) break;
+        full(j, integral_constant<int, 3>{}, std::true_type{});
+        if (++j == n1) break;
+        full(j, integral_constant<int, 0>{}, std::true_type{});
         ++j;
-        if constexpr (NB == 4) {
-          if (j == n1) break;
-          full(j, integral_constant<int, 3>{}, std::true_type{});
-          if (++j == n1) break;
-          full(j, integral_constant<int, 0>{}, std::true_type{});
-          ++j;
-        }
       }
       if (active) pv();
     }
