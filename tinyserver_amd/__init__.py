@@ -2,7 +2,8 @@
 
 Four hand-written HIP kernels behind a C ABI (include/tsa_api.h, libtsa.so):
 fused QK RMSNorm + RoPE, the paged K/V store, paged GQA decode attention and
-varlen causal prefill. ``tinyserver_amd.kernels`` mirrors the reference's
+varlen causal prefill; beside them an 8-bit paged cache, attention with a
+sliding window, and attention of drafted tokens' trees. ``tinyserver_amd.kernels`` mirrors the reference's
 kernel modules; ``tinyserver_amd.patches.qwen3`` mirrors its Qwen3 attention
 patch.
 """
