@@ -320,7 +320,8 @@ size_t tsa_paged_rows_workspace_bytes(int64_t num_seqs, int64_t max_nodes, int64
  * pool is not seen; lengths are taken within [0, the table's capacity]. A query
  * that sees nothing (length 0) gives 0. The workspace (256-byte aligned) needs
  * no initialisation; calls that share one must be ordered on one stream. out
- * may not overlap an input. */
+ * may not overlap an input. A seen value of V that is not finite makes the
+ * output of its dim not finite (an infinity may come out as NaN). */
 int tsa_paged_decode_window(const tsa_view* out, const tsa_view* query, const tsa_view* k_cache,
                             const tsa_view* v_cache, const tsa_view* k_scale, const tsa_view* v_scale,
                             const tsa_view* block_tables, const tsa_view* seq_lens, int64_t window,
@@ -333,8 +334,8 @@ int tsa_paged_decode_window(const tsa_view* out, const tsa_view* query, const ts
  * context_lens[s] + i. Node i sees the first context_lens[s] tokens and the
  * nodes j whose bit is set in its row of tree_mask (N, words) int64: bit j %
  * 64 of word j / 64 (a node sees itself only by its own bit). At most
- * max_nodes rows a sequence are computed, and no more than the mask has bits;
- * rows past those, and rows outside every sequence, are left as they were. A
+ * max_nodes rows a sequence are computed, and no more than the mask has bits
+ * (nodes past max_nodes are still keys for the others); rows past those, and rows outside every sequence, are left as they were. A
  * node that sees nothing gives 0. Page ids, lengths and the workspace as
  * tsa_paged_decode_window's. */
 int tsa_paged_tree(const tsa_view* out, const tsa_view* query, const tsa_view* k_cache,

@@ -122,6 +122,27 @@ def test_a_draft_behind_the_stored_nodes():
             row += 1
 
 
+@pytest.mark.parametrize("hq,d,dtype", [(8, 128, BF), (32, 128, BF), (4, 64, F16), (6, 80, BF)])
+def test_a_node_that_sees_one_past_max_nodes(hq, d, dtype):
+    """Only the first 3 rows of a sequence are computed; they may see its later nodes."""
+    hkv, page, ctx, nodes = 2, 16, [30, 5], [7, 40]
+    kc, vc, bt = pool([a + b for a, b in zip(ctx, nodes)], hkv, d, page, 9)
+    kc, vc = kc.to(dtype), vc.to(dtype)
+    g = torch.Generator().manual_seed(d)
+    q = torch.randn(47, hq, d, generator=g).to(dtype)
+    mask = torch.randint(0, 1 << 40, (47,), generator=g)
+    mask[:7] &= 127
+    out = torch.full((47, hq, d), 3.0, dtype=dtype, device=DEV)
+    paged_attention_tree(q.to(DEV), kc.to(DEV), vc.to(DEV), bt.to(DEV), page, _i32(ctx), _i32([0, 7, 47]), mask.to(DEV),
+                         max_nodes=3, out=out)
+    for s, at in enumerate((0, 7)):
+        for i in range(3):
+            see = list(range(ctx[s])) + [ctx[s] + j for j in range(nodes[s]) if int(mask[at + i]) >> j & 1]
+            ref, tol = attend(q[at + i], rows(kc, bt[s], see), rows(vc, bt[s], see), d**-0.5, half_step(dtype), half_step(dtype))
+            check(out[at + i], ref, tol, f"sequence {s} node {i}")
+        assert bool((out[at + 3 : at + nodes[s]] == 3).all())
+
+
 def _step(cache, hq, batch, longest, page=16, d=128, hkv=8):
     """A decode step over an 8-bit cache, a windowed one and a draft's, on inputs that a caller overwrites."""
     g = torch.Generator(device=DEV).manual_seed(batch + longest)

@@ -217,7 +217,7 @@ static bool quant8_takes_vec(const Quant8Args& a, const PagedAddr& addr, const t
                              const tsa_view* k_cache, const tsa_view* v_cache) {
   if ((k->dtype != TSA_BF16 && k->dtype != TSA_F16) || (a.D != 64 && a.D != 128)) return false;
   if (!rows_vec16(k) || !rows_vec16(v) || addr.nseq < 1 || addr.nseq > kQuant8LdsSeqs) return false;
-  if (addr.max_blocks >= (int64_t{1} << 31) / a.BS || a.T >= (int64_t{1} << 31)) return false;
+  if (addr.max_blocks >= (int64_t{1} << 31) / a.BS || a.T >= (int64_t{1} << 27)) return false;  // (a grid of 2^32 threads)
   for (const tsa_view* x : {k_cache, v_cache}) {
     if (x->stride[3] != 1 || reinterpret_cast<uintptr_t>(x->data) % 8) return false;
     for (int d = 0; d < 3; ++d)

@@ -75,9 +75,9 @@ __device__ __forceinline__ SeqRange seq_of(const RowsArgs& a, int s) {
     int64_t r0 = a.cu[s * a.cu_s], r1 = a.cu[(s + 1) * a.cu_s];
     r0 = r0 < 0 ? 0 : r0 > a.N ? a.N : r0;
     r1 = r1 < r0 ? r0 : r1 > a.N ? a.N : r1;
-    const int64_t n = r1 - r0 < a.T ? r1 - r0 : a.T;
+    const int64_t held = 32 * static_cast<int64_t>(a.words), n = r1 - r0 < held ? r1 - r0 : held;  // (those a mask names)
     r.row0 = r0;
-    r.nodes = static_cast<int>(n);
+    r.nodes = static_cast<int>(n < a.T ? n : a.T);
     r.end = static_cast<int>(len + n < cap ? len + n : cap);
   } else {
     r.row0 = s;

@@ -1,14 +1,12 @@
 // Attention of drafted tokens' trees on the matrix cores: the rows of a unit
 // (sequence, kv head) are its nodes' q-heads of that kv head, so every K/V byte
-// read serves nodes x heads rows.
+// read serves nodes x heads rows. This kernel takes up to 32 rows a unit
+// (paged_rows_tree_lds.h the others).
 //
-// What bounds it: HBM for small trees (each K/V byte once), the matrix cores
-// and the exponentials beside them from some 200 rows a unit on. A workgroup of
-// four waves takes up to 32, 64 or 128 rows (the sequence's count decides): RT =
-// 1, 2 or 4 tiles of 32 rows and 4 / RT runs of keys, wave (rt, kg) row tile rt
-// over every (4 / RT)-th 32-key block. A unit's keys are split over workgroups,
-// whose partials a second launch merges. Row blocks of one unit and split go to
-// one XCD, one after the other, and share its L2.
+// What bounds it: HBM (each K/V byte once; 64 sequences of 512-4096 tokens, 4
+// nodes, 32/8 heads: 129 us, 4.7 TB/s). A workgroup of four waves takes a unit's
+// rows, wave kg every fourth 32-key block. A unit's keys are split over
+// workgroups, whose partials a second launch merges.
 //
 // With lane (h, c) = (lane / 32, lane % 32), v_mfma_f32_32x32x16:
 //   S^T(32 keys x 32 rows) = K Q^T over D / 16 steps: lane (h, c) reads key c,
@@ -61,21 +59,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   constexpr int KJ = D / 16, NU = D / 32, PF = part_floats(D);
   typedef typename VPiece<2 * NU>::type VP;
   __shared__ __align__(16) float slots[4 * 32 * PF];
-  // ---- Which unit, split and row block.
-  const int id = blockIdx.x, k8 = id >> 3;
-  const int rb = k8 % a.RB, us = (k8 / a.RB) * 8 + (id & 7), U = a.B * a.Hkv;
+  // ---- Which unit and split.
+  const int us = blockIdx.x, U = a.B * a.Hkv;
   if (us >= U * a.S) return;
   const int sp = us / U, u = us - sp * U, s = u / a.Hkv, kvh = u - s * a.Hkv;
   const SeqRange r = seq_of(a, s);
-  const int all = r.nodes * a.G, R = 32 * a.RT, row_first = rb * R, rows = min(all - row_first, R);
+  const int rows = r.nodes * a.G;  // up to 32
   if (rows <= 0) return;
   const int nblk = (r.end + 31) >> 5, b0 = sp * a.per_split, b1 = min(nblk, b0 + a.per_split);
   if (b0 >= b1 && a.S > 1) return;  // (the merge takes the splits that have blocks)
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int RT = rows <= 32 ? 1 : rows <= 64 ? 2 : 4, KG = 4 / RT, rt = wave % RT, kg = wave / RT;
+  constexpr int KG = 4;
+  const int kg = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const int row = min(row_first + 32 * rt + c, all - 1);  // (past the last: it again, never stored)
+  const int row = min(c, rows - 1);  // (past the last: it again, never stored)
   const int node = row / a.G, head = kvh * a.G + row - node * a.G;
   const int64_t prow = r.row0 + node;
   const uint32_t* const my_mask = mask + prow * a.mask_s;
@@ -94,7 +91,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
     for (int e = 0; e < 16; ++e) acc[x][e] = 0.f;
 
   const int mine = b0 + kg < b1 ? (b1 - b0 - kg + KG - 1) / KG : 0;  // this wave's blocks
-  if (32 * rt < rows && mine > 0) {
+  if (mine > 0) {
     // Lane 2 i + half: the page and first slot of that half of the wave's
     // block i0 + i, for 32 blocks at a time.
     int my_page = 0, my_slot = 0;
@@ -259,7 +256,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
     l += __builtin_bit_cast(float, xor_lane32<32>(__builtin_bit_cast(uint32_t, l), lane));
   }
   // ---- The waves' partials to LDS, then the runs of keys together.
-  float* const slot = slots + (wave * 32 + c) * PF;
+  float* const slot = slots + (kg * 32 + c) * PF;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const int i = 8 * (e >> 2) + 4 * h + (e & 3);
@@ -275,7 +272,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
     const int rr = idx / (D / 2), d = 2 * (idx - rr * (D / 2));
     float M = kNegInfR, den = 0.f, o0 = 0.f, o1 = 0.f;
     for (int g = 0; g < KG; ++g) {
-      const float* const x = slots + (((rr >> 5) + RT * g) * 32 + (rr & 31)) * PF;
+      const float* const x = slots + (32 * g + rr) * PF;
       const f32x2 v = *reinterpret_cast<const f32x2*>(x + d), ml = *reinterpret_cast<const f32x2*>(x + D);
       const float mn = fmaxf(M, ml[0]), mu = mn == kNegInfR ? 0.f : mn;
       const float c_old = fast_exp2(M - mu), c_new = fast_exp2(ml[0] - mu);
@@ -284,14 +281,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
       den = fmaf(ml[1], c_new, den * c_old);
       M = mn;
     }
-    const int gr = row_first + rr;
     if (a.S == 1) {
-      const int nd = gr / a.G;
-      T* const out = static_cast<T*>(a.out) + (r.row0 + nd) * a.o_sr + (kvh * a.G + gr - nd * a.G) * a.o_sh;
+      const int nd = rr / a.G;
+      T* const out = static_cast<T*>(a.out) + (r.row0 + nd) * a.o_sr + (kvh * a.G + rr - nd * a.G) * a.o_sh;
       out[d * a.o_sd] = from_float<T>(den == 0.f ? 0.f : o0 / den);
       out[(d + 1) * a.o_sd] = from_float<T>(den == 0.f ? 0.f : o1 / den);
     } else {
-      float* const out = part + ((static_cast<int64_t>(u) * a.S + sp) * (a.T * a.G) + gr) * PF;
+      float* const out = part + ((static_cast<int64_t>(u) * a.S + sp) * (a.T * a.G) + rr) * PF;
       *reinterpret_cast<f32x2*>(out + d) = f32x2{o0, o1};
       if (d == 0) *reinterpret_cast<f32x2*>(out + D) = f32x2{M, den};
     }

@@ -26,7 +26,7 @@ TreeRowsPlan tree_rows_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64
   p.per_split = static_cast<int>(per < 4 ? 4 : per);
   p.S = static_cast<int>((blocks + p.per_split - 1) / p.per_split);
   if (p.S < 1) p.S = 1;
-  if (wgs * p.S >= (int64_t{1} << 22) || rows > (int64_t{1} << 18)) return TreeRowsPlan{};  // (grids' limits)
+  if (wgs * p.S >= (int64_t{1} << 22) || rows > 65536) return TreeRowsPlan{};  // (grids' limits)
   p.bytes = p.S == 1 ? 0 : static_cast<size_t>(B * Hkv * p.S) * static_cast<size_t>(rows) * (D + 4) * sizeof(float);
   return p;
 }
