@@ -112,6 +112,9 @@ constexpr int gqa_smem_bytes() {
   return 2 * (NW == 2 ? 2 : 4) * (32 * 2 * D) + NW * kOutStage + max_persist_seqs(NW) * 2 +
          kPlanItems * 6 * 4 + kPlanLevels * 4;
 }
+// With a window: and 1024 bits a wave.
+template <int D, int NW>
+constexpr int gqa_window_smem_bytes() { return gqa_smem_bytes<D, NW>() + NW * 128; }
 
 // LDS-staged GQA flash attention on 32x32 tiles, persistent. A work item is
 // one kv head of one sequence and 32 queries; a workgroup of NW = G waves
@@ -149,8 +152,8 @@ constexpr int gqa_smem_bytes() {
 // (window_blocks). Its masked blocks -- at the diagonal, at the window's low end,
 // at the first tokens' end -- may hold infinities or NaN in rows of V that a
 // query does not see, and 0 times those is NaN: a wave whose sums are not all
-// finite at an item's end computes its 32 rows again one by one
-// (prefill_window_row), over visible keys alone, in place of storing them. (A
+// finite at an item's end marks the item, and after the item loop computes its
+// 32 rows again one by one (prefill_window_row), over visible keys alone. (A
 // test of V in those blocks instead took 16 prompts of 128-2048 tokens, window
 // 512, 32/8 heads, from 381 to 402 us.)
 template <typename T, int D, int NW, int QS = 1, typename Args = PrefillArgs>
@@ -189,6 +192,13 @@ __device__ __forceinline__ void prefill_gqa_body(Args a, const int32_t* __restri
   const int my_head = QS == 1 ? wave : wave % HG, my_blk = QS == 1 ? 0 : wave / HG;
   const int nseq = a.nseq, Hkv = a.Hkv;
   const float cs = a.scale_log2;  // > 0 on this path
+  // (window) This wave's rounds whose rows are computed again, a bit each (the
+  // last bit: all rounds from kRedo - 1 on).
+  constexpr int kRedo = 1024;
+  uint32_t* const redo_s = reinterpret_cast<uint32_t*>(smem + gqa_smem_bytes<D, NW>()) + wave * (kRedo / 32);
+  if constexpr (kWindow<Args>) {
+    if (lane < kRedo / 32) redo_s[lane] = 0;
+  }
 
   // ---- Work items: (query block, sequence, kv head) with a non-empty query
   // block, heaviest (latest) query blocks first: level Q holds query block Q
@@ -225,8 +235,7 @@ __device__ __forceinline__ void prefill_gqa_body(Args a, const int32_t* __restri
     int64_t q_start;
     const T* kb;
     const T* vb;
-    WindowBlocks win;  // (window) the blocks; k_start: the sequence's first key
-    int64_t k_start;
+    WindowBlocks win;  // (window) the blocks
   };
   // (window) The item's blocks, in place of the causal range.
   auto set_window = [&](Item& it, int q_last) __attribute__((always_inline)) {
@@ -280,7 +289,6 @@ __device__ __forceinline__ void prefill_gqa_body(Args a, const int32_t* __restri
     it.jm = a.causal ? min(it.k_len / 32, Q * QS + my_blk) : it.k_len / 32;
     it.kfull = min(it.k_len, it.nblk * 32);
     set_window(it, q_last);
-    if constexpr (kWindow<Args>) it.k_start = ks;
     it.kb = static_cast<const T*>(a.k) + ks * a.k_st + it.kvh * a.k_sh;
     it.vb = static_cast<const T*>(a.v) + ks * a.v_st + it.kvh * a.v_sh;
   };
@@ -356,7 +364,6 @@ __device__ __forceinline__ void prefill_gqa_body(Args a, const int32_t* __restri
     it.jm = a.causal ? min(it.k_len / 32, Q * QS + my_blk) : it.k_len / 32;
     it.kfull = min(it.k_len, it.nblk * 32);
     set_window(it, q_last);
-    if constexpr (kWindow<Args>) it.k_start = ks;
     it.kb = static_cast<const T*>(a.k) + ks * a.k_st + it.kvh * a.k_sh;
     it.vb = static_cast<const T*>(a.v) + ks * a.v_st + it.kvh * a.v_sh;
   };
@@ -529,8 +536,7 @@ __device__ __forceinline__ void prefill_gqa_body(Args a, const int32_t* __restri
       if (!window_sees_all(a, qw, kb0, it.k_len)) {
         const uint32_t bits = window_bits(a, qw + c, kb0, it.k_len) >> (4 * h);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!(bits & (1u << (8 * (e >> 2) + (e & 3))))) sc[e] = kNegInfP;
+        for (int e = 0; e < 16; ++e) sc[e] = masked_score(sc[e], bits, 8 * (e >> 2) + (e & 3));
       }
       return;
     }
@@ -804,25 +810,36 @@ __device__ __forceinline__ void prefill_gqa_body(Args a, const int32_t* __restri
     // or NaN in V is NaN. So a bad V row reaches queries of its own 32 alone.)
     if constexpr (kWindow<Args>) {
       if (X.nblk > 0) pv();
-      float sum = 0.f * l;  // NaN where anything is not finite
+      float finite[4] = {0.f * l, 0.f, 0.f, 0.f};  // NaN where a sum is not finite
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sum = fmaf(acc[u][e], 0.f, sum);
-      if (__any(sum != 0.f)) {  // (uniform)
-        const int qw = X.q0 + 32 * my_blk, last = min(X.q_len, qw + 32);
-#pragma unroll 1
-        for (int qq = qw; qq < last; ++qq)
-          prefill_window_row<T>(a, X.q_start + qq, qq, X.kvh * HG + my_head, X.k_start, X.k_len);
-      } else {
-        store_out(X);
-      }
+        for (int e = 0; e < 16; ++e) finite[e & 3] = fmaf(acc[u][e], 0.f, finite[e & 3]);
+      const int r = min(round - 1, kRedo - 1);  // (the next item has been taken)
+      if (__any((finite[0] + finite[1]) + (finite[2] + finite[3]) != 0.f) && lane == 0) redo_s[r >> 5] |= 1u << (r & 31);
+      store_out(X);
     } else {
       if (X.nblk > 0 && !(QS > 1 && a.causal && 32 * j > X.q0 + 32 * my_blk)) pv();
       store_out(X);
     }
     X = Y;
     idx = nidx;
+  }
+  if constexpr (kWindow<Args>) {
+    wait_loads(integral_constant<int, 0>{});  // (and the outputs' stores)
+#pragma unroll 1
+    for (int k = 0; item_of(k) < n_items; ++k) {
+      const int r = min(k, kRedo - 1);
+      if (!((__builtin_amdgcn_readfirstlane(redo_s[r >> 5]) >> (r & 31)) & 1)) continue;
+      Item it;
+      resolve(item_of(k), it);
+      int64_t k_start, k_len;
+      seq_range(cu_k, a.cuk_s, it.b, a.total_k, k_start, k_len);
+      const int qw = it.q0 + 32 * my_blk, last = min(it.q_len, qw + 32);
+#pragma unroll 1
+      for (int qq = qw; qq < last; ++qq)
+        prefill_window_row<T>(a, it.q_start + qq, qq, it.kvh * HG + my_head, k_start, k_len);
+    }
   }
 }
 

@@ -18,7 +18,7 @@ namespace tsa {
 template <typename T, int D, int NW, int QS>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void varlen_window_gqa(
     PrefillWindowArgs a, const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k) {
-  __shared__ __align__(16) char smem[gqa_smem_bytes<D, NW>()];
+  __shared__ __align__(16) char smem[gqa_window_smem_bytes<D, NW>()];
   prefill_gqa_body<T, D, NW, QS>(a, cu_q, cu_k, smem, 0);
 }
 
