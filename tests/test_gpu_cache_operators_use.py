@@ -375,7 +375,7 @@ def test_pools_past_4_gb(hq, hkv, d, page, longest, batch):
     _same(b, a, "8 bits")
 
 
-@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 128), (4, 2, 128), (8, 2, 128), (16, 2, 128), (8, 2, 64), (4, 2, 80)])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 128), (4, 2, 128), (8, 2, 128), (16, 2, 128), (16, 1, 128), (8, 2, 64), (4, 2, 80)])
 def test_prefill_tokens_past_4_gb(hq, hkv, d):
     """Rows 2 MiB apart: the last sequences' lie past 4 GB."""
     lens, step = [1500, 700, 333], 1 << 20

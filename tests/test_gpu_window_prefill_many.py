@@ -28,7 +28,7 @@ def _check(q, k, v, out, starts, lens, at, window, sinks):
     check(out[torch.tensor(rows, device=DEV)], torch.stack(ref), torch.stack(tol), f"window {window}, {sinks}")
 
 
-@pytest.mark.parametrize("hq,hkv", [(32, 8), (16, 8)])
+@pytest.mark.parametrize("hq,hkv", [(32, 8), (16, 8), (64, 4)])
 @pytest.mark.parametrize("window,sinks", [(40, 5), (512, 0)])
 def test_a_long_prompt(hq, hkv, window, sinks):
     n = 140000
@@ -52,7 +52,7 @@ def test_a_long_prompt(hq, hkv, window, sinks):
     _check(q, k, v, out, [0], [n], at, window, sinks)
 
 
-@pytest.mark.parametrize("hq,hkv", [(8, 2), (4, 2), (16, 2)])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (4, 2), (16, 2), (12, 1), (32, 2)])
 def test_many_sequences(hq, hkv):
     g = torch.Generator().manual_seed(hq)
     lens = torch.randint(0, 300, (150,), generator=g).tolist()
@@ -68,3 +68,33 @@ def test_many_sequences(hq, hkv):
     at = [(s, i) for s in first for i in (0, 31, 48, 49, 70, 71, lens[s] - 1)]
     at += [(s, i) for s in range(0, 150, 5) for i in (0, lens[s] // 2, lens[s] - 1) if lens[s] and not (s in first and 50 <= i < 70)]
     _check(q, k, v, out, starts, lens, at, 20, 3)
+
+
+@pytest.mark.parametrize("hq,hkv,dtype", [(12, 1, BF), (16, 1, torch.float16), (32, 2, BF)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 2), (32, 0), (33, 33), (50, 1), (1000, 4), (16, 1000)])
+@pytest.mark.parametrize("lens_q,lens_k", [([70, 5, 160], [70, 5, 160]), ([100, 64, 3], [40, 90, 0])])
+def test_wide_groups(hq, hkv, dtype, window, sinks, lens_q, lens_k):
+    g = torch.Generator().manual_seed(window + hq)
+    q = torch.randn(sum(lens_q), hq, 128, generator=g).to(dtype)
+    k, v = (torch.randn(sum(lens_k), hkv, 128, generator=g).to(dtype) for _ in range(2))
+    cu_q, cu_k = (torch.tensor([0] + x).cumsum(0).to(torch.int32).to(DEV) for x in (lens_q, lens_k))
+    out = flash_attn_varlen_window(q.to(DEV), k.to(DEV), v.to(DEV), cu_q, cu_k, max(lens_q), max(lens_k), window, sinks)
+    ref, tol = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    a = b = 0
+    for nq, nk in zip(lens_q, lens_k):
+        for i in range(nq):
+            see = [b + j for j in range(min(nk, i + 1)) if j > i - window or j < sinks]
+            ref[a + i], tol[a + i] = attend(q[a + i], k[see], v[see], 128**-0.5, half_step(dtype), half_step(dtype))
+        a, b = a + nq, b + nk
+    check(out, ref, tol, f"{hq}/{hkv}, {window}+{sinks}")
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_wide_groups_rows_that_are_not_seen(bad):
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(300, h, 128, generator=g).to(BF) for h in (16, 1, 1))
+    v[50], k[121] = bad, bad
+    cu = torch.tensor([0, 200, 300], dtype=torch.int32, device=DEV)
+    out = flash_attn_varlen_window(q.to(DEV), k.to(DEV), v.to(DEV), cu, cu, 200, 100, 30, 3)
+    sees = [(0, i) for i in range(200) if not (50 <= i < 80 or 121 <= i < 151)]
+    _check(q.to(DEV), k.to(DEV), v.to(DEV), out, [0, 200], [200, 100], sees[::7] + [(0, 49), (0, 80), (0, 120), (0, 151), (1, 99)], 30, 3)

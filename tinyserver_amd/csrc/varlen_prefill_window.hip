@@ -2,11 +2,11 @@
 // visible: query i of a sequence sees the keys j <= i with j > i - window or
 // j < sinks (top-left positions, as tsa_varlen_prefill's causal mask).
 //
-// varlen_window_w64   bf16/f16, head_dim 128, GQA group 4 (12, 16, ...): 64
-//                     queries a wave (prefill_w64_body), and
-// varlen_window_gqa   head_dim 64 or group 2 or 8: the LDS-staged persistent
-//                     kernel (prefill_gqa_body), both over the blocks of the
-//                     window and of the first keys;
+// varlen_window_gqa   bf16/f16, GQA group 2, 4 or 8: the LDS-staged persistent
+//                     kernel (prefill_gqa_body), and
+// varlen_window_w64   head_dim 128, groups of 12, 16, ...: 64 queries a wave
+//                     (prefill_w64_body), both over the blocks of the window and
+//                     of the first keys;
 // varlen_prefill_mfma other groups;
 // varlen_window_generic  float32, other head_dims, strides and scales: one wave
 //                     per (query, q-head), VALU.
@@ -38,14 +38,12 @@ static int launch_window_gqa(const PrefillWindowArgs& a, hipStream_t stream) {
 
 template <typename T>
 static int launch_window_mfma(PrefillWindowArgs& a, int64_t max_seqlen_q, hipStream_t stream) {
-  // Groups of eight keep the eight waves of the LDS-staged kernel, which stage
-  // each K/V block once for all of them: 16 prompts of 128-2048 tokens, 64/8
-  // heads, window 128 / 512: 293 / 460 us against 309 / 477 with 64 queries a
-  // wave (four of 100-700: 34 / 35 against 35 / 39; one of 16384: 275 / 443
-  // against 242 / 422, window 4096 + 16: 1892 against 1874). Groups of four take
-  // 64 queries a wave: 228 / 364 -> 164 / 262.
-  if (prefill_takes_w64(a) && a.G != 8)
-    return prefill_w64_window_launch(a, std::is_same<T, bf16_t>::value, stream);
+  // Groups of 2, 4 and 8: the LDS-staged kernel. Beside it, 64 queries a wave, 16
+  // prompts of 128-2048 tokens, window 32 / 512 + 4: 32/8 heads 109 / 257 us
+  // against 135 / 273, 64/8 heads 217 / 455 against 253 / 485; four prompts of
+  // 100-700, 32/8 heads: 17 / 25 against 17 / 32; one of 16384, 32/8 heads, window
+  // 512 / 4096: 231 / 1029 against 229 / 1026. Other multiples of four (12, 16)
+  // take 64 queries a wave.
   if (prefill_takes_gqa(a)) {
     if (a.D == 128) {
       if (prefill_pairs(a)) return launch_window_gqa<T, 128, 4, 2>(a, stream);
@@ -55,6 +53,7 @@ static int launch_window_mfma(PrefillWindowArgs& a, int64_t max_seqlen_q, hipStr
     if (a.G == 2) return launch_window_gqa<T, 64, 2>(a, stream);
     return a.G == 4 ? launch_window_gqa<T, 64, 4>(a, stream) : launch_window_gqa<T, 64, 8>(a, stream);
   }
+  if (prefill_takes_w64(a)) return prefill_w64_window_launch(a, std::is_same<T, bf16_t>::value, stream);
   a.nqb = static_cast<int32_t>((max_seqlen_q + 31) / 32);
   if (a.nqb == 0) return TSA_OK;
   const dim3 grid(a.nqb, a.nseq, (a.Hq + 3) / 4);
