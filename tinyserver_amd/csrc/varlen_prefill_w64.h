@@ -41,14 +41,14 @@
 // With PrefillWindowArgs (a sliding window and first tokens) an item's blocks are
 // those that its 64 queries see (window_blocks). The next item's Q is loaded
 // during this one's blocks (peek_q): windowed items are alike, so without it the
-// workgroups all load Q at once between items (16 prompts of 2048 tokens, 32/8
-// heads, window 32 / 512: 252 / 441 us without, 226 / 425 with). An item whose
-// outputs are not all finite is marked, and its rows are computed again over
-// visible keys alone after the item loop (inlined at the item's end that cost 50
-// spilled registers: 16 prompts of 128-2048 tokens, window 512 + 4, 294 us against
-// 261). At window 512 an item of 19 blocks takes 58k cycles: 43k the blocks (five
-// masked half-iterations 1.2k more than the others), 3k the first scores, 6k the
-// output.
+// workgroups all load Q at once between items. An item whose outputs are not all
+// finite is marked, and its rows are computed again over visible keys alone after
+// the item loop (inlined at the item's end that cost 50 spilled registers). Both
+// measured with groups of four: 16 prompts of 2048 tokens, window 32 / 512, 252 /
+// 441 us without the first and 226 / 425 with it; 16 of 128-2048, window 512 + 4,
+// 294 us without the second and 261 with it. At window 512 an item of 19 blocks
+// takes 58k cycles: 43k the blocks (five masked half-iterations 1.2k more than the
+// others), 3k the first scores, 6k the output.
 #pragma once
 
 #include <type_traits>

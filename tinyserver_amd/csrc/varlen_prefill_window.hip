@@ -42,8 +42,9 @@ static int launch_window_mfma(PrefillWindowArgs& a, int64_t max_seqlen_q, hipStr
   // prompts of 128-2048 tokens, window 32 / 512 + 4: 32/8 heads 109 / 257 us
   // against 135 / 273, 64/8 heads 217 / 455 against 253 / 485; four prompts of
   // 100-700, 32/8 heads: 17 / 25 against 17 / 32; one of 16384, 32/8 heads, window
-  // 512 / 4096: 231 / 1029 against 229 / 1026. Other multiples of four (12, 16)
-  // take 64 queries a wave.
+  // 512 / 4096: 231 / 1029 against 229 / 1026. Other multiples of four take 64
+  // queries a wave (four of 500-2048, 128/8 heads: 139 / 264 against 236 / 1008 in
+  // varlen_prefill_mfma).
   if (prefill_takes_gqa(a)) {
     if (a.D == 128) {
       if (prefill_pairs(a)) return launch_window_gqa<T, 128, 4, 2>(a, stream);
