@@ -143,6 +143,33 @@ def test_a_node_that_sees_one_past_max_nodes(hq, d, dtype):
         assert bool((out[at + 3 : at + nodes[s]] == 3).all())
 
 
+@pytest.mark.parametrize("batch", [40, 128, 129])
+@pytest.mark.parametrize("most", [3, 9, 33])
+def test_many_ragged_trees(batch, most):
+    """More workgroups than CUs, lengths and node counts of all kinds (none among them)."""
+    hq, hkv, d, page = 16, 4, 64, 16
+    g = torch.Generator().manual_seed(batch + most)
+    ctx = torch.where(torch.rand(batch, generator=g) < 0.2, 0, torch.randint(1, 900, (batch,), generator=g)).tolist()
+    nodes = torch.randint(0, most + 1, (batch,), generator=g).tolist()
+    nodes[3], ctx[5], ctx[6] = most, 899, 899
+    kc, vc, bt = pool([a + b for a, b in zip(ctx, nodes)], hkv, d, page, 4)
+    kc, vc = kc.to(BF), vc.to(BF)
+    n = sum(nodes)
+    q = torch.randn(n, hq, d, generator=g).to(BF)
+    mask = torch.randint(0, 1 << most, (n,), generator=g)
+    cu = torch.tensor([0] + nodes).cumsum(0).tolist()
+    out = paged_attention_tree(q.to(DEV), kc.to(DEV), vc.to(DEV), bt.to(DEV), page, _i32(ctx), _i32(cu), mask.to(DEV))
+    ref, tol, at = [], [], []
+    for s in range(batch):
+        for i in {0, nodes[s] - 1} if nodes[s] else ():
+            see = list(range(ctx[s])) + [ctx[s] + j for j in range(nodes[s]) if int(mask[cu[s] + i]) >> j & 1]
+            r, t = attend(q[cu[s] + i], rows(kc, bt[s], see), rows(vc, bt[s], see), d**-0.5, half_step(BF), half_step(BF))
+            ref.append(r)
+            tol.append(t)
+            at.append(cu[s] + i)
+    check(out[torch.tensor(at, device=DEV)], torch.stack(ref), torch.stack(tol), f"{batch} trees of up to {most}")
+
+
 def _step(cache, hq, batch, longest, page=16, d=128, hkv=8):
     """A decode step over an 8-bit cache, a windowed one and a draft's, on inputs that a caller overwrites."""
     g = torch.Generator(device=DEV).manual_seed(batch + longest)

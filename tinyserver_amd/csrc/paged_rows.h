@@ -34,7 +34,8 @@ struct RowsArgs {
   int32_t S;          // splits of a unit's tokens (0: the stream)
   int32_t NW;         // waves of the stream
   int32_t out8;       // output rows are unit-stride, in 8-byte pieces
-  int32_t RT, RB, per_split;  // trees: 32-row tiles of a workgroup, row blocks of a unit, 32-key blocks of a split
+  int32_t RT, RB, per_split;  // trees: 32-row tiles of a workgroup, row blocks of a unit, most 32-key blocks of a split
+  int32_t order;              // trees: workgroups take the sequences by length (TreeOrder)
   // The matrix-core forms: page strides in bytes, and the tiles (16 tokens) of a
   // page as a multiplier and a shift (tiles_of_page).
   uint32_t k_page, v_page, ks_page, vs_page, page_mul, page_shift;
@@ -87,6 +88,13 @@ __device__ __forceinline__ SeqRange seq_of(const RowsArgs& a, int s) {
   r.ctx = static_cast<int>(len);
   r.lo = a.window > 0 && r.ctx > a.window ? r.ctx - a.window : 0;
   return r;
+}
+
+constexpr int kTreeOrderSeqs = 128;  // sequences of a call whose workgroups take them by length
+// 32-key blocks of a tree's splits: the unit's own, evenly, in fours (a wave each).
+__device__ __forceinline__ int tree_per_split(const RowsArgs& a, int nblk) {
+  const int even = ((nblk + a.S - 1) / a.S + 3) & ~3;
+  return min(a.per_split, max(even, 16));
 }
 
 // Host side: the checks of the entry points. k_scale and v_scale are NULL for

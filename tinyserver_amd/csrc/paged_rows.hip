@@ -308,6 +308,7 @@ extern "C" int tsa_paged_tree(const tsa_view* out, const tsa_view* query, const 
                   "workspace of %zu bytes is too small: %zu needed", workspace_bytes, p.bytes);
       TSA_REQUIRE(p.bytes == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
       a.S = p.S; a.RT = p.RT; a.RB = p.RB; a.per_split = p.per_split;
+      a.order = a.B > 1 && a.B <= kTreeOrderSeqs && int64_t{a.B} * a.Hkv * a.S * a.RB > 256;  // (more than one workgroup a CU: else a lookup for nothing)
       a.part = static_cast<float*>(workspace);
       return rows_tree_launch(a, query->dtype, static_cast<hipStream_t>(stream));
     }

@@ -4,7 +4,7 @@
 // (paged_rows_tree_lds.h the others).
 //
 // What bounds it: HBM (each K/V byte once; 64 sequences of 512-4096 tokens, 4
-// nodes, 32/8 heads: 129 us, 4.7 TB/s). A workgroup of four waves takes a unit's
+// nodes, 32/8 heads: 114 us, 5.3 TB/s). A workgroup of four waves takes a unit's
 // rows, wave kg every fourth 32-key block. A unit's keys are split over
 // workgroups, whose partials a second launch merges.
 //
@@ -53,6 +53,47 @@ __device__ __forceinline__ float flag_value(float n) {
   return nan || (pos && neg) ? __builtin_nanf("") : pos ? INFINITY : neg ? -INFINITY : 0.f;
 }
 
+// Which unit (sequence s, kv head), split and row block a workgroup takes; false:
+// none. Ids go round the XCDs, so those of one XCD and the row blocks of a unit
+// and split follow each other. With a.order the sequences go by falling length,
+// and every other run of 32 workgroups of an XCD (its CUs) backwards: a CU that
+// gets two has a long and a short one. (In the sequences' own order, 8 sequences
+// of 2000-8192 tokens, 40-64 nodes, 64/8 heads: 133 us against 122; 64 of
+// 512-4096, 4-16 nodes, 32/8 heads: 137 against 123.) keys: LDS, 128
+// words; all threads call.
+struct TreeWork {
+  int s, kvh, sp, rb, u;
+};
+__device__ __forceinline__ bool tree_work(const RowsArgs& a, int32_t* keys, TreeWork& w) {
+  const int U = a.B * a.Hkv, total = (U * a.S + 7) / 8 * a.RB;  // workgroups of an XCD
+  int k = static_cast<int>(blockIdx.x) >> 3;
+  if (a.order) {
+    const int lo = k & ~31;
+    if (lo & 32) k = lo + min(lo + 32, total) - 1 - k;
+  }
+  w.rb = k % a.RB;
+  const int us = k / a.RB * 8 + (static_cast<int>(blockIdx.x) & 7);
+  if (us >= U * a.S) return false;
+  w.sp = us / U;
+  const int u = us - w.sp * U;
+  w.s = u / a.Hkv;
+  w.kvh = u - w.s * a.Hkv;
+  if (a.order) {
+    const int t = threadIdx.x;
+    if (t < kTreeOrderSeqs) keys[t] = t < a.B ? max(a.lens[t * a.len_s], 0) : -1;
+    __syncthreads();
+    int rank = 0, mine = t < a.B ? keys[t] : -1;
+    for (int j = 0; j < a.B; ++j) rank += keys[j] > mine || (keys[j] == mine && j < t);
+    __syncthreads();
+    if (t < a.B && rank == w.s) keys[0] = t;
+    __syncthreads();
+    w.s = __builtin_amdgcn_readfirstlane(keys[0]);
+    __syncthreads();
+  }
+  w.u = w.s * a.Hkv + w.kvh;
+  return true;
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void paged_rows_tree(
     RowsArgs a, const int32_t* __restrict__ bt, const uint32_t* __restrict__ mask, float* __restrict__ part) {
@@ -60,13 +101,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void p
   typedef typename VPiece<2 * NU>::type VP;
   __shared__ __align__(16) float slots[4 * 32 * PF];
   // ---- Which unit and split.
-  const int us = blockIdx.x, U = a.B * a.Hkv;
-  if (us >= U * a.S) return;
-  const int sp = us / U, u = us - sp * U, s = u / a.Hkv, kvh = u - s * a.Hkv;
+  TreeWork w;
+  if (!tree_work(a, reinterpret_cast<int32_t*>(slots), w)) return;
+  const int sp = w.sp, u = w.u, s = w.s, kvh = w.kvh;
   const SeqRange r = seq_of(a, s);
   const int rows = r.nodes * a.G;  // up to 32
   if (rows <= 0) return;
-  const int nblk = (r.end + 31) >> 5, b0 = sp * a.per_split, b1 = min(nblk, b0 + a.per_split);
+  const int nblk = (r.end + 31) >> 5, per = tree_per_split(a, nblk), b0 = sp * per, b1 = min(nblk, b0 + per);
   if (b0 >= b1 && a.S > 1) return;  // (the merge takes the splits that have blocks)
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
   constexpr int KG = 4;

@@ -5,8 +5,8 @@
 namespace tsa {
 
 // Workgroups a call's units are split into, at least, where there are tokens for
-// it (64 sequences of 512-4096 tokens, 16 nodes, 32/8 heads: 512 138 us, 768 161;
-// 32 nodes: 156, 183; 8 of 8192 with 64 nodes, 64/8 heads: 169, 181; 256 are as 512), and
+// it (64 sequences of 512-4096 tokens, 16 nodes, 32/8 heads: 512 127 us, 1024 160;
+// 32 nodes: 146, 191; 8 of 8192 with 64 nodes, 64/8 heads: 181, 196), and
 // the least blocks of a split (one sequence of 300 tokens: 16 14.9 us, 4 18.1).
 constexpr int64_t kTreeWorkgroups = 512, kTreeMinSplit = 16;
 
@@ -41,7 +41,7 @@ static int launch_tree(const RowsArgs& a, hipStream_t stream) {
   else paged_rows_tree_lds<T, D, 4><<<grid, dim3(256), 0, stream>>>(a, a.bt, a.mask, a.part);
   if (int rc = check_launch("tsa_paged_tree")) return rc;
   if (a.S == 1) return TSA_OK;
-  launch_rows_merge<T, D>(a, a.T * a.G, a.per_split, stream);
+  launch_rows_merge<T, D>(a, a.T * a.G, 0, stream);
   return check_launch("tsa_paged_tree");
 }
 

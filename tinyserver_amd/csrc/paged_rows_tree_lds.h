@@ -23,7 +23,8 @@ namespace tsa {
 constexpr int kTreeMaxSplit = 256;  // 32-key blocks of a split: its page table in LDS
 // K/V slots: two workgroups fit a CU, which is what the plan's 512 give it, with
 // three blocks each in flight (64 sequences of 512-4096 tokens, 16 nodes, 32/8
-// heads: four 138 us, two, with four workgroups to a CU, 155).
+// heads, in the sequences' own order: four 138 us, two, with four workgroups to a
+// CU, 155).
 constexpr int kTreeSlots = 4;
 template <int D> constexpr int tree_lds_bytes() { return 2 * kTreeSlots * 32 * 2 * D + kTreeMaxSplit * 8 + 16; }
 
@@ -42,14 +43,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(NW == 2
   int32_t* const first_bad = tab + 2 * kTreeMaxSplit;            // the first block with such a half
 
   // ---- Which unit, split and row block.
-  const int id = blockIdx.x, k8 = id >> 3;
-  const int rb = k8 % a.RB, us = (k8 / a.RB) * 8 + (id & 7), U = a.B * a.Hkv;
-  if (us >= U * a.S) return;
-  const int sp = us / U, u = us - sp * U, s = u / a.Hkv, kvh = u - s * a.Hkv;
+  TreeWork w;
+  if (!tree_work(a, tab, w)) return;
+  const int rb = w.rb, sp = w.sp, u = w.u, s = w.s, kvh = w.kvh;
   const SeqRange r = seq_of(a, s);
   const int all = r.nodes * a.G, row_first = rb * 32 * NW;
   if (row_first >= all) return;
-  const int nblk = (r.end + 31) >> 5, b0 = sp * a.per_split, n = min(nblk, b0 + a.per_split) - b0;  // blocks
+  const int nblk = (r.end + 31) >> 5, per = tree_per_split(a, nblk), b0 = sp * per, n = min(nblk, b0 + per) - b0;  // blocks
   if (n <= 0 && a.S > 1) return;  // (the merge takes the splits that have blocks)
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);

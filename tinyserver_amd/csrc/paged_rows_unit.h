@@ -336,7 +336,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 // the same rows, a quarter of the splits each, then the quarters in order; else
 // each wave takes rows of its own and all their splits. Splits go in batches
 // whose loads are issued together (past the last: repeated and dropped). Grid:
-// units x row groups.
+// units x row groups. tiles_per_split: decode's (trees: tree_per_split).
 template <typename T, int D, bool SHARE>
 __global__ __launch_bounds__(256) void paged_rows_merge(RowsArgs a, const int32_t* __restrict__ lens,
                                                         const float* __restrict__ part, int tiles_per_split) {
@@ -349,7 +349,8 @@ __global__ __launch_bounds__(256) void paged_rows_merge(RowsArgs a, const int32_
   int nrows;
   if (a.cu) {
     const SeqRange r = seq_of(a, s);
-    n = (((r.end + 31) >> 5) + tiles_per_split - 1) / tiles_per_split;
+    const int nblk = (r.end + 31) >> 5, per = tree_per_split(a, nblk);
+    n = (nblk + per - 1) / per;
     row0 = r.row0;
     nrows = r.nodes * a.G;
   } else {
