@@ -68,6 +68,12 @@ template <typename C, typename T, bool HI> __device__ __forceinline__ uint32_t w
       return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
     else
       return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
+  } else if constexpr (std::is_same<T, f16_t>::value) {
+    // 1024 + (code + 128) is the f16 whose low byte is code + 128; less 1152, exactly the code. (Five instructions
+    // for four codes; nine by conversions.)
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 x = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, HI ? 0x04030402u : 0x04010400u));
+    return __builtin_bit_cast(uint32_t, x - h2{1152, 1152});
   } else {
     constexpr int b = HI ? 16 : 0;
     return pack2<T>(static_cast<float>(static_cast<int8_t>(w >> b)), static_cast<float>(static_cast<int8_t>(w >> (b + 8))));
