@@ -73,7 +73,9 @@ __global__ __launch_bounds__(256) void quant8_rows(Quant8Args a, PagedAddr addr)
 // residual: with the correctly rounded reciprocal that is the correctly rounded
 // x / scale (Markstein's theorem: one step from a quotient within a unit in the
 // last place; the first step gives that one). Residuals below the normal range
-// would lose bits, so rows of scales under 2^-80 divide.
+// would lose bits, so rows of scales under 2^-80 divide. The residual is y scale
+// - x, subtracted: that of -0 is +0, and -0 - 0 stays -0 (x - y scale, added,
+// would make it +0, another code of e4m3).
 constexpr int kQuant8Batch = 2;
 constexpr int kQuant8LdsSeqs = 2048;
 
@@ -105,8 +107,8 @@ template <typename C> __device__ __forceinline__ void quotients8(const float (&x
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float y = x[i] * r;
-      y = fmaf(fmaf(-y, scale, x[i]), r, y);
-      y = fmaf(fmaf(-y, scale, x[i]), r, y);
+      y = fmaf(-fmaf(y, scale, -x[i]), r, y);
+      y = fmaf(-fmaf(y, scale, -x[i]), r, y);
       q[i] = fminf(fmaxf(y, -kLargest8<C>), kLargest8<C>);
     }
   } else {
