@@ -1,5 +1,8 @@
-"""The 8-bit store and load at signed zeros: codes and scales bit-equal to the
-definition, values read back bit-equal to code * scale rounded once."""
+"""The 8-bit store and load in the forms that long and wide batches take, and at
+signed zeros: codes and scales bit-equal to the definition, values read back
+bit-equal to code * scale rounded once. Calls of 2048 tokens or more give a
+workgroup two kv heads (an odd one is left over), calls of more than 2048
+sequences search them elsewhere."""
 
 import pytest
 import torch
@@ -52,3 +55,30 @@ def test_signed_zeros(cache, dtype, d):
     _store_and_load(bt, codes, scales, [x.to(DEV), x.flip(0).to(DEV)], [8], 16)
     if cache == E4:
         assert int((codes[0].view(torch.uint8) == 0x80).sum()) > 0
+
+
+@pytest.mark.parametrize("cache", [E4, I8])
+@pytest.mark.parametrize("dtype,hkv,d,lens", [
+    (BF, 8, 128, [2000, 60]),
+    (F16, 3, 128, [700, 1, 0, 1400]),  # an odd head is left over
+    (BF, 1, 64, [2300]),
+    (F16, 5, 64, [1024, 1024]),        # the first call of two heads a workgroup
+    (BF, 5, 64, [1024, 1023]),         # the last of one
+])
+def test_two_heads_a_workgroup(cache, dtype, hkv, d, lens):
+    bt, codes, scales, g = _state(lens, hkv, d, 16, cache, hkv + d)
+    n = sum(lens)
+    src = [(torch.randn(n, hkv, d, generator=g) * torch.exp(2 * torch.randn(n, hkv, 1, generator=g))).to(dtype).to(DEV)
+           for _ in range(2)]
+    _store_and_load(bt, codes, scales, src, lens, 16)
+
+
+@pytest.mark.parametrize("cache", [E4, I8])
+@pytest.mark.parametrize("seqs", [2048, 2049])
+def test_many_sequences(cache, seqs):
+    """Sequences of 0 to 2 tokens, either side of the most whose starts are kept in LDS."""
+    g = torch.Generator().manual_seed(seqs)
+    lens = torch.randint(0, 3, (seqs,), generator=g).tolist()
+    bt, codes, scales, g = _state(lens, 2, 128, 16, cache, 4)
+    src = [torch.randn(sum(lens), 2, 128, generator=g).to(BF).to(DEV) for _ in range(2)]
+    _store_and_load(bt, codes, scales, src, lens, 16)
