@@ -114,7 +114,9 @@ __global__ __launch_bounds__(256) void varlen_prefill_mfma(Args a) {
       for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          p[ks][r] = fin ? fast_exp2(sv[ks][r] - m[qs]) : 0.f;
+          // (window: a row that has seen no key but NaN scores has no maximum, and its weights are NaN)
+          if constexpr (kWindow<Args>) p[ks][r] = fast_exp2(sv[ks][r] - (fin ? m[qs] : 0.f));
+          else p[ks][r] = fin ? fast_exp2(sv[ks][r] - m[qs]) : 0.f;
           l[qs] += p[ks][r];
         }
       const u32x4 pop = u32x4{pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]), pack2<T>(p[1][0], p[1][1]),
