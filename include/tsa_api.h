@@ -346,7 +346,9 @@ int tsa_paged_tree(const tsa_view* out, const tsa_view* query, const tsa_view* k
 /* tsa_varlen_prefill, causal, over part of the keys: query i of a sequence
  * sees the keys j <= i with j > i - window (window >= 1) or j < sinks. Keys
  * that are not seen have no influence, whatever their rows hold; a query that
- * sees none (its window past the last key, no first keys) gives 0. */
+ * sees none (its window past the last key, no first keys) gives 0. A seen value
+ * of V that is not finite makes the output of its dim not finite (an infinity may
+ * come out as NaN). */
 int tsa_varlen_prefill_window(const tsa_view* out, const tsa_view* q, const tsa_view* k,
                               const tsa_view* v, const tsa_view* cu_seqlens_q,
                               const tsa_view* cu_seqlens_k, int64_t max_seqlen_q, int64_t max_seqlen_k,

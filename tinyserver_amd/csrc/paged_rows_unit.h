@@ -27,6 +27,7 @@
 
 #include <type_traits>
 
+#include "nonfinite.h"
 #include "paged_decode.h"
 #include "paged_rows.h"
 
@@ -85,14 +86,6 @@ template <typename C, typename T> __device__ __forceinline__ u32x4 widen8(uint32
   return u32x4{widen2<C, T, false>(w0), widen2<C, T, true>(w0), widen2<C, T, false>(w1), widen2<C, T, true>(w1)};
 }
 
-// A lane's piece of a V row: N bytes (4, 8 or 16).
-template <int N> struct VPiece;
-template <> struct VPiece<4> { typedef uint32_t type; };
-template <> struct VPiece<8> { typedef u32x2 type; };
-template <> struct VPiece<16> { typedef u32x4 type; };
-__device__ __forceinline__ uint32_t word_of(uint32_t v, int) { return v; }
-__device__ __forceinline__ uint32_t word_of(const u32x2& v, int i) { return v[i]; }
-__device__ __forceinline__ uint32_t word_of(const u32x4& v, int i) { return v[i]; }
 template <bool NT, typename P, typename S> __device__ __forceinline__ P load_piece(const S* p) {
   if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const P*>(p));
   else return *reinterpret_cast<const P*>(p);

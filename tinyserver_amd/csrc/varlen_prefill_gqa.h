@@ -92,10 +92,12 @@ __device__ __forceinline__ void seq_range(const int32_t* cu, int64_t stride, int
   len = s1 - s0;
 }
 
-// varlen_prefill_window.h: one row, over the keys it sees.
-template <typename T>
-__device__ void prefill_window_row(const PrefillWindowArgs& a, int64_t qi, int64_t qq, int h, int64_t k_start,
-                                   int64_t k_len);
+// varlen_prefill_window.h: queries [q0, q0 + 32) of a sequence, q-head `head`,
+// whose sums over the blocks `win` were not all finite: computed again if a V that
+// some of them do not see may be why (or always).
+template <typename T, int D>
+__device__ void prefill_window_again(const PrefillWindowArgs& a, const WindowBlocks& win, int64_t q_start, int q0,
+                                     int q_len, int head, int64_t k_start, int k_len, bool always);
 
 // The work-item plan: up to kPlanItems item descriptors of a workgroup (6
 // int32 each), computed kPlanItems at a time, and the level table (items
@@ -152,11 +154,13 @@ constexpr int gqa_window_smem_bytes() { return gqa_smem_bytes<D, NW>() + NW * 12
 // (window_blocks). Its masked blocks -- at the diagonal, at the window's low end,
 // at the first tokens' end -- may hold infinities or NaN in rows of V that a
 // query does not see, and 0 times those is NaN: a wave whose sums are not all
-// finite at an item's end marks the item, and after the item loop computes its
-// 32 rows again one by one (prefill_window_row), over visible keys alone. (A
-// test of V in those blocks instead took 16 prompts of 128-2048 tokens, window
-// 512, 32/8 heads, from 381 to 402 us; the second pass inlined at the item's end,
-// 16/8 heads, 198 us against 119: 61 spilled registers against 24.)
+// finite at an item's end marks the item. After the item loop it looks at the V
+// rows of the item's masked blocks, and computes its 32 rows again if one that
+// some query does not see is not finite (prefill_window_again; values that every
+// query sees, a NaN in a first token say, are right as they are). (A test of V in
+// those blocks in the loop instead took 16 prompts of 128-2048 tokens, window 512,
+// 32/8 heads, from 381 to 402 us; the second pass inlined at the item's end, 16/8
+// heads, 198 us against 119: 61 spilled registers against 24.)
 template <typename T, int D, int NW, int QS = 1, typename Args = PrefillArgs>
 __device__ __forceinline__ void prefill_gqa_body(Args a, const int32_t* __restrict__ cu_q,
                                                  const int32_t* __restrict__ cu_k, char* smem, int wg_base) {
@@ -836,10 +840,8 @@ __device__ __forceinline__ void prefill_gqa_body(Args a, const int32_t* __restri
       resolve(item_of(k), it);
       int64_t k_start, k_len;
       seq_range(cu_k, a.cuk_s, it.b, a.total_k, k_start, k_len);
-      const int qw = it.q0 + 32 * my_blk, last = min(it.q_len, qw + 32);
-#pragma unroll 1
-      for (int qq = qw; qq < last; ++qq)
-        prefill_window_row<T>(a, it.q_start + qq, qq, it.kvh * HG + my_head, k_start, k_len);
+      prefill_window_again<T, D>(a, it.win, it.q_start, it.q0 + 32 * my_blk, it.q_len, it.kvh * HG + my_head, k_start,
+                                 it.k_len, false);
     }
   }
 }

@@ -4,7 +4,7 @@
 // window with first tokens.
 #pragma once
 
-#include "varlen_prefill_gqa.h"
+#include "varlen_prefill_window.h"
 
 namespace tsa {
 
@@ -142,8 +142,8 @@ __global__ __launch_bounds__(256) void varlen_prefill_mfma(Args a) {
   }
 
   if constexpr (kWindow<Args>) {
-    // Sums that are not finite: a key that a query does not see may have held
-    // an infinity or NaN. Then the rows one by one, over the keys each sees.
+    // Sums that are not finite: a V row that a query does not see may have held an
+    // infinity or NaN. Then the rows again, each over the keys it sees.
     float sum = 0.f;
 #pragma unroll
     for (int qs = 0; qs < 2; ++qs)
@@ -151,10 +151,10 @@ __global__ __launch_bounds__(256) void varlen_prefill_mfma(Args a) {
       for (int u = 0; u < 8; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) sum = fmaf(acc[qs][u][r], 0.f, sum);
-    if (__any(sum != 0.f)) {
-#pragma unroll 1
-      for (int64_t qq = row0; qq < q_len && qq < row0 + 32; ++qq)
-        prefill_window_row<T>(a, q_start + qq, qq, h, k_start, k_len);
+    if (__any(sum != 0.f) &&
+        window_leaks<T, D>(a, win, static_cast<int>(row0), static_cast<int>(q_len), kvh, k_start, static_cast<int>(k_len))) {
+      prefill_window_tile<T, D>(a, q_start, static_cast<int>(row0), static_cast<int>(q_len), h, k_start,
+                                static_cast<int>(k_len));
       return;
     }
   }

@@ -42,8 +42,8 @@
 // those that its 64 queries see (window_blocks). The next item's Q is loaded
 // during this one's blocks (peek_q): windowed items are alike, so without it the
 // workgroups all load Q at once between items. An item whose outputs are not all
-// finite is marked, and its rows are computed again over visible keys alone after
-// the item loop (inlined at the item's end that cost 50 spilled registers). Both
+// finite is marked, and looked at again after the item loop (prefill_window_again;
+// inlined at the item's end that cost 50 spilled registers). Both
 // measured with groups of four: 16 prompts of 2048 tokens, window 32 / 512, 252 /
 // 441 us without the first and 226 / 425 with it; 16 of 128-2048, window 512 + 4,
 // 294 us without the second and 261 with it. At window 512 an item of 19 blocks
@@ -66,7 +66,7 @@ constexpr int w64_smem_bytes() {
   return 2 * kW64Slots * 8192 + 4 * kW64QArea + 4 * kW64OutStage + kW64MaxSeqs * 2 + kPlanItems * 6 * 4 +
          kPlanLevels * 4;
 }
-constexpr int w64_window_smem_bytes() { return w64_smem_bytes() + 512; }
+constexpr int w64_window_smem_bytes() { return w64_smem_bytes() + 1024; }
 
 // Register homes. The output accumulators (2 x 64 fp32 per lane) live in
 // AGPRs, where the P.V MFMAs (builtins) accumulate them; Q lives in AGPRs
@@ -157,10 +157,13 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
   uint16_t* const nqt_s = reinterpret_cast<uint16_t*>(smem + COFF);
   int32_t* const plan_s = reinterpret_cast<int32_t*>(smem + PLOFF);
   int32_t* const lev_s = reinterpret_cast<int32_t*>(smem + LVOFF);
-  // (window) this wave's rounds whose rows are computed again, a bit each (the
-  // last bit: all rounds from kRedo - 1 on).
+  // (window) this wave's rounds that are looked at again, a bit each (the last
+  // bit: all rounds from kRedo - 1 on): whose outputs are not all finite, then
+  // those with such a denominator. A row's denominator is a product with the P
+  // operand of its partner 16 rows away too, by 0: a NaN score of either reaches
+  // both, and the item is computed again whatever V holds.
   constexpr int kRedo = 1024;
-  static_assert(w64_window_smem_bytes() == w64_smem_bytes() + 4 * kRedo / 8, "LDS layout and its size agree");
+  static_assert(w64_window_smem_bytes() == w64_smem_bytes() + 2 * 4 * kRedo / 8, "LDS layout and its size agree");
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -168,9 +171,10 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
   const int HG = a.G / 4;      // q-head groups per kv head
   const int HH = a.Hkv * HG;   // items per (sequence, query tile)
   const float cs = a.scale_log2;  // > 0 on this path
-  uint32_t* const redo_s = reinterpret_cast<uint32_t*>(smem + w64_smem_bytes()) + wave * (kRedo / 32);
+  uint32_t* const redo_s = reinterpret_cast<uint32_t*>(smem + w64_smem_bytes()) + wave * (2 * kRedo / 32);
   if constexpr (kWindow<Args>) {
-    if (lane < kRedo / 32) redo_s[lane] = 0;
+    static_assert(2 * kRedo / 32 == 64, "a word a lane");
+    redo_s[lane] = 0;
   }
 
   // ---- Work items (64-query tile, sequence, kv head, head group), heaviest
@@ -711,7 +715,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     char* pend_p[4];
     bool pend_ok[4];
     bool pend_full = true, have = false;
-    float finite[4] = {0.f, 0.f, 0.f, 0.f};  // (window) NaN where a sum is not finite
+    float finite[4] = {0.f, 0.f, 0.f, 0.f}, finite_l = 0.f;  // (window) NaN where a sum is not finite
     auto flush = [&]() __attribute__((always_inline)) {
       if (pend_full) {
 #pragma unroll
@@ -727,7 +731,7 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
       const float l0 = __shfl(lacc[t][0], c & 15, 64), l1 = __shfl(lacc[t][1], c & 15, 64);
       const float den = c < 16 ? l0 : l1;
       const float rl = kWindow<Args> && den == 0.f ? 0.f : 1.f / den;  // 1 / query c's denominator (window: nothing seen, 0)
-      if constexpr (kWindow<Args>) finite[t] = fmaf(den, 0.f, finite[t]);
+      if constexpr (kWindow<Args>) finite_l = fmaf(den, 0.f, finite_l);
       const int rbase = it.q0 + 32 * t;
       const bool full = rbase + 32 <= it.q_len;
       char* rowp[4];
@@ -773,7 +777,13 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
     flush();
     if constexpr (kWindow<Args>) {
       const int r = min(k, kRedo - 1);
-      if (__any((finite[0] + finite[1]) + (finite[2] + finite[3]) != 0.f) && lane == 0) redo_s[r >> 5] |= 1u << (r & 31);
+      if (__any((finite[0] + finite[1]) + (finite[2] + finite[3]) + finite_l != 0.f)) {
+        const bool bad_l = __any(finite_l != 0.f);
+        if (lane == 0) {
+          redo_s[r >> 5] |= 1u << (r & 31);
+          if (bad_l) redo_s[kRedo / 32 + (r >> 5)] |= 1u << (r & 31);
+        }
+      }
     }
   };
 
@@ -874,11 +884,14 @@ __device__ __forceinline__ void prefill_w64_body(Args a, const int32_t* __restri
   if constexpr (kWindow<Args>) {  // (that wait was for the outputs' stores too)
 #pragma unroll 1
     for (int k = 0; item_of(k) < n_items; ++k) {
-      if (!((__builtin_amdgcn_readfirstlane(redo_s[min(k, kRedo - 1) >> 5]) >> (min(k, kRedo - 1) & 31)) & 1)) continue;
+      const int r = min(k, kRedo - 1);
+      if (!((__builtin_amdgcn_readfirstlane(redo_s[r >> 5]) >> (r & 31)) & 1)) continue;
+      const bool bad_l = (__builtin_amdgcn_readfirstlane(redo_s[kRedo / 32 + (r >> 5)]) >> (r & 31)) & 1;
       locate(item_of(k), [&](int, int hh, int Q, int64_t qs, int64_t ql, int64_t ks, int64_t kl) {
-        const int head = hh / HG * a.G + hh % HG * 4 + wave, last = min(static_cast<int>(ql), 64 * Q + 64);
+        const int head = hh / HG * a.G + hh % HG * 4 + wave, n_q = static_cast<int>(ql), n_k = static_cast<int>(kl);
+        const WindowBlocks win = window_blocks(a, 64 * Q, min(n_q, 64 * Q + 64), n_k);
 #pragma unroll 1
-        for (int qq = 64 * Q; qq < last; ++qq) prefill_window_row<T>(a, qs + qq, qq, head, ks, kl);
+        for (int t = 0; t < 2; ++t) prefill_window_again<T, 128>(a, win, qs, 64 * Q + 32 * t, n_q, head, ks, n_k, bad_l);
       });
     }
   }
