@@ -230,9 +230,11 @@ static bool quant8_takes_vec(const Quant8Args& a, const PagedAddr& addr, const t
 
 template <typename T, typename C, bool STORE>
 static int launch_quant8_vec(const Quant8Args& a, const PagedAddr& addr, hipStream_t stream, const char* what) {
-  // Prompts: two heads a workgroup share a token's lookup (the 16 prompts' store
-  // and the 8 prefixes' load: 24.7 and 25.1 us; eight heads 25.3 and 26.9, one
-  // 26.3 and 29.5). Few tokens: one head each, for more workgroups.
+  // Heads a workgroup: one for few tokens, for more workgroups, two for many, which
+  // share a token's lookup. Both sides, one / two, us, e4m3, 8 heads of 128 dims: 64
+  // tokens store 3.6 / 4.5, load 3.2 / 3.5; 1024 4.5 / 5.3 and 4.3 / 4.4; 2048 6.2 /
+  // 6.4 and 5.5 / 5.4; 4096 9.9 / 10.3 and 9.2 / 8.3; 16384 26.9 / 27.3 and 28.9 / 24.7.
+  // (Eight: 16 prompts' store 25.3 against 24.7, 8 prefixes' load 26.9 against 25.1.)
   const int tok = 256 / static_cast<int>(a.D / 8), heads = a.T >= 2048 ? 2 : 1;
   const dim3 grid(static_cast<uint32_t>((a.T + tok - 1) / tok), static_cast<uint32_t>((a.H + heads - 1) / heads));
   if (a.D == 128) quant8_vec<T, C, 128, STORE><<<grid, dim3(256), 0, stream>>>(a, addr, heads);

@@ -5,9 +5,11 @@
 namespace tsa {
 
 // Workgroups a call's units are split into, at least, where there are tokens for
-// it (64 sequences of 512-4096 tokens, 16 nodes, 32/8 heads: 512 127 us, 1024 160;
-// 32 nodes: 146, 191; 8 of 8192 with 64 nodes, 64/8 heads: 181, 196), and
-// the least blocks of a split (one sequence of 300 tokens: 16 14.9 us, 4 18.1).
+// it (64 sequences of 512-4096 tokens, 16 nodes, 32/8 heads: 512 126 us, 1024 158;
+// 32 nodes: 144, 187; 8 of 8192 with 64 nodes, 64/8 heads: 177, 188), and the least
+// blocks of a split. (16 was the faster before tree_per_split dealt the blocks evenly;
+// with it 4 is: 8 nodes, 32/8 heads, one sequence of 300 / 1000 / 2000 tokens: 13.8 /
+// 17.7 / 17.7 us against 12.7 / 14.3 / 13.7. Larger plans have not been measured so.)
 constexpr int64_t kTreeWorkgroups = 512, kTreeMinSplit = 16;
 
 TreeRowsPlan tree_rows_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap) {

@@ -20,9 +20,14 @@ static int stream_workgroups() {
   return cus;
 }
 
-// Units of this many splits or more read K/V with non-temporal loads.
-constexpr int kRowsNtSplits = 16;
-
+// A unit that is one workgroup reads K/V with ordinary loads, a split's workgroup
+// with non-temporal ones. Both sides, ordinary / non-temporal, us, caches of several
+// calls in turn (past what the chip keeps, but for the first): one workgroup, e4m3 /
+// bf16, 4 x 16-512 tokens, 16/8 heads 8.2 / 8.6 and 9.4 / 10.9, 64 x 100-512, 32/8
+// heads 16.4 / 15.5 and 25.0 / 23.9, 256 of them 45.2 / 44.3 and 79.1 / 79.9; splits,
+// 32/8 heads, 16 x 512-1024 14.7 / 13.8 and 18.8 / 16.2, 16 x 1024-2048 21.1 / 19.8
+// and 29.7 / 26.4, 4 x 2048-4096 15.7 / 15.2 and 18.8 / 17.3, 1 x 16384-32768 21.3 /
+// 19.6 and 27.5 / 24.4.
 template <typename T, typename C, int D>
 static int launch_unit(const RowsArgs& a, hipStream_t stream, const char* what) {
   const int groups = (a.G + 15) / 16, items = a.B * a.Hkv * groups, rows = a.G < 16 ? a.G : 16;
@@ -33,10 +38,7 @@ static int launch_unit(const RowsArgs& a, hipStream_t stream, const char* what) 
     return check_launch(what);
   }
   const dim3 grid(static_cast<uint32_t>(items) * a.S), threads(64 * kUnitWavesSplit);
-  if (a.S >= kRowsNtSplits)
-    paged_rows_unit<T, C, D, kUnitWavesSplit, true><<<grid, threads, kUnitWavesSplit * row_bytes, stream>>>(a, a.bt, a.lens, a.part);
-  else
-    paged_rows_unit<T, C, D, kUnitWavesSplit, false><<<grid, threads, kUnitWavesSplit * row_bytes, stream>>>(a, a.bt, a.lens, a.part);
+  paged_rows_unit<T, C, D, kUnitWavesSplit, true><<<grid, threads, kUnitWavesSplit * row_bytes, stream>>>(a, a.bt, a.lens, a.part);
   if (int rc = check_launch(what)) return rc;
   launch_rows_merge<T, D>(a, a.G, kUnitWavesSplit * kUnitTiles, stream);
   return check_launch(what);
