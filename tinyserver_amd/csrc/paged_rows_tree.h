@@ -18,6 +18,11 @@
 //     accumulates row c, so the softmax's scales are the lane's own.
 // K of the next block is asked for as soon as the scores have taken this
 // block's, V after the second product.
+// A weight goes to the second product rounded once to T, off by at most 2^-8 (f16:
+// 2^-11) of itself, as in the prefill kernels; the decode kernels' two halves would
+// double that product, which bounds wide trees. So a tree's outputs are a little
+// further from 64 bits (2-norm, relative: 0.0023, f16 0.00029) than a decode
+// step's (0.0017, 0.00021, their own rounding), a tree of one node's too.
 //
 // A block of keys that every row sees (all of the context's but the last) takes
 // no mask. In the others each row has 32 bits: the context's tokens and its own

@@ -7,7 +7,10 @@
 // varlen_window_w64   head_dim 128, groups of 12, 16, ...: 64 queries a wave
 //                     (prefill_w64_body), both over the blocks of the window and
 //                     of the first keys;
-// varlen_prefill_mfma other groups;
+// varlen_prefill_mfma other groups (all three round a weight once to the type for the
+//                     second product, as the prefill without a window does: at most
+//                     2^-8, f16 2^-11, of itself; outputs 0.0021 from 64 bits where
+//                     their own rounding is 0.0016, bf16);
 // varlen_window_generic  float32, other head_dims, strides and scales: one wave
 //                     per (query, q-head), VALU.
 #include "varlen_prefill_mfma.h"

@@ -65,11 +65,13 @@ def load_kv_cache_quantized(
     """Rows of an 8-bit cache as packed (num_tokens, Hkv, D) keys and values of ``dtype``.
 
     Addressing as ``store_kv_cache_quantized``'s: what it wrote for a packed
-    batch, this reads for the same cu_seqlens and positions (a cached prefix
-    for ``flash_attn_varlen_func``, say). Each value is ``code * scale``
-    in float32, rounded to ``dtype``. A token that no sequence holds, or whose page is past the
-    table or outside the pool, reads as 0. k_out and v_out, if given, set the
-    dtype.
+    batch, this reads for the same cu_seqlens and positions: a sequence on its
+    way to a 16-bit pool (``store_kv_cache_paged``) or out of the cache. (The
+    varlen functions place a sequence's queries at its start, so a chunk's
+    queries behind rows read here are not theirs to attend from.) Each value
+    is ``code * scale`` in float32, rounded to ``dtype``. A token that no
+    sequence holds, or whose page is past the table or outside the pool, reads
+    as 0. k_out and v_out, if given, set the dtype.
     """
     if k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("k_cache and v_cache must be 4D tensors (num_blocks, num_kv_heads, block_size, head_dim)")

@@ -46,7 +46,9 @@ def paged_attention_tree(
     gives 0.
 
     ``max_nodes``: at least the largest number of nodes a sequence has; by
-    default the most that the mask's width and N allow. Rows past max_nodes or
+    default the most that the mask's width and N allow. Give it where it is
+    known: the kernel, the splits and the workspace go by it, and small trees
+    of a large batch would be taken for ones of 64 nodes. Rows past max_nodes or
     the mask's width in their sequence, and rows outside
     ``cu_nodes[0]:cu_nodes[B]``, are left as they were in ``out``.
     """
