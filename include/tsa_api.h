@@ -50,6 +50,13 @@
  *   tsa_paged_tree          no counterpart: the same for drafted tokens' trees
  *   tsa_varlen_prefill_window  no counterpart: flash_attn_varlen_func with a
  *                           sliding window and first tokens
+ *   tsa_step_tables         server/model/block_manager.py:102-134 (the new tokens'
+ *                           pages) and server/model/patches/qwen3.py:296-318,
+ *                           388-397 (mappings and padded tables), on the device
+ *   tsa_paged_chunk         no counterpart: attention of new tokens over a paged
+ *                           cache that holds tokens before them
+ *   tsa_token_logprobs      no counterpart: log probabilities, entropy and the
+ *                           most likely tokens of rows of logits
  */
 #ifndef TSA_API_H
 #define TSA_API_H
@@ -353,6 +360,67 @@ int tsa_varlen_prefill_window(const tsa_view* out, const tsa_view* q, const tsa_
                               const tsa_view* v, const tsa_view* cu_seqlens_q,
                               const tsa_view* cu_seqlens_k, int64_t max_seqlen_q, int64_t max_seqlen_k,
                               int64_t window, int64_t sinks, double softmax_scale, void* stream);
+
+/* A step's tables from its requests' lengths, one launch. tables (R, W) int32
+ * holds the block tables of all requests, request s's in row rows[s] (rows NULL:
+ * row s). With context_lens[s] cached and query_lens[s] new tokens (both (B) int32,
+ * taken within [0, 2^30)) and pages of block_size tokens, request s holds have =
+ * ceil(context / block_size) pages and needs need = ceil((context + query) /
+ * block_size), both at most W. With free_blocks (F) int32, columns have .. need - 1
+ * of its table take the next entries of that list, from entry num_free - 1
+ * downwards (num_free (1) int32, within [0, F]; NULL: F) in request order, -1 past
+ * its end, and free_left (1) = num_free - the pages needed. Without it (num_free and
+ * free_left NULL) have = need. Outputs, all int32: block_tables (B, width), the
+ * first `need` entries, then 0; cu_seqlens (B + 1) and seq_lens (B) =
+ * context + query (saturating); for new token t of the T that positions,
+ * block_mapping and slot_mapping hold: its position, its page and its slot there
+ * (page -1 past column W), or 0, -1 and -1 where no request has it. A row outside
+ * tables takes no page; its page entries are -1. A row may stand once in rows.
+ * free_left may not be num_free. */
+int tsa_step_tables(const tsa_view* block_tables, const tsa_view* cu_seqlens, const tsa_view* seq_lens,
+                    const tsa_view* positions, const tsa_view* block_mapping, const tsa_view* slot_mapping,
+                    const tsa_view* free_left, const tsa_view* tables, const tsa_view* rows,
+                    const tsa_view* context_lens, const tsa_view* query_lens, const tsa_view* free_blocks,
+                    const tsa_view* num_free, int64_t block_size, void* stream);
+
+/* Bytes of workspace tsa_paged_chunk needs for calls of these sizes on the current
+ * device: the partial results of rows whose keys are split; 0 where none are. */
+size_t tsa_paged_chunk_workspace_bytes(int64_t num_seqs, int64_t num_tokens, int64_t max_seqlen, int64_t num_heads,
+                                       int64_t num_kv_heads, int64_t head_dim, int64_t max_blocks_per_seq,
+                                       int64_t block_size);
+
+/* Attention of a chunk of new tokens over the paged cache. Sequence s's new tokens
+ * are rows cu_seqlens[s] .. cu_seqlens[s + 1] of query/out (N, Hq, D), cu_seqlens
+ * (B + 1) int32 non-decreasing; row i stands at position context_lens[s] + i, where
+ * its key and value are in the caches (NB, Hkv, BS, D) of query's dtype already, and
+ * sees the positions up to its own, kv head h / (Hq / Hkv). At most max_seqlen rows a
+ * sequence are computed; rows past those, and rows outside every sequence, are left
+ * as they were. A token whose page id is outside the pool, or past the table, is not
+ * seen, and what is not seen has no influence, whatever its rows hold; a row that
+ * sees nothing gives 0. A seen value of V that is not finite makes the output of its
+ * dim not finite (an infinity may come out as NaN). The workspace (256-byte aligned)
+ * needs no initialisation; calls that share one must be ordered on one stream. out
+ * may not overlap an input. */
+int tsa_paged_chunk(const tsa_view* out, const tsa_view* query, const tsa_view* k_cache, const tsa_view* v_cache,
+                    const tsa_view* block_tables, const tsa_view* context_lens, const tsa_view* cu_seqlens,
+                    int64_t max_seqlen, double softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace tsa_token_logprobs needs: the partial results of rows that
+ * are split over workgroups; 0 where none are. */
+size_t tsa_token_logprobs_workspace_bytes(int64_t num_tokens, int64_t vocab_size, int64_t num_top);
+
+/* For each row x of logits (N, V) (bf16, f16 or f32), in f32: logprobs[n] =
+ * log softmax(x)[tokens[n]] (tokens (N) int32 or int64; -inf for one outside [0,
+ * V)), entropy[n] = -sum p log p in nats, and the num_top largest logits' log
+ * probabilities and indices in top_logprobs (N, num_top) f32 and top_tokens (N,
+ * num_top) int64, falling, the lowest index first where logits tie (0 and -0 do) and
+ * NaN last. A logit of -inf has p = 0 and adds nothing. A row that holds a NaN or
+ * +inf, or nothing but -inf, has NaN for all its log probabilities and its entropy.
+ * num_top is at most V and 64. The workspace (256-byte aligned) needs no
+ * initialisation; calls that share one must be ordered on one stream. */
+int tsa_token_logprobs(const tsa_view* logprobs, const tsa_view* entropy, const tsa_view* top_logprobs,
+                       const tsa_view* top_tokens, const tsa_view* logits, const tsa_view* tokens,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -85,6 +85,11 @@ SIGNATURES = {
     ),
     "tsa_paged_tree": (c_int, [_V] * 8 + [c_int64, c_double, c_void_p, c_size_t, c_void_p]),
     "tsa_varlen_prefill_window": (c_int, [_V] * 6 + [c_int64, c_int64, c_int64, c_int64, c_double, c_void_p]),
+    "tsa_step_tables": (c_int, [_V] * 13 + [c_int64, c_void_p]),
+    "tsa_paged_chunk_workspace_bytes": (c_size_t, [c_int64] * 8),
+    "tsa_paged_chunk": (c_int, [_V] * 7 + [c_int64, c_double, c_void_p, c_size_t, c_void_p]),
+    "tsa_token_logprobs_workspace_bytes": (c_size_t, [c_int64] * 3),
+    "tsa_token_logprobs": (c_int, [_V] * 6 + [c_void_p, c_size_t, c_void_p]),
 }
 
 ABI_VERSION = 1
@@ -126,7 +131,8 @@ def host():
         except ImportError as e:
             raise RuntimeError("tinyserver_amd/_tsa_host.so is missing or does not load: build it first "
                                "(python -m tinyserver_amd._build or __graft_entry__.build())") from e
-        _entry.update({name: i for i, name in enumerate((*_tsa_host.entries(), *_tsa_host.extra_entries()))})
+        _entry.update({name: i for i, name in enumerate(
+            (*_tsa_host.entries(), *_tsa_host.extra_entries(), *_tsa_host.step_entries()))})
         _host = _tsa_host
     return _host
 

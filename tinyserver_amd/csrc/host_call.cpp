@@ -18,7 +18,8 @@
 namespace {
 
 enum Entry { kDecode, kDecodeStep, kNormRope, kNormRopeStore, kPrefill, kMixed, kSample, kSampleWs,
-             kStoreQuant, kLoadQuant, kDecodeWindow, kTree, kPrefillWindow };
+             kStoreQuant, kLoadQuant, kDecodeWindow, kTree, kPrefillWindow,
+             kStepTables, kChunk, kLogprobs };
 struct Shape { const char* name; int views, doubles, ints; };
 constexpr Shape kShapes[] = {
     {"tsa_paged_decode", 6, 1, 4},      {"tsa_paged_decode_step", 12, 2, 4}, {"tsa_qk_norm_rope", 8, 1, 1},
@@ -26,11 +27,12 @@ constexpr Shape kShapes[] = {
     {"tsa_sample_tokens", 6, 0, 1},     {"tsa_sample_tokens_ws", 6, 0, 3},
     {"tsa_store_kv_quantized", 9, 0, 1}, {"tsa_load_kv_quantized", 9, 0, 1}, {"tsa_paged_decode_window", 8, 1, 5},
     {"tsa_paged_tree", 8, 1, 4},        {"tsa_varlen_prefill_window", 6, 1, 5},
+    {"tsa_step_tables", 13, 0, 2},      {"tsa_paged_chunk", 7, 1, 4},         {"tsa_token_logprobs", 6, 0, 3},
 };
 constexpr int kEntries = sizeof(kShapes) / sizeof(kShapes[0]);
-// entries() lists the reference's path, the entry points before this one;
-// extra_entries() the others.
-constexpr int kExtra = kStoreQuant;
+// entries() lists the reference's path, the entry points before kExtra;
+// extra_entries() the 8-bit cache, windows and trees; step_entries() the others.
+constexpr int kExtra = kStoreQuant, kStep = kStepTables;
 constexpr int kMaxViews = 16, kMaxDoubles = 4, kMaxInts = 8;
 
 // A tensor's view, as _lib.view describes it. False with a Python error set
@@ -96,6 +98,14 @@ int run(int e, const tsa_view* const* v, const double* d, const int64_t* i) {
                             static_cast<size_t>(i[2]), p(3));
     case kPrefillWindow:
       return tsa_varlen_prefill_window(v[0], v[1], v[2], v[3], v[4], v[5], i[0], i[1], i[2], i[3], d[0], p(4));
+    case kStepTables:
+      return tsa_step_tables(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9], v[10], v[11], v[12], i[0],
+                             p(1));
+    case kChunk:
+      return tsa_paged_chunk(v[0], v[1], v[2], v[3], v[4], v[5], v[6], i[0], d[0], p(1), static_cast<size_t>(i[2]),
+                             p(3));
+    case kLogprobs:
+      return tsa_token_logprobs(v[0], v[1], v[2], v[3], v[4], v[5], p(0), static_cast<size_t>(i[1]), p(2));
     default:
       return tsa_sample_tokens_ws(v[0], v[1], v[2], v[3], v[4], v[5], p(0), static_cast<size_t>(i[1]), p(2));
   }
@@ -165,20 +175,22 @@ PyObject* device_index(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// The entry points call() knows, in order: entries(), then extra_entries().
+// The entry points call() knows, in order: entries(), extra_entries(), step_entries().
 PyObject* names(int from, int to) {
   PyObject* t = PyTuple_New(to - from);
   for (int e = from; t && e < to; ++e) PyTuple_SET_ITEM(t, e - from, PyUnicode_FromString(kShapes[e].name));
   return t;
 }
 PyObject* entries(PyObject*, PyObject*) { return names(0, kExtra); }
-PyObject* extra_entries(PyObject*, PyObject*) { return names(kExtra, kEntries); }
+PyObject* extra_entries(PyObject*, PyObject*) { return names(kExtra, kStep); }
+PyObject* step_entries(PyObject*, PyObject*) { return names(kStep, kEntries); }
 
 PyMethodDef kMethods[] = {
     {"call", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(call)), METH_FASTCALL, nullptr},
     {"device_index", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(device_index)), METH_FASTCALL, nullptr},
     {"entries", entries, METH_NOARGS, nullptr},
     {"extra_entries", extra_entries, METH_NOARGS, nullptr},
+    {"step_entries", step_entries, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tsa_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

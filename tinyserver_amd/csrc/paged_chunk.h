@@ -1,0 +1,54 @@
+// Attention of a chunk of new tokens a sequence over the paged cache that holds
+// them and the tokens before them (tsa_paged_chunk): the argument block, what a row
+// sees, and what the entry point calls.
+#pragma once
+
+#include <cmath>
+
+#include "tsa_common.h"
+
+namespace tsa {
+
+struct ChunkArgs {
+  void* out;
+  const void* q;
+  const void* kc;
+  const void* vc;
+  const int32_t* bt;
+  const int32_t* ctx;  // (B) tokens of each sequence before its new ones
+  const int32_t* cu;   // (B + 1) ranges of the packed new tokens
+  int64_t o_sr, o_sh, o_sd, q_sr, q_sh, q_sd;
+  int64_t kc_b, kc_h, kc_s, kc_d, vc_b, vc_h, vc_s, vc_d;
+  int64_t bt_s0, bt_s1, ctx_s, cu_s;
+  int64_t NB, N;  // pages; packed rows
+  int32_t B, Hq, Hkv, G, BS, max_blocks, D;
+  int32_t T;      // rows of a sequence that are computed, at most
+  float scale_log2;
+};
+
+constexpr float kNegInfC = -INFINITY;
+
+// A sequence's rows row0 .. row0 + n - 1 of q/out stand at positions ctx ..; end:
+// past its last token that the block table holds. Row i sees the keys below
+// min(ctx + i + 1, end).
+struct ChunkSeq {
+  int ctx, n, end;
+  int64_t row0;
+};
+__device__ __forceinline__ ChunkSeq chunk_seq(const ChunkArgs& a, int s) {
+  ChunkSeq r;
+  const int64_t cap = static_cast<int64_t>(a.max_blocks) * a.BS;  // (below 2^27)
+  int64_t c = a.ctx[s * a.ctx_s];
+  c = c < 0 ? 0 : c > cap ? cap : c;
+  int64_t r0 = a.cu[s * a.cu_s], r1 = a.cu[(s + 1) * a.cu_s];
+  r0 = r0 < 0 ? 0 : r0 > a.N ? a.N : r0;
+  r1 = r1 < r0 ? r0 : r1 > a.N ? a.N : r1;
+  const int64_t n = r1 - r0 < a.T ? r1 - r0 : a.T;
+  r.ctx = static_cast<int>(c);
+  r.n = static_cast<int>(n);
+  r.end = static_cast<int>(c + n < cap ? c + n : cap);
+  r.row0 = r0;
+  return r;
+}
+
+}  // namespace tsa

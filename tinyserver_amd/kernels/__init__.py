@@ -6,15 +6,20 @@ the gfx950 HIP library; plus the fused QK RMSNorm + RoPE the reference runs as
 eager PyTorch, the batched sampler of server/model/sampling.py, and a
 continuous-batching step's prefill and decode attention in one launch; the
 paged cache in 8 bits, attention with a sliding window and first tokens, and
-attention of drafted tokens' trees.
+attention of drafted tokens' trees; a step's block tables and slots built on the
+GPU, attention of a chunk of new tokens over the paged cache, and log
+probabilities of given tokens.
 """
 
+from .chunk_attention import paged_attention_chunk
 from .kv_cache import store_kv_cache, store_kv_cache_batched, store_kv_cache_paged
 from .kv_cache_quantized import load_kv_cache_quantized, paged_attention_quantized, store_kv_cache_quantized
+from .logprobs import TokenLogprobs, token_logprobs
 from .mixed_attention import mixed_attention
 from .paged_attention import paged_attention_forward, paged_decode_step
 from .qk_norm_rope import qk_norm_rope, qk_norm_rope_store
 from .sampling import sample_tokens
+from .step_tables import StepTables, step_tables
 from .tree_attention import paged_attention_tree
 from .varlen_attention import flash_attn_varlen_func
 from .window_attention import flash_attn_varlen_window, paged_attention_window
@@ -36,4 +41,9 @@ __all__ = [
     "paged_attention_window",
     "flash_attn_varlen_window",
     "paged_attention_tree",
+    "paged_attention_chunk",
+    "StepTables",
+    "step_tables",
+    "TokenLogprobs",
+    "token_logprobs",
 ]
