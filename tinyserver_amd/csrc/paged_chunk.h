@@ -5,7 +5,7 @@
 
 #include <cmath>
 
-#include "tsa_common.h"
+#include "paged_rows.h"
 
 namespace tsa {
 
@@ -24,6 +24,12 @@ struct ChunkArgs {
   int32_t B, Hq, Hkv, G, BS, max_blocks, D;
   int32_t T;      // rows of a sequence that are computed, at most
   float scale_log2;
+  // The matrix-core form: page strides in bytes, the tiles (16 tokens) of a page as
+  // a multiplier and a shift (page_of_tile), whether output rows go in 8-byte
+  // pieces; the queries of a row block, the least blocks of a run, whether runs are
+  // whole items, and 2^16 / G rounded up (row / G of the 128 rows of a block).
+  uint32_t k_page, v_page, page_mul, page_shift;
+  int32_t out8, QB, min_run, whole, g_mul;
 };
 
 constexpr float kNegInfC = -INFINITY;
@@ -50,5 +56,14 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkArgs& a, int s) {
   r.row0 = r0;
   return r;
 }
+
+// paged_chunk_stream.hip: the plan of a call on the matrix cores (runs 0: sizes past
+// its limits) and its launch.
+struct ChunkPlan {
+  int runs, QB, min_run, whole;
+  size_t bytes;
+};
+ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap);
+int chunk_stream_launch(const ChunkArgs& a, const ChunkPlan& p, int dt, void* workspace, hipStream_t stream);
 
 }  // namespace tsa

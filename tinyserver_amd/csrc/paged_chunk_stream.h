@@ -1,0 +1,699 @@
+// Attention of a chunk over the paged cache on the matrix cores: a run of 32-key
+// blocks a workgroup, whatever sequences they belong to.
+//
+// An item is (sequence, kv head, row block): QB queries times the G q-heads of the kv
+// head, up to 32 NW rows (row = query G + head), so that one K/V byte serves all of
+// them and a wave takes 32 rows. Item i has as many 32-key blocks as its last query
+// sees. A step may hold one sequence with 2048 new tokens beside sixty with one, over
+// a few or 30,000 cached ones, so work is not dealt by sequence: all items' blocks in
+// a row (sequence, kv head, row block), total W, are cut into runs of ceil(W / P)
+// blocks, one a workgroup, and an item that a cut goes through is put together by a
+// second launch from its runs' partial results. The lengths are on the device only:
+// each workgroup sums them itself and looks its start up (chunk_start).
+// Runs that follow each other share K and V and go to one XCD.
+//
+// In a workgroup K and V go from their pages straight into LDS
+// (global_load_lds_dwordx4, no registers), NB slots of each, A = NB - 1 blocks ahead;
+// page ids come from a table in LDS that a segment's prologue fills. With lane (h, c)
+// = (lane / 32, lane % 32), v_mfma_f32_32x32x16:
+//   S^T(32 keys x 32 rows) = K Q^T: lane (h, c) reads key c, dims 16 j + 8 h..+8, and
+//     holds row c's Q; element e of the result is the score of key 8 (e / 4) + 4 h +
+//     e % 4 for row c;
+//   O^T(dims x 32 rows) += V^T P^T over two 16-key steps: the P^T operand is the lane's
+//     own weights, V's comes from transposed LDS reads. Lane (h, c) accumulates row c,
+//     so the softmax's scales are the lane's own.
+// The 16-byte chunk ch of LDS row r sits at position ch ^ swz(r), free of bank
+// conflicts in both reads. S(j + 1) runs under the exponentials of block j, P V of
+// block j - 1 under its maximum; two workgroups a CU give a SIMD two waves, of which
+// one's exponentials run under the other's products.
+//
+// Blocks that every row sees whole take no mask. The others (the chunk's own last
+// ones, and those with a page that is not there) leave the pipeline and follow one at
+// a time: there scores that a row does not see become -inf, V rows that are not there
+// become 0, and elements of V that are not finite reach the rows that see them through
+// a product of flags (a weight of 0 times one would be NaN).
+// A weight goes to the second product rounded once to T, off by at most 2^-8 (f16:
+// 2^-11) of itself, as in the prefill kernels.
+#pragma once
+
+#include "nonfinite.h"
+#include "paged_chunk.h"
+
+namespace tsa {
+
+constexpr int kChunkSlots = 4;       // K/V blocks in LDS
+constexpr int kChunkTab = 1024;      // 32-key blocks that the page table in LDS holds
+constexpr float kChunkRescale = 8.f; // log2 units a maximum grows before it moves
+
+// ---- The plan on the device.
+// 32-key blocks of a sequence's row blocks 0 .. i - 1: sum of ceil(min(ctx + (k + 1)
+// QB, end) / 32). With QB = 32 qh + ql the remainders of ql repeat after 32 terms.
+__device__ __forceinline__ int64_t chunk_blocks(int ctx, int end, int QB, int i) {
+  const int full = min(i, (end - ctx) / QB), ql = QB & 31, y = ctx + QB + 31;
+  int64_t sum = static_cast<int64_t>(i - full) * ((end + 31) >> 5) + static_cast<int64_t>(y >> 5) * full +
+                static_cast<int64_t>(QB >> 5) * full * (full - 1) / 2;
+  if (ql) {
+    const int K = full >> 5, J = full & 31;
+    int all = 0, part = 0, v = y & 31;
+    for (int j = 0; j < 32; ++j, v += ql) {
+      all += v >> 5;
+      part += j < J ? v >> 5 : 0;
+    }
+    sum += static_cast<int64_t>(K) * all + static_cast<int64_t>(ql) * (16 * static_cast<int64_t>(K) * (K - 1) + static_cast<int64_t>(K) * J) + part;
+  }
+  return sum;
+}
+__device__ __forceinline__ int chunk_row_blocks(const ChunkSeq& r, int QB) { return (r.n + QB - 1) / QB; }
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x)));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32)));
+  return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+__device__ __forceinline__ ChunkSeq chunk_seq_uniform(const ChunkArgs& a, int s) {
+  ChunkSeq r = chunk_seq(a, s);
+  r.ctx = __builtin_amdgcn_readfirstlane(r.ctx);
+  r.n = __builtin_amdgcn_readfirstlane(r.n);
+  r.end = __builtin_amdgcn_readfirstlane(r.end);
+  r.row0 = uniform64(r.row0);
+  return r;
+}
+
+// Where a run starts: block `blk` of row block rb of (sequence s, kv head kvh).
+struct ChunkStart {
+  int s, kvh, rb, blk;
+};
+// A segment: blocks blk0 .. blk1 - 1 of an item's nblk. In LDS, with what its next
+// one follows from.
+struct ChunkSegment {
+  int32_t s, kvh, nq, pos, end;  // pos: position of the item's first query
+  int32_t blk0, blk1, nblk;      // blk1 0: no more
+  int64_t row;                   // packed row of that query
+};
+struct ChunkWork {
+  ChunkSegment seg;
+  ChunkSeq r;
+  int32_t rb, left;
+  // The segment from block blk of row block rb on. One thread.
+  __device__ __forceinline__ void set(const ChunkArgs& a, int blk) {
+    const int q0 = rb * a.QB;
+    seg.nq = min(a.QB, r.n - q0);
+    seg.pos = r.ctx + q0;
+    seg.end = r.end;
+    seg.row = r.row0 + q0;
+    seg.nblk = (min(seg.pos + seg.nq, r.end) + 31) >> 5;  // keys that its last query sees
+    seg.blk0 = blk;
+    seg.blk1 = a.whole ? seg.nblk : min(seg.nblk, blk + left);
+    left -= seg.blk1 - blk;
+  }
+  __device__ __forceinline__ void next(const ChunkArgs& a) {
+    if (left <= 0) {
+      seg.blk1 = 0;
+      return;
+    }
+    if (++rb * a.QB >= r.n) {
+      rb = 0;
+      if (++seg.kvh == a.Hkv) {
+        seg.kvh = 0;
+        do r = chunk_seq(a, ++seg.s);
+        while (r.n == 0 && seg.s < a.B - 1);
+      }
+    }
+    set(a, 0);
+  }
+};
+// What a workgroup's second launch needs of run r: the item that r starts inside of.
+struct ChunkSplit {
+  int64_t row0;              // packed row of the item's first query
+  int32_t kvh, queries;      // its kv head and queries
+  int32_t runs;              // runs r .. r + runs - 1 end it; 0: r is not its first cut
+};
+constexpr size_t kChunkHead = 64;  // bytes before the splits: the number of runs
+// A partial result: 32 NW rows, in the order of the lanes' accumulators, then each
+// row's maximum and sum.
+template <int D, int NW> constexpr int chunk_part_floats() { return 32 * NW * (D + 2); }
+
+template <int NT>
+__device__ __forceinline__ uint64_t chunk_scan(uint64_t x, uint64_t* waves, uint64_t& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint64_t incl = wave_scan_u64(x);
+  if (lane == 63) waves[w] = incl;
+  __syncthreads();
+  uint64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) {
+    before += i < w ? waves[i] : 0;
+    total += waves[i];
+  }
+  __syncthreads();
+  return before + incl - x;
+}
+
+// The blocks of all items, and the place of block run * per of them, per = the blocks
+// of a run. smem: 64 + 8 bytes. All threads call.
+template <int NT>
+__device__ __forceinline__ bool chunk_start(const ChunkArgs& a, uint64_t* smem, int P, int64_t& total, int& per, int& run,
+                                            ChunkStart& st) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  auto weight = [&](int s) -> uint64_t {
+    if (s >= a.B) return 0;
+    const ChunkSeq r = chunk_seq(a, s);
+    return static_cast<uint64_t>(chunk_blocks(r.ctx, r.end, a.QB, chunk_row_blocks(r, a.QB))) * a.Hkv;
+  };
+  uint64_t mine = 0, sum;
+  for (int s = tid; s < a.B; s += NT) mine += weight(s);
+  chunk_scan<NT>(mine, smem, sum);
+  total = uniform64(static_cast<int64_t>(sum));
+  const int64_t even = (total + P - 1) / P;
+  per = __builtin_amdgcn_readfirstlane(static_cast<int>(even > a.min_run ? even : a.min_run));
+  const int runs = static_cast<int>((total + per - 1) / per);
+  // Runs of an XCD (workgroups go round the XCDs) follow each other.
+  const int of_xcd = (runs + 7) >> 3, i = static_cast<int>(blockIdx.x) >> 3;
+  run = (static_cast<int>(blockIdx.x) & 7) * of_xcd + i;
+  if (i >= of_xcd || run >= runs) return false;
+  const uint64_t x0 = static_cast<uint64_t>(run) * per;
+  uint64_t before = 0;
+  int32_t* const found = reinterpret_cast<int32_t*>(smem + 8);
+  for (int base = 0; base < a.B; base += NT) {
+    const uint64_t w = weight(base + tid), b = before + chunk_scan<NT>(w, smem, sum);
+    if (b <= x0 && x0 < b + w) {
+      found[0] = base + tid;
+      reinterpret_cast<uint64_t*>(found)[1] = x0 - b;
+    }
+    before += sum;
+    if (x0 < before) break;  // (uniform)
+  }
+  __syncthreads();
+  st.s = __builtin_amdgcn_readfirstlane(found[0]);
+  int64_t off = uniform64(reinterpret_cast<int64_t*>(found)[1]);
+  __syncthreads();
+  const ChunkSeq r = chunk_seq_uniform(a, st.s);
+  const int RB = chunk_row_blocks(r, a.QB);
+  const int64_t head = uniform64(chunk_blocks(r.ctx, r.end, a.QB, RB));
+  st.kvh = __builtin_amdgcn_readfirstlane(static_cast<int>(off / head));
+  off -= head * st.kvh;
+  int lo = 0, n = RB;  // the row block is one of lo .. lo + n - 1
+  while (n > 1) {
+    const int step = (n + 63) >> 6, k = min(lo + lane * step, RB);
+    const int at = __builtin_popcountll(__ballot(lane * step < n && chunk_blocks(r.ctx, r.end, a.QB, k) <= off)) - 1;
+    n = min(step, n - at * step);
+    lo += at * step;
+  }
+  st.rb = lo;
+  st.blk = __builtin_amdgcn_readfirstlane(static_cast<int>(off - chunk_blocks(r.ctx, r.end, a.QB, lo)));
+  return true;
+}
+
+// The arguments, read where they are used: held in registers from the start, those
+// that only a segment's ends need would spill others' out of the loop over blocks.
+// (The kernel's first parameter is its ChunkArgs.)
+__device__ __forceinline__ const ChunkArgs& chunk_args() {
+  typedef const __attribute__((address_space(4))) ChunkArgs* Ptr;
+  Ptr p = (Ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const ChunkArgs*)p;
+}
+
+template <int D> constexpr int chunk_lds_bytes() { return 2 * kChunkSlots * 32 * 2 * D + kChunkTab * 8 + 16 + sizeof(ChunkWork); }
+
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_stream(
+    ChunkArgs a, const int32_t* __restrict__ bt, int32_t* __restrict__ head, ChunkSplit* __restrict__ splits,
+    float* __restrict__ part) {
+  constexpr int KJ = D / 16, NU = D / 32, CPR = D / 8, RB = 2 * D, BLKB = 32 * RB;
+  constexpr int NB = kChunkSlots, A = NB - 1;
+  constexpr int RPI = 1024 / RB;            // rows of a 1 KB load instruction
+  constexpr int IPW = 2 * (32 / RPI) / NW;  // load instructions of a wave and block
+  constexpr int IPH = 16 / RPI;             // load instructions of a 16-row half
+  constexpr int VOFF = NB * BLKB, TOFF = 2 * NB * BLKB;
+  constexpr int kInFlight = (A - 1) * IPW;
+  __shared__ __align__(16) char smem[chunk_lds_bytes<D>()];
+  int32_t* const tab = reinterpret_cast<int32_t*>(smem + TOFF);  // page id of each half of the blocks, -1: none
+  int32_t* const first_bad = tab + 2 * kChunkTab;                // the first block with such a half
+  ChunkWork* const work = reinterpret_cast<ChunkWork*>(first_bad + 4);
+
+  int64_t total;
+  int per, run;
+  ChunkStart st;
+  const int P = static_cast<int>(gridDim.x);
+  const bool has = chunk_start<64 * NW>(a, reinterpret_cast<uint64_t*>(smem), P, total, per, run, st);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *head = static_cast<int32_t>((total + per - 1) / per);
+  if (!has) return;
+
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float cs = a.scale_log2;  // > 0 here
+
+  // ---- Loads: waves 0 .. NW / 2 - 1 the K rows, the others the V rows, IPW
+  // instructions of RPI rows; lane l of one whose first row is R0 fetches the
+  // chunk that belongs at row R0 + l / CPR, position l % CPR. Halves without a
+  // page read page 0's first rows (masked); blocks past the last repeat it.
+  auto swz = [](int x) {
+    return D == 128 ? ((x & 3) << 2) | ((x >> 2) & 3) : (((x >> 1) & 1) << 2) | ((x >> 2) & 3);
+  };
+  typedef __attribute__((address_space(3))) void lds_void;
+  const uint32_t smem_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)smem));
+  const bool k_wave = wave < NW / 2;
+  const int row0w = (wave % (NW / 2)) * IPW * RPI;
+  const uint32_t slot_b = static_cast<uint32_t>(k_wave ? a.kc_s : a.vc_s) * 2, page_b = k_wave ? a.k_page : a.v_page;
+  const uint32_t lds_w = smem_lds + (k_wave ? 0 : VOFF) + row0w * RB;  // this wave's rows of slot 0
+  const int lrow = lane / CPR;
+  // The lane's place in instruction i: row r0w % 16 + i RPI + lrow of the half, chunk
+  // (lane % CPR) ^ swz(that row), where i changes two bits of swz (one at D = 64).
+  const uint32_t rpart = static_cast<uint32_t>(row0w % 16 + lrow) * slot_b;
+  const uint32_t cpart = 16u * static_cast<uint32_t>((lane % CPR) ^ swz(row0w + lrow));
+  constexpr int NH = IPW > IPH ? 2 : 1;  // halves a wave loads
+  const int ka0 = c * RB + 16 * (h ^ swz(c));  // K operand j at ka0 ^ 32 j of a slot
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  int vofs[NU];
+#pragma unroll
+  for (int x = 0; x < NU; ++x) {
+    const int jl = c & 15, rr = 4 * h + (jl >> 2), ch = 4 * x + 2 * (c >> 4) + ((jl & 3) >> 1);
+    vofs[x] = rr * RB + 16 * (ch ^ swz(rr)) + 8 * (jl & 1);
+  }
+
+  // The run's segments, one after the other: thread 0 keeps them in LDS (held in
+  // registers they cost the loop over blocks 160 spilled ones).
+  if (tid == 0) {
+    splits[run].runs = 0;
+    work->r = chunk_seq(a, st.s);
+    work->seg.s = st.s;
+    work->seg.kvh = st.kvh;
+    work->rb = st.rb;
+    const int64_t rest = total - static_cast<int64_t>(run) * per;
+    work->left = static_cast<int>(rest < per ? rest : per);
+    work->set(a, st.blk);
+    if (a.whole && st.blk > 0) work->next(a);  // (whole items: to the run that their first block is in)
+  }
+  __syncthreads();
+#pragma unroll 1
+  while (work->seg.blk1 > 0) {
+    auto of = [&](const int32_t& x) { return __builtin_amdgcn_readfirstlane(x); };
+    const ChunkSegment& seg = work->seg;
+    const ChunkArgs& g = chunk_args();
+    const int blk0 = of(seg.blk0), blk1 = of(seg.blk1), pos = of(seg.pos), end = of(seg.end);
+    const bool active = 32 * wave < of(seg.nq) * g.G;
+    // The lane's row, looked up where it is used: query and q-head, and the packed
+    // row of q/out. (Rows past the item's last: its query again, never stored.)
+    struct Row {
+      int q, head;
+      int64_t at;
+      bool ok;
+    };
+    auto my_row = [&](const ChunkArgs& x) __attribute__((always_inline)) {
+      int t = threadIdx.x;
+      asm volatile("" : "+v"(t));
+      const int rw = (t >> 6) * 32 + (t & 31), rq = (rw * x.g_mul) >> 16;
+      Row row;
+      row.q = min(rq, of(seg.nq) - 1);
+      row.head = of(seg.kvh) * x.G + rw - rq * x.G;
+      row.at = seg.row + row.q;
+      row.ok = rq < of(seg.nq);
+      return row;
+    };
+    {
+      u32x4 qop[KJ];
+      {
+        const Row row = my_row(g);
+        const T* const qp = static_cast<const T*>(g.q) + row.at * g.q_sr + row.head * g.q_sh + 8 * h;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) qop[j] = *reinterpret_cast<const u32x4*>(qp + 16 * j);
+      }
+      const char* const pool = k_wave ? static_cast<const char*>(g.kc) + of(seg.kvh) * g.kc_h * 2
+                                      : static_cast<const char*>(g.vc) + of(seg.kvh) * g.vc_h * 2;
+      float m = kNegInfC, l = 0.f;
+      f32x16 acc[NU];
+#pragma unroll
+      for (int x = 0; x < NU; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[x][e] = 0.f;
+      u32x4 kop[KJ];
+      auto kread = [&](int ks) __attribute__((always_inline)) {
+        int ka = ka0;
+        asm volatile("" : "+v"(ka));  // (its places are made here: eight of them held would spill)
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) kop[j] = *reinterpret_cast<const u32x4*>(smem + ks * BLKB + (ka ^ (32 * j)));
+      };
+      auto qk = [&](f32x16& sc) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) sc = mfma_k16x32<T>(kop[j], qop[j], sc);
+      };
+      auto block_max = [&](const f32x16& sc) __attribute__((always_inline)) {
+        float mx = kNegInfC;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * cs;
+      };
+      auto rescale = [&](float mt) __attribute__((always_inline)) {
+        // (A row's own scores alone move its maximum, so that what other rows of the
+        // wave see does not change its rounding.)
+        const bool up = mt > m + kChunkRescale;
+        if (__any(up)) {
+          const float mn = up ? mt : m, alpha = up ? fast_exp2(m - mn) : 1.f;
+          l *= alpha;
+#pragma unroll
+          for (int x = 0; x < NU; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[x][e] *= alpha;
+          m = mn;
+        }
+      };
+      u32x4 pop[2];
+      auto softmax_exp = [&](const f32x16& sc) __attribute__((always_inline)) {
+        const float mu = m == kNegInfC ? 0.f : m;
+        float p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          p[e] = fast_exp2(fmaf(sc[e], cs, -mu));
+          l += p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) pop[e >> 3][(e & 7) >> 1] = pack2<T>(p[e], p[e + 1]);
+      };
+      u32x4 vop[2][NU];  // V[keys of P's slots][dim 32 x + c]
+      auto vread = [&](int vs) __attribute__((always_inline)) {
+        int vofx[NU];  // (made here: held, they spill)
+#pragma unroll
+        for (int x = 0; x < NU; ++x) {
+          vofx[x] = vofs[x];
+          asm volatile("" : "+v"(vofx[x]));
+          vofx[x] ^= 32;
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int x = 0; x < NU; ++x) {
+            const int base = VOFF + vs * BLKB + 16 * s2 * RB;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(smem + base + vofs[x]));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(smem + base + 8 * RB + vofx[x]));
+            const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
+            vop[s2][x] = u32x4{lo2[0], lo2[1], hi2[0], hi2[1]};
+          }
+      };
+      auto pv = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int x = 0; x < NU; ++x) acc[x] = mfma_k16x32<T>(vop[s2][x], pop[s2], acc[x]);
+      };
+
+      // ---- The segment's blocks, kChunkTab at a time.
+#pragma unroll 1
+      for (int b0 = blk0; b0 < blk1; b0 += kChunkTab) {
+        const int n = min(blk1 - b0, kChunkTab);
+        if (tid == 0) *first_bad = n;
+        __syncthreads();
+        const ChunkArgs& f = chunk_args();
+        for (int i = tid; i < 2 * n; i += 64 * NW) {
+          const uint32_t tile = static_cast<uint32_t>(2 * b0 + i), lb = page_of_tile(tile, a.page_mul, a.page_shift);
+          const bool in = static_cast<int>(16u * tile) < end;
+          const int page = bt[of(seg.s) * f.bt_s0 + min(static_cast<int>(lb), f.max_blocks - 1) * f.bt_s1];
+          const bool ok = in && page >= 0 && page < f.NB;
+          tab[i] = ok ? page : -1;
+          if (!ok) atomicMin(first_bad, i >> 1);
+        }
+        __syncthreads();
+        // The first masked block: some row does not see it whole.
+        const int jm = min(__builtin_amdgcn_readfirstlane(*first_bad),
+                           max((min(pos + 1, end) >> 5) - b0, 0));
+        auto load_block = [&](int blk, int slot) __attribute__((always_inline)) {
+          const int j = min(blk, n - 1);
+          uint32_t lds0 = lds_w;
+          asm volatile("" : "+s"(lds0));  // (each load's place is added to it here: sixteen of them held would spill)
+          const char* base[NH];
+#pragma unroll
+          for (int y = 0; y < NH; ++y) {
+            const int half = row0w / 16 + y;
+            const int ent = __builtin_amdgcn_readfirstlane(tab[2 * j + half]);
+            const uint32_t tile = static_cast<uint32_t>(2 * (b0 + j) + half), lb = page_of_tile(tile, a.page_mul, a.page_shift);
+            const uint32_t page = ent < 0 ? 0u : static_cast<uint32_t>(ent);
+            const uint32_t slot0 = ent < 0 ? 0u : 16u * tile - lb * static_cast<uint32_t>(a.BS);
+            base[y] = pool + static_cast<uint64_t>(page) * page_b + slot0 * slot_b;
+          }
+#pragma unroll
+          for (int i = 0; i < IPW; ++i) {
+            uint32_t chunk = cpart;
+            asm volatile("" : "+v"(chunk));  // (and the lane's offsets are made here)
+            dma16_sv(base[NH == 1 ? 0 : i / IPH] + static_cast<uint32_t>((i % IPH) * RPI) * slot_b,
+                     rpart + (chunk ^ (D == 128 ? 16u * (i & 3) : 32u * (i & 1))), lds0 + slot * BLKB + i * 1024);
+          }
+        };
+        // Masked blocks: the keys that the lane's row sees, and those that are there
+        // at all.
+        uint32_t vis = ~0u, there = ~0u;
+        int sees = 0;  // (of masked blocks) keys that the lane's row sees
+        int hm = h;  // (h again: what is computed from it here stays here)
+        auto mask_block = [&](f32x16& sc, int j) __attribute__((always_inline)) {
+          auto below = [](int x) { return x >= 32 ? ~0u : x > 0 ? (1u << x) - 1u : 0u; };
+          const int k0 = 32 * (b0 + j);
+          const int e0 = __builtin_amdgcn_readfirstlane(tab[2 * j]), e1 = __builtin_amdgcn_readfirstlane(tab[2 * j + 1]);
+          there = below(end - k0) & ((e0 < 0 ? 0u : 0xFFFFu) | (e1 < 0 ? 0u : 0xFFFF0000u));
+          vis = below(sees - k0) & there;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (!((vis >> (8 * (e >> 2) + 4 * hm + (e & 3))) & 1)) sc[e] = kNegInfC;
+        };
+        auto fix_v = [&]() __attribute__((always_inline)) {
+          bool bad = false;
+#pragma unroll
+          for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int e = 8 * s2 + 2 * k;
+              const uint32_t b = there >> (8 * (e >> 2) + 4 * hm + (e & 3));
+              const uint32_t keep = (b & 1 ? 0xFFFFu : 0u) | (b & 2 ? 0xFFFF0000u : 0u);
+#pragma unroll
+              for (int x = 0; x < NU; ++x) {
+                vop[s2][x][k] &= keep;
+                bad |= nonfinite2<T>(vop[s2][x][k]) != 0;
+              }
+            }
+          if (!__any(bad)) return;
+          constexpr uint32_t one = std::is_same<T, bf16_t>::value ? 0x3F80u : 0x3C00u;
+          u32x4 see[2];
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const uint32_t b = vis >> (8 * (e >> 2) + 4 * hm + (e & 3));
+            see[e >> 3][(e & 7) >> 1] = (b & 1 ? one : 0u) | (b & 2 ? one << 16 : 0u);
+          }
+#pragma unroll
+          for (int x = 0; x < NU; ++x) {
+            f32x16 f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) f[e] = 0.f;
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+              u32x4 w;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t v = vop[s2][x][k], nf = nonfinite2<T>(v);
+                w[k] = flag16<T>(v & 0xFFFFu) | flag16<T>(v >> 16) << 16;
+                vop[s2][x][k] = v & (nf & 1 ? 0xFFFF0000u : ~0u) & (nf & 2 ? 0xFFFFu : ~0u);
+              }
+              f = mfma_k16x32<T>(w, see[s2], f);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[x][e] += flag_value(f[e]);
+          }
+        };
+        f32x16 sca, scb;  // S of the even / odd blocks
+        // One block that every row sees whole: on entry S(j) is in registers, K block
+        // j + 1 and V block j in their slots, and (PREV) block j - 1's P and V
+        // operands in registers.
+        auto full = [&](int j, auto S, auto prev) __attribute__((always_inline)) {
+          constexpr int s0 = decltype(S)::value;
+          f32x16& cur = (s0 & 1) ? scb : sca;
+          f32x16& nxt = (s0 & 1) ? sca : scb;
+          const bool issue = j < n - A;
+          if (issue) load_block(j + A + (k_wave ? 1 : 0), k_wave ? s0 : (s0 + NB - 1) % NB);
+          if (active) {
+            kread((s0 + 1) % NB);
+            if constexpr (decltype(prev)::value) pv();
+            const float mt = block_max(cur);
+            if constexpr (decltype(prev)::value) {
+#pragma unroll
+              for (int i = 0; i < 2 * NU; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+              }
+            }
+            rescale(mt);
+            qk(nxt);
+            softmax_exp(cur);
+            vread(s0);
+#pragma unroll
+            for (int jj = 0; jj < KJ; ++jj) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 56 / KJ, 0);
+              __builtin_amdgcn_sched_group_barrier(0x100, 4 * NU / KJ, 0);
+            }
+            asm volatile("" : "+v"(pop[0]), "+v"(pop[1]), "+v"(l));
+          }
+          if (issue) wait_vmcnt<kInFlight>();
+          else wait_vmcnt<0>();
+          lds_barrier();
+        };
+
+        using std::integral_constant;
+        if (k_wave) {
+          load_block(0, 0);
+#pragma unroll
+          for (int x = 0; x < A; ++x)
+            if (x < n) load_block(x + 1, x + 1);
+        } else {
+#pragma unroll
+          for (int x = 0; x < A; ++x)
+            if (x < n) load_block(x, x);
+        }
+        // K(0) and step 0. (Also the Q loads, which the compiler's own waits would
+        // otherwise put into the loop.)
+        if (n >= A) wait_vmcnt<kInFlight>();
+        else wait_vmcnt<0>();
+        lds_barrier();
+        // ---- The blocks before jm, in the pipeline.
+        const int n1 = min(n, jm);
+        if (n1 > 0) {
+          kread(0);
+          qk(sca);
+          lds_barrier();  // iteration 0's loads overwrite K(0)'s slot
+          full(0, integral_constant<int, 0>{}, std::false_type{});
+          for (int j = 1; j < n1;) {
+            full(j, integral_constant<int, 1>{}, std::true_type{});
+            if (++j == n1) break;
+            full(j, integral_constant<int, 2>{}, std::true_type{});
+            if (++j == n1) break;
+            full(j, integral_constant<int, 3>{}, std::true_type{});
+            if (++j == n1) break;
+            full(j, integral_constant<int, 0>{}, std::true_type{});
+            ++j;
+          }
+          if (active) pv();
+        }
+        // ---- The others, one at a time: masks and what they need stay out of the
+        // pipeline's registers.
+        if (n1 < n) sees = min(pos + my_row(chunk_args()).q + 1, end);
+#pragma unroll 1
+        for (int j = n1; j < n; ++j) {
+          if (active) kread(j % NB);
+          lds_barrier();  // step j + A overwrites K(j)'s slot and V(j - 1)'s
+          const bool issue = j < n - A;
+          if (issue) load_block(j + A + (k_wave ? 1 : 0), k_wave ? j % NB : (j + NB - 1) % NB);
+          if (active) {
+            asm volatile("" : "+v"(hm));
+            qk(sca);
+            mask_block(sca, j);
+            rescale(block_max(sca));
+            softmax_exp(sca);
+            vread(j % NB);
+            fix_v();
+            pv();
+          }
+          if (issue) wait_vmcnt<kInFlight>();
+          else wait_vmcnt<0>();
+          lds_barrier();
+        }
+      }
+      // ---- What the segment gives: the item's rows, or a partial result.
+      l += __builtin_bit_cast(float, xor_lane32<32>(__builtin_bit_cast(uint32_t, l), lane));
+      const ChunkArgs& o = chunk_args();
+      int he = h;
+      asm volatile("" : "+v"(he));
+      if (blk0 == 0 && blk1 == of(seg.nblk)) {
+        const Row row = my_row(o);
+        if (active && row.ok) {
+          T* const out = static_cast<T*>(o.out) + row.at * o.o_sr + row.head * o.o_sh;
+          const int64_t o_sd = o.o_sd;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+          for (int x = 0; x < NU; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const int d = 32 * x + 8 * (e >> 2) + 4 * he;
+              u32x2 w = {pack2<T>(acc[x][e] * inv, acc[x][e + 1] * inv), pack2<T>(acc[x][e + 2] * inv, acc[x][e + 3] * inv)};
+              if (l == 0.f) w = u32x2{0, 0};
+              if (o.out8) {
+                *reinterpret_cast<u32x2*>(out + d) = w;
+              } else {
+                uint16_t* const o16 = reinterpret_cast<uint16_t*>(out);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o16[(d + i) * o_sd] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+              }
+            }
+        }
+      } else {
+        // Slot 0: of the item that the run starts inside of; 1: of the one it starts.
+        float* const slot = part + (2 * static_cast<int64_t>(run) + (blk0 == 0 ? 1 : 0)) * chunk_part_floats<D, NW>();
+        if (active) {
+#pragma unroll
+          for (int x = 0; x < NU; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              *reinterpret_cast<f32x4*>(slot + 4 * ((wave * (4 * NU) + 4 * x + (e >> 2)) * 64 + lane)) =
+                  f32x4{acc[x][e], acc[x][e + 1], acc[x][e + 2], acc[x][e + 3]};
+          if (h == 0) *reinterpret_cast<f32x2*>(slot + 32 * NW * D + 2 * (32 * wave + c)) = f32x2{m, l};
+        }
+        if (blk0 > 0 && tid == 0) {
+          const int64_t item = static_cast<int64_t>(run) * per - blk0;  // (the run starts with this segment)
+          ChunkSplit sp;
+          sp.row0 = seg.row;
+          sp.kvh = seg.kvh;
+          sp.queries = seg.nq;
+          sp.runs = item >= static_cast<int64_t>(run - 1) * per
+                        ? static_cast<int>((item + seg.nblk - 1) / per) - run + 1 : 0;
+          splits[run] = sp;
+        }
+      }
+    }
+    __syncthreads();
+    if (tid == 0) work->next(chunk_args());
+    __syncthreads();
+  }
+}
+
+// Items that a cut goes through: the first run that starts inside of one puts its
+// partial results together, a wave's rows a workgroup.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(256) void paged_chunk_merge(ChunkArgs a, const int32_t* __restrict__ head,
+                                                         const ChunkSplit* __restrict__ splits,
+                                                         const float* __restrict__ part) {
+  constexpr int NU = D / 32;
+  const int run = static_cast<int>(blockIdx.x) + 1, wave = blockIdx.y;
+  if (run >= *head) return;
+  const ChunkSplit sp = splits[run];
+  if (sp.runs == 0 || 32 * wave >= sp.queries * a.G) return;
+  const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31, rw = 32 * wave + c, rq = rw / a.G;
+  float M = kNegInfC, den = 0.f;
+  f32x4 o[NU];
+#pragma unroll
+  for (int i = 0; i < NU; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k = -1; k < sp.runs; ++k) {
+    const float* const slot = part + (2 * static_cast<int64_t>(run + k) + (k < 0 ? 1 : 0)) * chunk_part_floats<D, NW>();
+    const f32x2 ml = *reinterpret_cast<const f32x2*>(slot + 32 * NW * D + 2 * rw);
+    f32x4 v[NU];
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+      v[i] = *reinterpret_cast<const f32x4*>(slot + 4 * ((wave * (4 * NU) + (threadIdx.x >> 6) + 4 * i) * 64 + lane));
+    const float mn = fmaxf(M, ml[0]), mu = mn == kNegInfC ? 0.f : mn;
+    const float c_old = fast_exp2(M - mu), c_new = fast_exp2(ml[0] - mu);
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[i][x] = fmaf(v[i][x], c_new, o[i][x] * c_old);
+    den = fmaf(ml[1], c_new, den * c_old);
+    M = mn;
+  }
+  if (rq >= sp.queries) return;
+  T* const out = static_cast<T*>(a.out) + (sp.row0 + rq) * a.o_sr + (sp.kvh * a.G + rw - rq * a.G) * a.o_sh;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+  for (int i = 0; i < NU; ++i) {
+    const int d = 32 * i + 8 * (threadIdx.x >> 6) + 4 * h;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) out[(d + x) * a.o_sd] = from_float<T>(den == 0.f ? 0.f : o[i][x] * inv);
+  }
+}
+
+}  // namespace tsa

@@ -53,12 +53,13 @@ constexpr float kNegInfR = -INFINITY;
 __host__ __device__ __forceinline__ uint32_t page_of_tile(uint32_t tile, uint32_t mul, uint32_t shift) {
   return static_cast<uint32_t>((static_cast<uint64_t>(tile) * mul) >> (23 + shift));
 }
-inline void set_page_div(RowsArgs& a) {
-  const uint64_t d = static_cast<uint64_t>(a.BS) / 16;
-  a.page_shift = 0;
-  while ((uint64_t{1} << a.page_shift) < d) ++a.page_shift;
-  a.page_mul = static_cast<uint32_t>(((uint64_t{1} << (23 + a.page_shift)) + d - 1) / d);
+inline void page_div(int64_t block_size, uint32_t& mul, uint32_t& shift) {
+  const uint64_t d = static_cast<uint64_t>(block_size) / 16;
+  shift = 0;
+  while ((uint64_t{1} << shift) < d) ++shift;
+  mul = static_cast<uint32_t>(((uint64_t{1} << (23 + shift)) + d - 1) / d);
 }
+inline void set_page_div(RowsArgs& a) { page_div(a.BS, a.page_mul, a.page_shift); }
 
 // A sequence's tokens: ctx of the cache's, then the drafted nodes at positions
 // ctx .. ctx + nodes - 1; end is past the last that its block table holds. rows
