@@ -42,8 +42,9 @@
 namespace tsa {
 
 constexpr int kChunkSlots = 4;       // K/V blocks in LDS
-constexpr int kChunkTab = 1024;      // 32-key blocks that the page table in LDS holds
+constexpr int kChunkTab = 480;       // 32-key blocks whose places the table in LDS holds
 constexpr float kChunkRescale = 8.f; // log2 units a maximum grows before it moves
+constexpr float kChunkNone = -3.402823466e38f;  // the maximum of no score: below every one but -inf, and its weights 0
 
 // ---- The plan on the device.
 // 32-key blocks of a sequence's row blocks 0 .. i - 1: sum of ceil(min(ctx + (k + 1)
@@ -214,7 +215,7 @@ __device__ __forceinline__ const ChunkArgs& chunk_args() {
   return *(const ChunkArgs*)p;
 }
 
-template <int D> constexpr int chunk_lds_bytes() { return 2 * kChunkSlots * 32 * 2 * D + kChunkTab * 8 + 16 + sizeof(ChunkWork); }
+template <int D> constexpr int chunk_lds_bytes() { return 2 * kChunkSlots * 32 * 2 * D + kChunkTab * 32 + 16 + sizeof(ChunkWork); }
 
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_stream(
@@ -228,8 +229,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   constexpr int VOFF = NB * BLKB, TOFF = 2 * NB * BLKB;
   constexpr int kInFlight = (A - 1) * IPW;
   __shared__ __align__(16) char smem[chunk_lds_bytes<D>()];
-  int32_t* const tab = reinterpret_cast<int32_t*>(smem + TOFF);  // page id of each half of the blocks, -1: none
-  int32_t* const first_bad = tab + 2 * kChunkTab;                // the first block with such a half
+  // For the halves (16 keys) of a segment's blocks, the byte offset of the first row
+  // in the K pool, then (kChunkTab blocks on) in the V pool; bit 63: no such page.
+  uint64_t* const tab = reinterpret_cast<uint64_t*>(smem + TOFF);
+  int32_t* const first_bad = reinterpret_cast<int32_t*>(tab + 4 * kChunkTab);  // the first block with such a half
   ChunkWork* const work = reinterpret_cast<ChunkWork*>(first_bad + 4);
 
   int64_t total;
@@ -255,7 +258,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   const uint32_t smem_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_void*)smem));
   const bool k_wave = wave < NW / 2;
   const int row0w = (wave % (NW / 2)) * IPW * RPI;
-  const uint32_t slot_b = static_cast<uint32_t>(k_wave ? a.kc_s : a.vc_s) * 2, page_b = k_wave ? a.k_page : a.v_page;
+  const uint32_t slot_b = static_cast<uint32_t>(k_wave ? a.kc_s : a.vc_s) * 2;
   const uint32_t lds_w = smem_lds + (k_wave ? 0 : VOFF) + row0w * RB;  // this wave's rows of slot 0
   const int lrow = lane / CPR;
   // The lane's place in instruction i: row r0w % 16 + i RPI + lrow of the half, chunk
@@ -321,18 +324,22 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       }
       const char* const pool = k_wave ? static_cast<const char*>(g.kc) + of(seg.kvh) * g.kc_h * 2
                                       : static_cast<const char*>(g.vc) + of(seg.kvh) * g.vc_h * 2;
-      float m = kNegInfC, l = 0.f;
+      float m = kChunkNone, l = 0.f;
       f32x16 acc[NU];
 #pragma unroll
       for (int x = 0; x < NU; ++x)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[x][e] = 0.f;
       u32x4 kop[KJ];
-      auto kread = [&](int ks) __attribute__((always_inline)) {
-        int ka = ka0;
-        asm volatile("" : "+v"(ka));  // (its places are made here: eight of them held would spill)
+      // (`it`, the loop's counter, keeps the operands' places from being computed once
+      // and held: they would spill.)
+      auto kread = [&](int ks, int it) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < KJ; ++j) kop[j] = *reinterpret_cast<const u32x4*>(smem + ks * BLKB + (ka ^ (32 * j)));
+        for (int j = 0; j < KJ; ++j) {
+          int ka = ka0;
+          if (j > 0) asm("v_xor_b32 %0, %1, %2" : "=v"(ka) : "n"(32 * j), "v"(ka0), "s"(it));
+          kop[j] = *reinterpret_cast<const u32x4*>(smem + ks * BLKB + ka);
+        }
       };
       auto qk = [&](f32x16& sc) __attribute__((always_inline)) {
 #pragma unroll
@@ -363,35 +370,30 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       };
       u32x4 pop[2];
       auto softmax_exp = [&](const f32x16& sc) __attribute__((always_inline)) {
-        const float mu = m == kNegInfC ? 0.f : m;
         float p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          p[e] = fast_exp2(fmaf(sc[e], cs, -mu));
+          p[e] = fast_exp2(fmaf(sc[e], cs, -m));
           l += p[e];
         }
 #pragma unroll
         for (int e = 0; e < 16; e += 2) pop[e >> 3][(e & 7) >> 1] = pack2<T>(p[e], p[e + 1]);
       };
       u32x4 vop[2][NU];  // V[keys of P's slots][dim 32 x + c]
-      auto vread = [&](int vs) __attribute__((always_inline)) {
-        int vofx[NU];  // (made here: held, they spill)
+      auto vread = [&](int vs, int it) __attribute__((always_inline)) {
 #pragma unroll
         for (int x = 0; x < NU; ++x) {
-          vofx[x] = vofs[x];
-          asm volatile("" : "+v"(vofx[x]));
-          vofx[x] ^= 32;
-        }
+          int vofx;  // (8 rows on)
+          asm("v_xor_b32 %0, 32, %1" : "=v"(vofx) : "v"(vofs[x]), "s"(it));
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-          for (int x = 0; x < NU; ++x) {
+          for (int s2 = 0; s2 < 2; ++s2) {
             const int base = VOFF + vs * BLKB + 16 * s2 * RB;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(smem + base + vofs[x]));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(smem + base + 8 * RB + vofx[x]));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(smem + base + 8 * RB + vofx));
             const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
             vop[s2][x] = u32x4{lo2[0], lo2[1], hi2[0], hi2[1]};
           }
+        }
       };
       auto pv = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -408,38 +410,50 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         __syncthreads();
         const ChunkArgs& f = chunk_args();
         for (int i = tid; i < 2 * n; i += 64 * NW) {
-          const uint32_t tile = static_cast<uint32_t>(2 * b0 + i), lb = page_of_tile(tile, a.page_mul, a.page_shift);
+          const uint32_t tile = static_cast<uint32_t>(2 * b0 + i), lb = page_of_tile(tile, f.page_mul, f.page_shift);
           const bool in = static_cast<int>(16u * tile) < end;
           const int page = bt[of(seg.s) * f.bt_s0 + min(static_cast<int>(lb), f.max_blocks - 1) * f.bt_s1];
           const bool ok = in && page >= 0 && page < f.NB;
-          tab[i] = ok ? page : -1;
+          const uint32_t slot0 = 16u * tile - lb * static_cast<uint32_t>(f.BS);
+          const uint64_t none = uint64_t{1} << 63;
+          tab[i] = ok ? static_cast<uint64_t>(page) * f.k_page + slot0 * static_cast<uint64_t>(2 * f.kc_s) : none;
+          tab[2 * kChunkTab + i] = ok ? static_cast<uint64_t>(page) * f.v_page + slot0 * static_cast<uint64_t>(2 * f.vc_s) : none;
           if (!ok) atomicMin(first_bad, i >> 1);
         }
         __syncthreads();
         // The first masked block: some row does not see it whole.
         const int jm = min(__builtin_amdgcn_readfirstlane(*first_bad),
                            max((min(pos + 1, end) >> 5) - b0, 0));
-        auto load_block = [&](int blk, int slot) __attribute__((always_inline)) {
+        // The wave's places of a block; the loads of one, and of the places of the one
+        // after it.
+        uint64_t at[NH];
+        const uint64_t* const my_tab = tab + (k_wave ? 0 : 2 * kChunkTab) + row0w / 16;
+        auto look_up = [&](int blk) __attribute__((always_inline)) {
           const int j = min(blk, n - 1);
+#pragma unroll
+          for (int y = 0; y < NH; ++y) at[y] = my_tab[2 * j + y];
+        };
+        auto load_block = [&](int blk, int slot) __attribute__((always_inline)) {
           uint32_t lds0 = lds_w;
-          asm volatile("" : "+s"(lds0));  // (each load's place is added to it here: sixteen of them held would spill)
+          asm("" : "+s"(lds0) : "s"(blk));  // (each load's place is added to it here: sixteen of them held would spill)
           const char* base[NH];
 #pragma unroll
           for (int y = 0; y < NH; ++y) {
-            const int half = row0w / 16 + y;
-            const int ent = __builtin_amdgcn_readfirstlane(tab[2 * j + half]);
-            const uint32_t tile = static_cast<uint32_t>(2 * (b0 + j) + half), lb = page_of_tile(tile, a.page_mul, a.page_shift);
-            const uint32_t page = ent < 0 ? 0u : static_cast<uint32_t>(ent);
-            const uint32_t slot0 = ent < 0 ? 0u : 16u * tile - lb * static_cast<uint32_t>(a.BS);
-            base[y] = pool + static_cast<uint64_t>(page) * page_b + slot0 * slot_b;
+            const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at[y]));
+            const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at[y] >> 32)) & 0x7FFFFFFFu;
+            base[y] = pool + ((static_cast<uint64_t>(hi) << 32) | lo);
           }
 #pragma unroll
           for (int i = 0; i < IPW; ++i) {
-            uint32_t chunk = cpart;
-            asm volatile("" : "+v"(chunk));  // (and the lane's offsets are made here)
-            dma16_sv(base[NH == 1 ? 0 : i / IPH] + static_cast<uint32_t>((i % IPH) * RPI) * slot_b,
-                     rpart + (chunk ^ (D == 128 ? 16u * (i & 3) : 32u * (i & 1))), lds0 + slot * BLKB + i * 1024);
+            // (rpart + (cpart ^ bits of i), made here)
+            uint32_t off;
+            constexpr uint32_t kBits = D == 128 ? 16u : 32u;
+            const uint32_t x = kBits * (D == 128 ? i & 3 : i & 1);
+            asm("v_xad_u32 %0, %1, %2, %3" : "=v"(off) : "v"(cpart), "n"(x), "v"(rpart), "s"(blk));
+            dma16_sv(base[NH == 1 ? 0 : i / IPH] + static_cast<uint32_t>((i % IPH) * RPI) * slot_b, off,
+                     lds0 + slot * BLKB + i * 1024);
           }
+          look_up(blk + 1);
         };
         // Masked blocks: the keys that the lane's row sees, and those that are there
         // at all.
@@ -449,7 +463,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         auto mask_block = [&](f32x16& sc, int j) __attribute__((always_inline)) {
           auto below = [](int x) { return x >= 32 ? ~0u : x > 0 ? (1u << x) - 1u : 0u; };
           const int k0 = 32 * (b0 + j);
-          const int e0 = __builtin_amdgcn_readfirstlane(tab[2 * j]), e1 = __builtin_amdgcn_readfirstlane(tab[2 * j + 1]);
+          const int e0 = __builtin_amdgcn_readfirstlane(static_cast<int>(tab[2 * j] >> 32));
+          const int e1 = __builtin_amdgcn_readfirstlane(static_cast<int>(tab[2 * j + 1] >> 32));
           there = below(end - k0) & ((e0 < 0 ? 0u : 0xFFFFu) | (e1 < 0 ? 0u : 0xFFFF0000u));
           vis = below(sees - k0) & there;
 #pragma unroll
@@ -510,7 +525,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           const bool issue = j < n - A;
           if (issue) load_block(j + A + (k_wave ? 1 : 0), k_wave ? s0 : (s0 + NB - 1) % NB);
           if (active) {
-            kread((s0 + 1) % NB);
+            kread((s0 + 1) % NB, j);
             if constexpr (decltype(prev)::value) pv();
             const float mt = block_max(cur);
             if constexpr (decltype(prev)::value) {
@@ -523,7 +538,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             rescale(mt);
             qk(nxt);
             softmax_exp(cur);
-            vread(s0);
+            vread(s0, j);
 #pragma unroll
             for (int jj = 0; jj < KJ; ++jj) {
               __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -538,6 +553,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         };
 
         using std::integral_constant;
+        look_up(0);
         if (k_wave) {
           load_block(0, 0);
 #pragma unroll
@@ -556,7 +572,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         // ---- The blocks before jm, in the pipeline.
         const int n1 = min(n, jm);
         if (n1 > 0) {
-          kread(0);
+          kread(0, b0);
           qk(sca);
           lds_barrier();  // iteration 0's loads overwrite K(0)'s slot
           full(0, integral_constant<int, 0>{}, std::false_type{});
@@ -577,7 +593,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         if (n1 < n) sees = min(pos + my_row(chunk_args()).q + 1, end);
 #pragma unroll 1
         for (int j = n1; j < n; ++j) {
-          if (active) kread(j % NB);
+          if (active) kread(j % NB, j);
           lds_barrier();  // step j + A overwrites K(j)'s slot and V(j - 1)'s
           const bool issue = j < n - A;
           if (issue) load_block(j + A + (k_wave ? 1 : 0), k_wave ? j % NB : (j + NB - 1) % NB);
@@ -587,7 +603,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             mask_block(sca, j);
             rescale(block_max(sca));
             softmax_exp(sca);
-            vread(j % NB);
+            vread(j % NB, j);
             fix_v();
             pv();
           }
@@ -626,7 +642,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       } else {
         // Slot 0: of the item that the run starts inside of; 1: of the one it starts.
         float* const slot = part + (2 * static_cast<int64_t>(run) + (blk0 == 0 ? 1 : 0)) * chunk_part_floats<D, NW>();
-        if (active) {
+        if (active && my_row(o).ok) {
 #pragma unroll
           for (int x = 0; x < NU; ++x)
 #pragma unroll
@@ -664,8 +680,9 @@ __global__ __launch_bounds__(256) void paged_chunk_merge(ChunkArgs a, const int3
   if (run >= *head) return;
   const ChunkSplit sp = splits[run];
   if (sp.runs == 0 || 32 * wave >= sp.queries * a.G) return;
-  const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31, rw = 32 * wave + c, rq = rw / a.G;
-  float M = kNegInfC, den = 0.f;
+  const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31, rw = 32 * wave + c, rq = (rw * a.g_mul) >> 16;
+  if (rq >= sp.queries) return;
+  float M = kChunkNone, den = 0.f;
   f32x4 o[NU];
 #pragma unroll
   for (int i = 0; i < NU; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -676,8 +693,7 @@ __global__ __launch_bounds__(256) void paged_chunk_merge(ChunkArgs a, const int3
 #pragma unroll
     for (int i = 0; i < NU; ++i)
       v[i] = *reinterpret_cast<const f32x4*>(slot + 4 * ((wave * (4 * NU) + (threadIdx.x >> 6) + 4 * i) * 64 + lane));
-    const float mn = fmaxf(M, ml[0]), mu = mn == kNegInfC ? 0.f : mn;
-    const float c_old = fast_exp2(M - mu), c_new = fast_exp2(ml[0] - mu);
+    const float mn = fmaxf(M, ml[0]), c_old = fast_exp2(M - mn), c_new = fast_exp2(ml[0] - mn);
 #pragma unroll
     for (int i = 0; i < NU; ++i)
 #pragma unroll
@@ -685,14 +701,20 @@ __global__ __launch_bounds__(256) void paged_chunk_merge(ChunkArgs a, const int3
     den = fmaf(ml[1], c_new, den * c_old);
     M = mn;
   }
-  if (rq >= sp.queries) return;
   T* const out = static_cast<T*>(a.out) + (sp.row0 + rq) * a.o_sr + (sp.kvh * a.G + rw - rq * a.G) * a.o_sh;
   const float inv = den == 0.f ? 0.f : 1.f / den;
 #pragma unroll
   for (int i = 0; i < NU; ++i) {
     const int d = 32 * i + 8 * (threadIdx.x >> 6) + 4 * h;
+    u32x2 w = {pack2<T>(o[i][0] * inv, o[i][1] * inv), pack2<T>(o[i][2] * inv, o[i][3] * inv)};
+    if (den == 0.f) w = u32x2{0, 0};
+    if (a.out8) {
+      *reinterpret_cast<u32x2*>(out + d) = w;
+    } else {
+      uint16_t* const o16 = reinterpret_cast<uint16_t*>(out);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) out[(d + x) * a.o_sd] = from_float<T>(den == 0.f ? 0.f : o[i][x] * inv);
+      for (int x = 0; x < 4; ++x) o16[(d + x) * a.o_sd] = static_cast<uint16_t>(w[x >> 1] >> (16 * (x & 1)));
+    }
   }
 }
 
