@@ -8,6 +8,10 @@
 // adds nothing; a NaN, a +inf or a row of nothing but -inf makes S NaN, and with it
 // the row's results.
 //
+// One read of the logits; what bounds it: HBM for many rows (a large copy's rate), and
+// for a few the chain load -> sums -> threshold -> candidates -> rank. The vector
+// units come next: 7.5 operations and an exponential a logit.
+//
 // Order of the alternatives: by value, the lowest index first where values tie (0 and
 // -0 do), NaN last. One whole number a logit has that order (rank_of), and no two of a
 // row are alike.
@@ -25,10 +29,12 @@ struct LogprobArgs {
   int64_t lp_s, en_s, tl_s0, tl_s1, tt_s0, tt_s1, x_s0, x_s1, tok_s;
   int64_t N;
   int32_t V, top;
+  int32_t segments, tiles;  // of a row; tiles of a segment
   bool tok64;
 };
 
 constexpr int kMaxTop = 64;
+constexpr int kThreads = 256;
 
 __device__ __forceinline__ uint64_t rank_of(float x, uint32_t i) {
   uint32_t b = __float_as_uint(x + 0.f);
@@ -42,8 +48,433 @@ __device__ __forceinline__ int64_t token_of(const LogprobArgs& a, int64_t row) {
   return a.tok64 ? static_cast<const int64_t*>(a.tokens)[row * a.tok_s] : static_cast<const int32_t*>(a.tokens)[row * a.tok_s];
 }
 
-// Any strides: a workgroup a row, the row read for the maximum, the sums and each
-// alternative.
+// What sorts in the other order than its bits: rank_of's value.
+__device__ __forceinline__ float value_of(uint64_t rank) {
+  uint32_t b = static_cast<uint32_t>(rank >> 32);
+  if (b == 0) return __builtin_nanf("");
+  return __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b);
+}
+
+// The k-th largest (k from 1) of the wave's 64 numbers: a bitonic sort over the
+// lanes, the largest in lane 0.
+template <int J>
+__device__ __forceinline__ void sort_step(uint64_t& x, int lane, bool down) {
+  const uint64_t o = xor_lane64<J>(x, lane);
+  x = ((lane & J) == 0) == down ? (o > x ? o : x) : (o < x ? o : x);
+}
+__device__ __forceinline__ uint64_t wave_kth(uint64_t x, int k, int lane) {
+  sort_step<1>(x, lane, !(lane & 2));
+  sort_step<2>(x, lane, !(lane & 4)); sort_step<1>(x, lane, !(lane & 4));
+  sort_step<4>(x, lane, !(lane & 8)); sort_step<2>(x, lane, !(lane & 8)); sort_step<1>(x, lane, !(lane & 8));
+  sort_step<8>(x, lane, !(lane & 16)); sort_step<4>(x, lane, !(lane & 16)); sort_step<2>(x, lane, !(lane & 16));
+  sort_step<1>(x, lane, !(lane & 16));
+  sort_step<16>(x, lane, !(lane & 32)); sort_step<8>(x, lane, !(lane & 32)); sort_step<4>(x, lane, !(lane & 32));
+  sort_step<2>(x, lane, !(lane & 32)); sort_step<1>(x, lane, !(lane & 32));
+  sort_step<32>(x, lane, true); sort_step<16>(x, lane, true); sort_step<8>(x, lane, true);
+  sort_step<4>(x, lane, true); sort_step<2>(x, lane, true); sort_step<1>(x, lane, true);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), k - 1);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), k - 1);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
+// The candidates of a row, in LDS.
+constexpr int kCand = 1024;
+struct Candidates {
+  uint64_t list[kCand];
+  uint64_t fours[64];  // the largest of four lanes
+  int count, reach;
+};
+// The k-th largest of the 64 groups' largest, where each thread gives the largest of
+// its part: at least k of all the numbers reach it. All threads call.
+__device__ __forceinline__ uint64_t group_kth(Candidates& c, uint64_t mine, int k) {
+  const int lane = threadIdx.x & 63;
+  uint64_t o = xor_lane64<1>(mine, lane);
+  mine = o > mine ? o : mine;
+  o = xor_lane64<2>(mine, lane);
+  mine = o > mine ? o : mine;
+  __syncthreads();
+  if ((lane & 3) == 0) c.fours[threadIdx.x >> 2] = mine;
+  __syncthreads();
+  return wave_kth(c.fours[lane], k, lane);
+}
+// Leaves out candidates that k others are larger than, while more than `most` are left
+// (no two are alike, so each round leaves out one at least). All threads call.
+__device__ __forceinline__ uint64_t prune(Candidates& c, int k, int most, uint64_t floor) {
+  constexpr int kPer = kCand / kThreads;
+  while (true) {
+    __syncthreads();
+    const int n = c.count;
+    if (n <= most) return floor;
+    uint64_t x[kPer], top = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int at = static_cast<int>(threadIdx.x) + i * kThreads;
+      x[i] = at < n ? c.list[at] : 0;
+      top = x[i] > top ? x[i] : top;
+    }
+    const uint64_t t = group_kth(c, top, k);
+    floor = t > floor ? t : floor;
+    __syncthreads();
+    if (threadIdx.x == 0) c.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (x[i] != 0 && x[i] >= floor) c.list[atomicAdd(&c.count, 1)] = x[i];
+  }
+}
+// The k largest candidates in order, write(place, number); places past the last
+// candidate get 0.
+template <typename F>
+__device__ __forceinline__ void write_top(Candidates& c, int k, F write) {
+  prune(c, k, kThreads, 0);
+  __syncthreads();
+  const int n = c.count, tid = threadIdx.x;
+  if (tid < n) {
+    const uint64_t x = c.list[tid];
+    int place = 0;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) place += c.list[i] > x;
+    if (place < k) write(place, x);
+  }
+  if (tid >= n && tid < k) write(tid, uint64_t{0});
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kNoMax = -3.402823466e38f;  // the reference of no logit
+constexpr float kMove = 16.f;               // a logit may pass the reference by so much
+
+// Sums over logits x, relative to a reference m that is within kMove below the
+// largest: s = sum 2^y, e = sum 2^y y, y = (x - m) log2 e.
+struct Sums {
+  float m, s, e;
+  __device__ __forceinline__ void move(float to) {
+    const float d = fmaxf((m - to) * kLog2e, -1e30f), f = fast_exp2(d);
+    e = f * fmaf(d, s, e);
+    s *= f;
+    m = to;
+  }
+  // (a logit of -inf adds 0; a NaN, or an infinity's inf - inf, makes s NaN)
+  __device__ __forceinline__ void add(float x) {
+    const float y = (x - m) * kLog2e, p = fast_exp2(y);
+    s += p;
+    e = fmaf(p, fmaxf(y, -1e30f), e);
+  }
+  __device__ __forceinline__ void join(const Sums& o) {
+    Sums b = o;
+    const float to = fmaxf(m, o.m);
+    move(to);
+    b.move(to);
+    s += b.s;
+    e += b.e;
+  }
+};
+__device__ __forceinline__ Sums block_sums(Sums v, Sums* waves) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    Sums o;
+    o.m = __shfl_xor(v.m, off, 64);
+    o.s = __shfl_xor(v.s, off, 64);
+    o.e = __shfl_xor(v.e, off, 64);
+    v.join(o);
+  }
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = waves[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 64; ++w) v.join(waves[w]);
+  return v;
+}
+
+// A row's results from its sums and the candidates of its largest logits.
+template <typename T>
+__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, Sums v, Candidates& c) {
+  const float s = v.s == 0.f ? __builtin_nanf("") : v.s, lse = logf(s);  // (nothing but -inf: no distribution)
+  if (threadIdx.x == 0) {
+    const int64_t t = token_of(a, row);
+    const float x = t >= 0 && t < a.V ? to_float(static_cast<const T*>(a.x)[row * a.x_s0 + t * a.x_s1]) : -INFINITY;
+    a.logp[row * a.lp_s] = (x - v.m) - lse;
+    a.entropy[row * a.en_s] = lse - kLn2 * (v.e / s);
+  }
+  if (a.top > 0)
+    write_top(c, a.top, [&](int place, uint64_t rank) {
+      a.top_tok[row * a.tt_s0 + place * a.tt_s1] = index_of(rank);
+      a.top_logp[row * a.tl_s0 + place * a.tl_s1] = (value_of(rank) - v.m) - lse;
+    });
+}
+
+// 16 bytes of logits.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+  static constexpr int n = 4;
+  static constexpr uint32_t none = 0xFF800000u;
+  static __device__ __forceinline__ float at(const u32x4& v, int i) { return __uint_as_float(v[i]); }
+};
+template <> struct Piece<bf16_t> {
+  static constexpr int n = 8;
+  static constexpr uint32_t none = 0xFF80FF80u;
+  static __device__ __forceinline__ float at(const u32x4& v, int i) { return i & 1 ? hi_f<bf16_t>(v[i >> 1]) : lo_f<bf16_t>(v[i >> 1]); }
+};
+template <> struct Piece<f16_t> {
+  static constexpr int n = 8;
+  static constexpr uint32_t none = 0xFC00FC00u;
+  static __device__ __forceinline__ float at(const u32x4& v, int i) { return i & 1 ? hi_f<f16_t>(v[i >> 1]) : lo_f<f16_t>(v[i >> 1]); }
+};
+
+constexpr int kUnroll = 8;   // pieces of a thread in flight: a tile is 256 x 8 pieces
+constexpr int kGroups = 12;  // runs of tiles of which each thread keeps its largest logit
+constexpr int kTilePieces = kThreads * kUnroll;
+
+// What a row's segment leaves for the second launch: its sums, then its k largest.
+__host__ __device__ constexpr int part_words(int top) { return 4 + 2 * top; }
+
+// A workgroup a segment of a row (a.tiles tiles of 256 x 8 pieces of 16 bytes; a row
+// is cut where there are few). The logits before the first 16-byte boundary and behind
+// the last one are the first and the last segment's, one a thread.
+//
+// The loop only sums, and keeps each thread's largest logit of each group of tiles.
+// Then the top-th largest of 64 groups' largest is a threshold that at least `top`
+// logits reach and few others (about 24 for 20 where their places are random), and
+// threads with a group that reaches it read that again. More than kCand of them: those
+// above the threshold and the lowest of those that tie with it, or else all of them a
+// wave's piece at a time, under a floor that rises.
+template <typename T, bool SPLIT>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6))) void token_logprobs_stream(LogprobArgs a, float* __restrict__ part) {
+  typedef Piece<T> PT;
+  constexpr int VE = PT::n;
+  __shared__ Candidates c;
+  __shared__ float group_max[kGroups][kThreads];
+  __shared__ Sums waves[kThreads / 64];
+  const int tid = threadIdx.x;
+  const int64_t items = a.N * a.segments;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = item / a.segments;
+    const int seg = static_cast<int>(item - row * a.segments);
+    const T* const x = static_cast<const T*>(a.x) + row * a.x_s0;
+    const int head = min(a.V, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
+    const int pieces = (a.V - head) / VE, tail = a.V - head - pieces * VE;
+    const T* const body = x + head;
+    const int t0 = seg * a.tiles, t1 = min(t0 + a.tiles, (pieces + kTilePieces - 1) / kTilePieces);
+    const int per_group = (a.tiles + kGroups - 1) / kGroups;
+
+    Sums v{kNoMax, 0.f, 0.f};
+    float largest = -INFINITY;
+    // A tile's pieces of this thread; those past the row's are none.
+    auto load = [&](int t, u32x4 (&w)[kUnroll]) __attribute__((always_inline)) {
+      const int p0 = t * kTilePieces + tid;
+      if ((t + 1) * kTilePieces <= pieces) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          w[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(body) + p0 + u * kThreads);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          const int p = p0 + u * kThreads;
+          w[u] = u32x4{PT::none, PT::none, PT::none, PT::none};
+          if (p < pieces) w[u] = reinterpret_cast<const u32x4*>(body)[p];
+        }
+      }
+    };
+    for (int g = 0, t = t0; t < t1; ++g) {
+      float gm = -INFINITY;
+      for (const int end = min(t + per_group, t1); t < end; ++t) {
+        u32x4 w[kUnroll];
+        load(t, w);
+        // (a piece at a time: its logits as floats, a few registers, serve both loops)
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < VE; i += 2) mx = fmaxf(fmaxf(mx, PT::at(w[u], i)), PT::at(w[u], i + 1));
+          if (mx > v.m + kMove) v.move(mx);
+          gm = fmaxf(gm, mx);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) v.add(PT::at(w[u], i));
+        }
+      }
+      group_max[g][tid] = gm;
+      largest = fmaxf(largest, gm);
+    }
+    // The edges: thread i has logit i, thread 32 + i the i-th behind the pieces.
+    const bool has_head = seg == 0 && tid < head;
+    const bool has_tail = seg == a.segments - 1 && tid >= 32 && tid - 32 < tail;
+    const int edge = has_head ? tid : a.V - tail + tid - 32;
+    float at_edge = -INFINITY;
+    if (has_head || has_tail) {
+      at_edge = to_float(x[edge]);
+      if (at_edge > v.m + kMove) v.move(at_edge);
+      v.add(at_edge);
+      largest = fmaxf(largest, at_edge);
+    }
+
+    if (a.top > 0) {
+      const uint64_t t = group_kth(c, rank_of(largest, 0xFFFFFFFFu), a.top);
+      const float threshold = value_of(t);
+      auto append = [&](uint64_t r) __attribute__((always_inline)) {
+        const int at = atomicAdd(&c.count, 1);
+        if (at < kCand) c.list[at] = r;
+      };
+      // The logits that reach the threshold, from the groups that do (whole pieces at
+      // once); `above`: those past it. False: there are too many.
+      const int groups = t1 > t0 ? (t1 - t0 + per_group - 1) / per_group : 0;
+      // (of 64 groups, about -64 ln(1 - top / 64) threads' groups reach it; all do where it is a mask's value)
+      const int here = (min(t1 * kTilePieces, pieces) - t0 * kTilePieces) * VE;
+      const int most = here <= kCand ? groups * kThreads : min(8 * a.top + 64, groups * kThreads - 1);
+      auto gather = [&](bool above) {
+        auto in = [&](float xi) { return above ? xi > threshold : !(xi < threshold); };  // (a NaN reaches any, and passes none)
+        __syncthreads();
+        if (tid == 0) c.count = c.reach = 0;
+        __syncthreads();
+        int reach = 0;
+        for (int g = 0; g < groups; ++g) reach += in(group_max[g][tid]);
+        if (reach) atomicAdd(&c.reach, reach);
+        __syncthreads();
+        if (c.reach > most) return false;
+        if ((has_head || has_tail) && in(at_edge)) append(rank_of(at_edge, edge));
+#pragma unroll 1
+        for (int g = 0; g < groups; ++g) {
+          if (!in(group_max[g][tid])) continue;
+#pragma unroll 1
+          for (int y = t0 + g * per_group, end = min(y + per_group, t1); y < end; ++y) {
+            u32x4 w[kUnroll];
+            load(y, w);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+              const int p = y * kTilePieces + u * kThreads + tid;
+              uint32_t high = 0;
+#pragma unroll
+              for (int i = 0; i < VE; ++i) high |= (in(PT::at(w[u], i)) ? 1u : 0u) << i;
+              if (p >= pieces) high = 0;
+              for (; high; high &= high - 1) {
+                const int i = __builtin_ctz(high);
+                append(rank_of(to_float(body[p * VE + i]), head + p * VE + i));
+              }
+            }
+          }
+        }
+        __syncthreads();
+        return c.count <= kCand;
+      };
+      bool done = gather(false);
+      if (!done && gather(true)) {
+        // Many tie at the threshold (a mask's value, with fewer tokens allowed than
+        // asked for): those of them among the segment's first logits are the lowest.
+        const int i = (seg == 0 ? 0 : head + t0 * kTilePieces * VE) + tid;
+        const int end = seg == a.segments - 1 ? a.V : head + min(t1 * kTilePieces, pieces) * VE;
+        if (tid < 2 * a.top + 16 && i < end && to_float(x[i]) == threshold) append(rank_of(threshold, i));
+        __syncthreads();
+        done = c.count >= a.top && c.count <= kCand;
+      }
+      if (!done) {
+        // Again, a wave's piece at a time, leaving out what a rising floor allows.
+        uint64_t floor = 0;
+        __syncthreads();
+        if (tid == 0) c.count = 0;
+        __syncthreads();
+        if (has_head || has_tail) append(rank_of(at_edge, edge));
+#pragma unroll 1
+        for (int y = t0; y < t1; ++y) {
+          // (the largest that this thread's logits of the tile can be)
+          const float gm = group_max[(y - t0) / per_group][tid];
+          const bool may = floor == 0 || rank_of(gm, head + y * kTilePieces * VE) > floor;
+          if (!__syncthreads_or(may)) continue;
+#pragma unroll 1
+          for (int i = 0; i < kUnroll * (kThreads / 64); ++i) {
+            const int p = y * kTilePieces + (i >> 2) * kThreads + tid;
+            floor = prune(c, a.top, kCand - 64 * VE, floor);
+            if (may && tid >> 6 == (i & 3) && p < pieces) {
+#pragma unroll 1
+              for (int e = 0; e < VE; ++e) {
+                const uint64_t r = rank_of(to_float(body[p * VE + e]), head + p * VE + e);
+                if (r > floor) append(r);
+              }
+            }
+          }
+        }
+        __syncthreads();
+      }
+    }
+    v = block_sums(v, waves);
+    if constexpr (SPLIT) {
+      float* const out = part + item * part_words(a.top);
+      if (tid == 0) {
+        out[0] = v.m;
+        out[1] = v.s;
+        out[2] = v.e;
+      }
+      if (a.top > 0) write_top(c, a.top, [&](int place, uint64_t rank) { reinterpret_cast<uint64_t*>(out + 4)[place] = rank; });
+    } else {
+      write_row<T>(a, row, v, c);
+    }
+    __syncthreads();
+  }
+}
+
+// The second launch of rows that were cut: a workgroup a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void token_logprobs_join(LogprobArgs a, const float* __restrict__ part) {
+  __shared__ Candidates c;
+  __shared__ Sums waves[kThreads / 64];
+  const int tid = threadIdx.x;
+  for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+    const float* const mine = part + row * a.segments * part_words(a.top);
+    Sums v{kNoMax, 0.f, 0.f};
+    if (tid < a.segments) {
+      const float* const p = mine + tid * part_words(a.top);
+      v = Sums{p[0], p[1], p[2]};
+    }
+    if (tid == 0) c.count = 0;
+    __syncthreads();
+    for (int i = tid; i < a.segments * a.top; i += kThreads) {
+      const int sg = i / a.top;
+      const uint64_t r = reinterpret_cast<const uint64_t*>(mine + sg * part_words(a.top) + 4)[i - sg * a.top];
+      if (r != 0) c.list[atomicAdd(&c.count, 1)] = r;
+    }
+    v = block_sums(v, waves);
+    write_row<T>(a, row, v, c);
+    __syncthreads();
+  }
+}
+
+// Rows are cut until there are kWorkgroups, at tiles and at most as the second
+// launch's candidates allow.
+constexpr int64_t kWorkgroups = 1024;
+struct RowCut {
+  int segments, tiles;
+};
+static RowCut cut_rows(int64_t N, int64_t V, int64_t top, int elem_bytes) {
+  const int64_t pieces = V * elem_bytes / 16, tiles = (pieces + kTilePieces - 1) / kTilePieces;
+  int64_t s = N < 512 ? (kWorkgroups + N - 1) / N : 1;
+  if (s > tiles) s = tiles;
+  const int64_t most = top > 0 ? kCand / top : kThreads;
+  if (s > most) s = most;
+  if (s > kThreads) s = kThreads;
+  if (s < 1) s = 1;
+  const int64_t per = (tiles + s - 1) / s > 1 ? (tiles + s - 1) / s : 1;
+  return RowCut{static_cast<int>(tiles > 0 ? (tiles + per - 1) / per : 1), static_cast<int>(per)};
+}
+static size_t cut_bytes(int64_t N, const RowCut& r, int64_t top) {
+  return r.segments > 1 ? sizeof(float) * static_cast<size_t>(N) * r.segments * part_words(static_cast<int>(top)) : 0;
+}
+
+template <typename T>
+static int launch_stream(LogprobArgs& a, const RowCut& r, void* workspace, hipStream_t stream) {
+  a.segments = r.segments;
+  a.tiles = r.tiles;
+  const int64_t items = a.N * a.segments;
+  const dim3 grid(static_cast<uint32_t>(items < (1 << 22) ? items : 1 << 22)), rows(static_cast<uint32_t>(a.N < (1 << 22) ? a.N : 1 << 22));
+  float* const part = static_cast<float*>(workspace);
+  if (r.segments == 1) {
+    token_logprobs_stream<T, false><<<grid, dim3(kThreads), 0, stream>>>(a, nullptr);
+    return check_launch("tsa_token_logprobs");
+  }
+  token_logprobs_stream<T, true><<<grid, dim3(kThreads), 0, stream>>>(a, part);
+  if (int rc = check_launch("tsa_token_logprobs")) return rc;
+  token_logprobs_join<T><<<rows, dim3(kThreads), 0, stream>>>(a, part);
+  return check_launch("tsa_token_logprobs");
+}
+
+// Logits that do not lie side by side: a workgroup a row, the row read for the maximum,
+// the sums and each alternative.
 template <typename T>
 __global__ __launch_bounds__(256) void token_logprobs_rows(LogprobArgs a) {
   __shared__ uint64_t best[4];
@@ -148,9 +579,20 @@ extern "C" int tsa_token_logprobs(const tsa_view* logprobs, const tsa_view* entr
   a.tok_s = tokens->stride[0];
   a.N = N; a.V = static_cast<int32_t>(V); a.top = static_cast<int32_t>(top);
   a.tok64 = tokens->dtype == TSA_I64;
-  (void)workspace;
-  (void)workspace_bytes;
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a.x_s1 == 1 || V == 1) {
+    a.x_s1 = 1;
+    const RowCut r = cut_rows(N, V, top, dtype_bytes(logits->dtype));
+    const size_t need = cut_bytes(N, r, top);
+    TSA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need),
+                "workspace of %zu bytes is too small: %zu needed", workspace_bytes, need);
+    TSA_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
+    switch (logits->dtype) {
+      case TSA_BF16: return launch_stream<bf16_t>(a, r, workspace, st);
+      case TSA_F16: return launch_stream<f16_t>(a, r, workspace, st);
+      default: return launch_stream<float>(a, r, workspace, st);
+    }
+  }
   switch (logits->dtype) {
     case TSA_BF16: return launch_rows<bf16_t>(a, st);
     case TSA_F16: return launch_rows<f16_t>(a, st);
@@ -158,4 +600,13 @@ extern "C" int tsa_token_logprobs(const tsa_view* logprobs, const tsa_view* entr
   }
 }
 
-extern "C" size_t tsa_token_logprobs_workspace_bytes(int64_t, int64_t, int64_t) { return 0; }
+extern "C" size_t tsa_token_logprobs_workspace_bytes(int64_t num_tokens, int64_t vocab_size, int64_t num_top) {
+  if (num_tokens <= 0 || vocab_size <= 0 || vocab_size >= (int64_t{1} << 30) || num_top < 0 || num_top > kMaxTop)
+    return 0;  // (calls of such sizes are refused, or have nothing to do)
+  size_t most = 0;
+  for (const int bytes : {2, 4}) {
+    const size_t n = cut_bytes(num_tokens, cut_rows(num_tokens, vocab_size, num_top, bytes), num_top);
+    most = n > most ? n : most;
+  }
+  return most;
+}
