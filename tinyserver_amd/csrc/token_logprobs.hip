@@ -29,12 +29,13 @@ struct LogprobArgs {
   int64_t lp_s, en_s, tl_s0, tl_s1, tt_s0, tt_s1, x_s0, x_s1, tok_s;
   int64_t N;
   int32_t V, top;
-  int32_t segments, tiles;  // of a row; tiles of a segment
+  int32_t per_group, parts;  // tiles of a group; parts that rows are cut into
   bool tok64;
 };
 
 constexpr int kMaxTop = 64;
 constexpr int kThreads = 256;
+constexpr int64_t kWholeRows = 512;  // rows of a call from which on none is cut
 
 __device__ __forceinline__ uint64_t rank_of(float x, uint32_t i) {
   uint32_t b = __float_as_uint(x + 0.f);
@@ -78,11 +79,12 @@ __device__ __forceinline__ uint64_t wave_kth(uint64_t x, int k, int lane) {
 }
 
 // The candidates of a row, in LDS.
-constexpr int kCand = 1024;
+constexpr int kCand = 1024, kWork = 8 * kMaxTop + 64;
 struct Candidates {
   uint64_t list[kCand];
   uint64_t fours[64];  // the largest of four lanes
   int count, reach;
+  int work[kWork];     // groups of tiles to read again: group << 8 | thread
 };
 // The k-th largest of the 64 groups' largest, where each thread gives the largest of
 // its part: at least k of all the numbers reach it. All threads call.
@@ -168,7 +170,7 @@ struct Sums {
     e += b.e;
   }
 };
-__device__ __forceinline__ Sums block_sums(Sums v, Sums* waves) {
+__device__ __forceinline__ Sums wave_sums(Sums v) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) {
     Sums o;
@@ -177,29 +179,16 @@ __device__ __forceinline__ Sums block_sums(Sums v, Sums* waves) {
     o.e = __shfl_xor(v.e, off, 64);
     v.join(o);
   }
+  return v;
+}
+__device__ __forceinline__ Sums block_sums(Sums v, Sums* waves) {
+  v = wave_sums(v);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
   __syncthreads();
   v = waves[0];
 #pragma unroll
   for (int w = 1; w < kThreads / 64; ++w) v.join(waves[w]);
   return v;
-}
-
-// A row's results from its sums and the candidates of its largest logits.
-template <typename T>
-__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, Sums v, Candidates& c) {
-  const float s = v.s == 0.f ? __builtin_nanf("") : v.s, lse = logf(s);  // (nothing but -inf: no distribution)
-  if (threadIdx.x == 0) {
-    const int64_t t = token_of(a, row);
-    const float x = t >= 0 && t < a.V ? to_float(static_cast<const T*>(a.x)[row * a.x_s0 + t * a.x_s1]) : -INFINITY;
-    a.logp[row * a.lp_s] = (x - v.m) - lse;
-    a.entropy[row * a.en_s] = lse - kLn2 * (v.e / s);
-  }
-  if (a.top > 0)
-    write_top(c, a.top, [&](int place, uint64_t rank) {
-      a.top_tok[row * a.tt_s0 + place * a.tt_s1] = index_of(rank);
-      a.top_logp[row * a.tl_s0 + place * a.tl_s1] = (value_of(rank) - v.m) - lse;
-    });
 }
 
 // 16 bytes of logits.
@@ -221,255 +210,275 @@ template <> struct Piece<f16_t> {
 };
 
 constexpr int kUnroll = 8;   // pieces of a thread in flight: a tile is 256 x 8 pieces
-constexpr int kGroups = 12;  // runs of tiles of which each thread keeps its largest logit
+constexpr int kGroups = 12;  // runs of tiles of a row, of which each thread keeps its largest logit
 constexpr int kTilePieces = kThreads * kUnroll;
 
-// What a row's segment leaves for the second launch: its sums, then its k largest.
-__host__ __device__ constexpr int part_words(int top) { return 4 + 2 * top; }
+// A row: `head` logits before the first 16-byte boundary, whole pieces, `tail` behind
+// them. Thread i has the i-th of the head, thread 32 + i that of the tail (the edges).
+template <typename T>
+struct Row {
+  typedef Piece<T> PT;
+  static constexpr int VE = PT::n;
+  const T* x;
+  const T* body;
+  int V, head, pieces, tail, tiles;
+  __device__ __forceinline__ Row(const LogprobArgs& a, int64_t row) {
+    x = static_cast<const T*>(a.x) + row * a.x_s0;
+    V = a.V;
+    head = min(V, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
+    body = x + head;
+    pieces = (V - head) / VE;
+    tail = V - head - pieces * VE;
+    tiles = (pieces + kTilePieces - 1) / kTilePieces;
+  }
+  __device__ __forceinline__ int edge() const {  // the thread's, -1: none
+    const int t = threadIdx.x;
+    return t < head ? t : t >= 32 && t - 32 < tail ? V - tail + t - 32 : -1;
+  }
+  // A tile's pieces of this thread; those past the row's are of -inf.
+  __device__ __forceinline__ void load(int t, u32x4 (&w)[kUnroll]) const {
+    const u32x4* const p = reinterpret_cast<const u32x4*>(body);
+    const int p0 = t * kTilePieces + static_cast<int>(threadIdx.x);
+    if ((t + 1) * kTilePieces <= pieces) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) w[u] = __builtin_nontemporal_load(p + p0 + u * kThreads);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        w[u] = u32x4{PT::none, PT::none, PT::none, PT::none};
+        if (p0 + u * kThreads < pieces) w[u] = p[p0 + u * kThreads];
+      }
+    }
+  }
+  // Sums over tiles t .. end - 1; the thread's largest of them.
+  __device__ __forceinline__ float sum(Sums& v, int t, int end) const {
+    float gm = -INFINITY;
+    for (; t < end; ++t) {
+      u32x4 w[kUnroll];
+      load(t, w);
+      // (a piece at a time: its logits as floats, a few registers, serve both loops)
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VE; i += 2) mx = fmaxf(fmaxf(mx, PT::at(w[u], i)), PT::at(w[u], i + 1));
+        if (mx > v.m + kMove) v.move(mx);
+        gm = fmaxf(gm, mx);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) v.add(PT::at(w[u], i));
+      }
+    }
+    return gm;
+  }
+  __device__ __forceinline__ void sum_edge(Sums& v) const {
+    const int e = edge();
+    if (e < 0) return;
+    const float xe = to_float(x[e]);
+    if (xe > v.m + kMove) v.move(xe);
+    v.add(xe);
+  }
+};
 
-// A workgroup a segment of a row (a.tiles tiles of 256 x 8 pieces of 16 bytes; a row
-// is cut where there are few). The logits before the first 16-byte boundary and behind
-// the last one are the first and the last segment's, one a thread.
-//
-// The loop only sums, and keeps each thread's largest logit of each group of tiles.
-// Then the top-th largest of 64 groups' largest is a threshold that at least `top`
-// logits reach and few others (about 24 for 20 where their places are random), and
-// threads with a group that reaches it read that again. More than kCand of them: those
-// above the threshold and the lowest of those that tie with it, or else all of them a
-// wave's piece at a time, under a floor that rises.
-template <typename T, bool SPLIT>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6))) void token_logprobs_stream(LogprobArgs a, float* __restrict__ part) {
+// The candidates of a row's `top` largest logits. The top-th largest of 64 groups'
+// largest is a threshold that at least `top` logits reach and few others (about 24 for
+// 20 where their places are random), and threads with a group of tiles (group_max[g],
+// tiles per g) that reaches it read that again. More than kCand of them: those above
+// the threshold and the lowest of those that tie with it, or else all of them a wave's
+// piece at a time, under a floor that rises. All threads call.
+template <typename T>
+__device__ __forceinline__ void candidates(const Row<T>& r, int top, int per, const float (&group_max)[kGroups][kThreads],
+                                           Candidates& c) {
   typedef Piece<T> PT;
   constexpr int VE = PT::n;
+  const int tid = threadIdx.x, groups = (r.tiles + per - 1) / per, edge = r.edge();
+  const float at_edge = edge >= 0 ? to_float(r.x[edge]) : -INFINITY;
+  float largest = at_edge;
+  for (int g = 0; g < groups; ++g) largest = fmaxf(largest, group_max[g][tid]);
+  const float threshold = value_of(group_kth(c, rank_of(fmaxf(largest, -INFINITY), 0xFFFFFFFFu), top));
+  auto append = [&](uint64_t rank) __attribute__((always_inline)) {
+    const int at = atomicAdd(&c.count, 1);
+    if (at < kCand) c.list[at] = rank;
+  };
+  // The logits that reach the threshold, from the groups that do (whole pieces at
+  // once); `above`: those past it. False: there are too many. (Of 64 groups, about
+  // -64 ln(1 - top / 64) threads' groups reach it; all do where it is a mask's value.)
+  const int most = r.V <= kCand ? kThreads : min(min(8 * top + 64, kWork), groups * kThreads - 1);
+  auto gather = [&](bool above) {
+    auto in = [&](float x) { return above ? x > threshold : !(x < threshold); };  // (a NaN reaches any, and passes none)
+    __syncthreads();
+    if (tid == 0) c.count = c.reach = 0;
+    __syncthreads();
+    for (int g = 0; g < groups; ++g) {
+      if (!in(group_max[g][tid])) continue;
+      const int at = atomicAdd(&c.reach, 1);
+      if (at < kWork) c.work[at] = g << 8 | tid;
+    }
+    __syncthreads();
+    if (c.reach > most) return false;
+    if (edge >= 0 && in(at_edge)) append(rank_of(at_edge, edge));
+    // (a piece a thread: they are all in flight at once)
+    const int reads = c.reach * per * kUnroll;
+    for (int i = tid; i < reads; i += kThreads) {
+      const int w = c.work[i / (per * kUnroll)], u = i % (per * kUnroll);
+      const int p = (w >> 8) * per * kTilePieces + u * kThreads + (w & 255);
+      if (p >= r.pieces) continue;
+      const u32x4 v = reinterpret_cast<const u32x4*>(r.body)[p];
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (in(PT::at(v, e))) append(rank_of(PT::at(v, e), r.head + p * VE + e));
+    }
+    __syncthreads();
+    return c.count <= kCand;
+  };
+  if (gather(false)) return;
+  if (gather(true)) {
+    // Many tie at the threshold (a mask's value, with fewer tokens allowed than asked
+    // for): those of them among the row's first logits are the lowest.
+    if (tid < min(r.V, 2 * top + 16) && to_float(r.x[tid]) == threshold) append(rank_of(threshold, tid));
+    __syncthreads();
+    if (c.count >= top && c.count <= kCand) return;
+  }
+  uint64_t floor = 0;
+  __syncthreads();
+  if (tid == 0) c.count = 0;
+  __syncthreads();
+  if (edge >= 0) append(rank_of(at_edge, edge));
+#pragma unroll 1
+  for (int y = 0; y < r.tiles; ++y) {
+    // (the largest that this thread's logits of the tile can be)
+    const bool may = floor == 0 || rank_of(group_max[y / per][tid], r.head + y * kTilePieces * VE) > floor;
+    if (!__syncthreads_or(may)) continue;
+#pragma unroll 1
+    for (int i = 0; i < kUnroll * (kThreads / 64); ++i) {
+      const int p = y * kTilePieces + (i >> 2) * kThreads + tid;
+      floor = prune(c, top, kCand - 64 * VE, floor);
+      if (may && tid >> 6 == (i & 3) && p < r.pieces) {
+#pragma unroll 1
+        for (int e = 0; e < VE; ++e) {
+          const uint64_t rank = rank_of(to_float(r.body[p * VE + e]), r.head + p * VE + e);
+          if (rank > floor) append(rank);
+        }
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// A row's results from its sums and the candidates of its largest logits.
+template <typename T>
+__device__ __forceinline__ void write_row(const LogprobArgs& a, int64_t row, const T* x, Sums v, Candidates& c) {
+  const float s = v.s == 0.f ? __builtin_nanf("") : v.s, lse = logf(s);  // (nothing but -inf: no distribution)
+  if (threadIdx.x == 0) {
+    const int64_t t = token_of(a, row);
+    a.logp[row * a.lp_s] = ((t >= 0 && t < a.V ? to_float(x[t]) : -INFINITY) - v.m) - lse;
+    a.entropy[row * a.en_s] = lse - kLn2 * (v.e / s);
+  }
+  if (a.top > 0)
+    write_top(c, a.top, [&](int place, uint64_t rank) {
+      a.top_tok[row * a.tt_s0 + place * a.tt_s1] = index_of(rank);
+      a.top_logp[row * a.tl_s0 + place * a.tl_s1] = (value_of(rank) - v.m) - lse;
+    });
+}
+
+// A workgroup a row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6))) void token_logprobs_stream(LogprobArgs a) {
   __shared__ Candidates c;
   __shared__ float group_max[kGroups][kThreads];
   __shared__ Sums waves[kThreads / 64];
-  const int tid = threadIdx.x;
-  const int64_t items = a.N * a.segments;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t row = item / a.segments;
-    const int seg = static_cast<int>(item - row * a.segments);
-    const T* const x = static_cast<const T*>(a.x) + row * a.x_s0;
-    const int head = min(a.V, static_cast<int>((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
-    const int pieces = (a.V - head) / VE, tail = a.V - head - pieces * VE;
-    const T* const body = x + head;
-    const int t0 = seg * a.tiles, t1 = min(t0 + a.tiles, (pieces + kTilePieces - 1) / kTilePieces);
-    const int per_group = (a.tiles + kGroups - 1) / kGroups;
-
+  for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+    const Row<T> r(a, row);
     Sums v{kNoMax, 0.f, 0.f};
-    float largest = -INFINITY;
-    // A tile's pieces of this thread; those past the row's are none.
-    auto load = [&](int t, u32x4 (&w)[kUnroll]) __attribute__((always_inline)) {
-      const int p0 = t * kTilePieces + tid;
-      if ((t + 1) * kTilePieces <= pieces) {
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          w[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(body) + p0 + u * kThreads);
-      } else {
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          const int p = p0 + u * kThreads;
-          w[u] = u32x4{PT::none, PT::none, PT::none, PT::none};
-          if (p < pieces) w[u] = reinterpret_cast<const u32x4*>(body)[p];
-        }
-      }
-    };
-    for (int g = 0, t = t0; t < t1; ++g) {
-      float gm = -INFINITY;
-      for (const int end = min(t + per_group, t1); t < end; ++t) {
-        u32x4 w[kUnroll];
-        load(t, w);
-        // (a piece at a time: its logits as floats, a few registers, serve both loops)
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < VE; i += 2) mx = fmaxf(fmaxf(mx, PT::at(w[u], i)), PT::at(w[u], i + 1));
-          if (mx > v.m + kMove) v.move(mx);
-          gm = fmaxf(gm, mx);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) v.add(PT::at(w[u], i));
-        }
-      }
-      group_max[g][tid] = gm;
-      largest = fmaxf(largest, gm);
-    }
-    // The edges: thread i has logit i, thread 32 + i the i-th behind the pieces.
-    const bool has_head = seg == 0 && tid < head;
-    const bool has_tail = seg == a.segments - 1 && tid >= 32 && tid - 32 < tail;
-    const int edge = has_head ? tid : a.V - tail + tid - 32;
-    float at_edge = -INFINITY;
-    if (has_head || has_tail) {
-      at_edge = to_float(x[edge]);
-      if (at_edge > v.m + kMove) v.move(at_edge);
-      v.add(at_edge);
-      largest = fmaxf(largest, at_edge);
-    }
-
-    if (a.top > 0) {
-      const uint64_t t = group_kth(c, rank_of(largest, 0xFFFFFFFFu), a.top);
-      const float threshold = value_of(t);
-      auto append = [&](uint64_t r) __attribute__((always_inline)) {
-        const int at = atomicAdd(&c.count, 1);
-        if (at < kCand) c.list[at] = r;
-      };
-      // The logits that reach the threshold, from the groups that do (whole pieces at
-      // once); `above`: those past it. False: there are too many.
-      const int groups = t1 > t0 ? (t1 - t0 + per_group - 1) / per_group : 0;
-      // (of 64 groups, about -64 ln(1 - top / 64) threads' groups reach it; all do where it is a mask's value)
-      const int here = (min(t1 * kTilePieces, pieces) - t0 * kTilePieces) * VE;
-      const int most = here <= kCand ? groups * kThreads : min(8 * a.top + 64, groups * kThreads - 1);
-      auto gather = [&](bool above) {
-        auto in = [&](float xi) { return above ? xi > threshold : !(xi < threshold); };  // (a NaN reaches any, and passes none)
-        __syncthreads();
-        if (tid == 0) c.count = c.reach = 0;
-        __syncthreads();
-        int reach = 0;
-        for (int g = 0; g < groups; ++g) reach += in(group_max[g][tid]);
-        if (reach) atomicAdd(&c.reach, reach);
-        __syncthreads();
-        if (c.reach > most) return false;
-        if ((has_head || has_tail) && in(at_edge)) append(rank_of(at_edge, edge));
-#pragma unroll 1
-        for (int g = 0; g < groups; ++g) {
-          if (!in(group_max[g][tid])) continue;
-#pragma unroll 1
-          for (int y = t0 + g * per_group, end = min(y + per_group, t1); y < end; ++y) {
-            u32x4 w[kUnroll];
-            load(y, w);
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-              const int p = y * kTilePieces + u * kThreads + tid;
-              uint32_t high = 0;
-#pragma unroll
-              for (int i = 0; i < VE; ++i) high |= (in(PT::at(w[u], i)) ? 1u : 0u) << i;
-              if (p >= pieces) high = 0;
-              for (; high; high &= high - 1) {
-                const int i = __builtin_ctz(high);
-                append(rank_of(to_float(body[p * VE + i]), head + p * VE + i));
-              }
-            }
-          }
-        }
-        __syncthreads();
-        return c.count <= kCand;
-      };
-      bool done = gather(false);
-      if (!done && gather(true)) {
-        // Many tie at the threshold (a mask's value, with fewer tokens allowed than
-        // asked for): those of them among the segment's first logits are the lowest.
-        const int i = (seg == 0 ? 0 : head + t0 * kTilePieces * VE) + tid;
-        const int end = seg == a.segments - 1 ? a.V : head + min(t1 * kTilePieces, pieces) * VE;
-        if (tid < 2 * a.top + 16 && i < end && to_float(x[i]) == threshold) append(rank_of(threshold, i));
-        __syncthreads();
-        done = c.count >= a.top && c.count <= kCand;
-      }
-      if (!done) {
-        // Again, a wave's piece at a time, leaving out what a rising floor allows.
-        uint64_t floor = 0;
-        __syncthreads();
-        if (tid == 0) c.count = 0;
-        __syncthreads();
-        if (has_head || has_tail) append(rank_of(at_edge, edge));
-#pragma unroll 1
-        for (int y = t0; y < t1; ++y) {
-          // (the largest that this thread's logits of the tile can be)
-          const float gm = group_max[(y - t0) / per_group][tid];
-          const bool may = floor == 0 || rank_of(gm, head + y * kTilePieces * VE) > floor;
-          if (!__syncthreads_or(may)) continue;
-#pragma unroll 1
-          for (int i = 0; i < kUnroll * (kThreads / 64); ++i) {
-            const int p = y * kTilePieces + (i >> 2) * kThreads + tid;
-            floor = prune(c, a.top, kCand - 64 * VE, floor);
-            if (may && tid >> 6 == (i & 3) && p < pieces) {
-#pragma unroll 1
-              for (int e = 0; e < VE; ++e) {
-                const uint64_t r = rank_of(to_float(body[p * VE + e]), head + p * VE + e);
-                if (r > floor) append(r);
-              }
-            }
-          }
-        }
-        __syncthreads();
-      }
-    }
+    for (int g = 0; g * a.per_group < r.tiles; ++g)
+      group_max[g][threadIdx.x] = r.sum(v, g * a.per_group, min((g + 1) * a.per_group, r.tiles));
+    r.sum_edge(v);
+    if (a.top > 0) candidates<T>(r, a.top, a.per_group, group_max, c);
     v = block_sums(v, waves);
-    if constexpr (SPLIT) {
-      float* const out = part + item * part_words(a.top);
-      if (tid == 0) {
-        out[0] = v.m;
-        out[1] = v.s;
-        out[2] = v.e;
-      }
-      if (a.top > 0) write_top(c, a.top, [&](int place, uint64_t rank) { reinterpret_cast<uint64_t*>(out + 4)[place] = rank; });
-    } else {
-      write_row<T>(a, row, v, c);
-    }
+    write_row<T>(a, row, r.x, v, c);
     __syncthreads();
   }
 }
 
-// The second launch of rows that were cut: a workgroup a row.
+// Few rows: a workgroup a group of a row's tiles, whose sums and threads' largest go
+// to the workspace, then one a row for the rest. The choice of the alternatives once a
+// row, and not once a part of it, is what keeps the second launch short (64 rows of
+// 151936, 20 alternatives: 17.2 + 6.6 us with each part's own 20).
+__host__ __device__ constexpr int part_words(int top) { return 4 + (top > 0 ? kThreads : 0); }
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6))) void token_logprobs_parts(
+    LogprobArgs a, float* __restrict__ part) {
+  __shared__ Sums waves[kThreads / 64];
+  const int64_t items = a.N * a.parts;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t row = item / a.parts;
+    const int g = static_cast<int>(item - row * a.parts);
+    const Row<T> r(a, row);
+    Sums v{kNoMax, 0.f, 0.f};
+    const float gm = r.sum(v, g * a.per_group, min((g + 1) * a.per_group, r.tiles));
+    if (g == 0) r.sum_edge(v);
+    float* const out = part + item * part_words(a.top);
+    if (a.top > 0) out[4 + threadIdx.x] = gm;
+    v = block_sums(v, waves);
+    if (threadIdx.x == 0) *reinterpret_cast<f32x4*>(out) = f32x4{v.m, v.s, v.e, 0.f};
+    __syncthreads();
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void token_logprobs_join(LogprobArgs a, const float* __restrict__ part) {
   __shared__ Candidates c;
-  __shared__ Sums waves[kThreads / 64];
-  const int tid = threadIdx.x;
+  __shared__ float group_max[kGroups][kThreads];
   for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
-    const float* const mine = part + row * a.segments * part_words(a.top);
-    Sums v{kNoMax, 0.f, 0.f};
-    if (tid < a.segments) {
-      const float* const p = mine + tid * part_words(a.top);
+    const Row<T> r(a, row);
+    const float* const mine = part + row * a.parts * part_words(a.top);
+    Sums v{kNoMax, 0.f, 0.f};  // (a part a lane, the same in every wave)
+    const int lane = threadIdx.x & 63;
+    if (lane < a.parts) {
+      const f32x4 p = *reinterpret_cast<const f32x4*>(mine + lane * part_words(a.top));
       v = Sums{p[0], p[1], p[2]};
     }
-    if (tid == 0) c.count = 0;
-    __syncthreads();
-    for (int i = tid; i < a.segments * a.top; i += kThreads) {
-      const int sg = i / a.top;
-      const uint64_t r = reinterpret_cast<const uint64_t*>(mine + sg * part_words(a.top) + 4)[i - sg * a.top];
-      if (r != 0) c.list[atomicAdd(&c.count, 1)] = r;
+    if (a.top > 0) {
+      float gm[kGroups];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g)
+        gm[g] = g < a.parts ? mine[g * part_words(a.top) + 4 + threadIdx.x] : -INFINITY;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) group_max[g][threadIdx.x] = gm[g];
     }
-    v = block_sums(v, waves);
-    write_row<T>(a, row, v, c);
+    v = wave_sums(v);
+    if (a.top > 0) candidates<T>(r, a.top, a.per_group, group_max, c);
+    write_row<T>(a, row, r.x, v, c);
     __syncthreads();
   }
 }
 
-// Rows are cut until there are kWorkgroups, at tiles and at most as the second
-// launch's candidates allow.
-constexpr int64_t kWorkgroups = 1024;
+// Tiles of a group, and the parts that rows are cut into (1: none).
 struct RowCut {
-  int segments, tiles;
+  int per_group, parts;
 };
-static RowCut cut_rows(int64_t N, int64_t V, int64_t top, int elem_bytes) {
-  const int64_t pieces = V * elem_bytes / 16, tiles = (pieces + kTilePieces - 1) / kTilePieces;
-  int64_t s = N < 512 ? (kWorkgroups + N - 1) / N : 1;
-  if (s > tiles) s = tiles;
-  const int64_t most = top > 0 ? kCand / top : kThreads;
-  if (s > most) s = most;
-  if (s > kThreads) s = kThreads;
-  if (s < 1) s = 1;
-  const int64_t per = (tiles + s - 1) / s > 1 ? (tiles + s - 1) / s : 1;
-  return RowCut{static_cast<int>(tiles > 0 ? (tiles + per - 1) / per : 1), static_cast<int>(per)};
+static RowCut cut_rows(int64_t N, int64_t V, int elem_bytes) {
+  const int64_t tiles = (V * elem_bytes / 16 + kTilePieces - 1) / kTilePieces;
+  const int64_t per = tiles > kGroups ? (tiles + kGroups - 1) / kGroups : 1, groups = (tiles + per - 1) / per;
+  return RowCut{static_cast<int>(per), static_cast<int>(N < kWholeRows && groups > 1 ? groups : 1)};
 }
 static size_t cut_bytes(int64_t N, const RowCut& r, int64_t top) {
-  return r.segments > 1 ? sizeof(float) * static_cast<size_t>(N) * r.segments * part_words(static_cast<int>(top)) : 0;
+  return r.parts > 1 ? sizeof(float) * static_cast<size_t>(N) * r.parts * part_words(static_cast<int>(top)) : 0;
 }
 
 template <typename T>
 static int launch_stream(LogprobArgs& a, const RowCut& r, void* workspace, hipStream_t stream) {
-  a.segments = r.segments;
-  a.tiles = r.tiles;
-  const int64_t items = a.N * a.segments;
-  const dim3 grid(static_cast<uint32_t>(items < (1 << 22) ? items : 1 << 22)), rows(static_cast<uint32_t>(a.N < (1 << 22) ? a.N : 1 << 22));
-  float* const part = static_cast<float*>(workspace);
-  if (r.segments == 1) {
-    token_logprobs_stream<T, false><<<grid, dim3(kThreads), 0, stream>>>(a, nullptr);
+  a.per_group = r.per_group;
+  a.parts = r.parts;
+  auto grid = [](int64_t n) { return dim3(static_cast<uint32_t>(n < (1 << 22) ? n : 1 << 22)); };
+  if (r.parts == 1) {
+    token_logprobs_stream<T><<<grid(a.N), dim3(kThreads), 0, stream>>>(a);
     return check_launch("tsa_token_logprobs");
   }
-  token_logprobs_stream<T, true><<<grid, dim3(kThreads), 0, stream>>>(a, part);
+  float* const part = static_cast<float*>(workspace);
+  token_logprobs_parts<T><<<grid(a.N * r.parts), dim3(kThreads), 0, stream>>>(a, part);
   if (int rc = check_launch("tsa_token_logprobs")) return rc;
-  token_logprobs_join<T><<<rows, dim3(kThreads), 0, stream>>>(a, part);
+  token_logprobs_join<T><<<grid(a.N), dim3(kThreads), 0, stream>>>(a, part);
   return check_launch("tsa_token_logprobs");
 }
 
@@ -582,7 +591,7 @@ extern "C" int tsa_token_logprobs(const tsa_view* logprobs, const tsa_view* entr
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.x_s1 == 1 || V == 1) {
     a.x_s1 = 1;
-    const RowCut r = cut_rows(N, V, top, dtype_bytes(logits->dtype));
+    const RowCut r = cut_rows(N, V, dtype_bytes(logits->dtype));
     const size_t need = cut_bytes(N, r, top);
     TSA_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need),
                 "workspace of %zu bytes is too small: %zu needed", workspace_bytes, need);
@@ -605,7 +614,7 @@ extern "C" size_t tsa_token_logprobs_workspace_bytes(int64_t num_tokens, int64_t
     return 0;  // (calls of such sizes are refused, or have nothing to do)
   size_t most = 0;
   for (const int bytes : {2, 4}) {
-    const size_t n = cut_bytes(num_tokens, cut_rows(num_tokens, vocab_size, num_top, bytes), num_top);
+    const size_t n = cut_bytes(num_tokens, cut_rows(num_tokens, vocab_size, bytes), num_top);
     most = n > most ? n : most;
   }
   return most;
