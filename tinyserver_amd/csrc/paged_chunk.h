@@ -27,7 +27,7 @@ struct ChunkArgs {
   // The matrix-core form: page strides in bytes, the tiles (16 tokens) of a page as
   // a multiplier and a shift (page_of_tile), whether output rows go in 8-byte
   // pieces; the queries of a row block, the least blocks of a run, whether runs are
-  // whole items, and 2^16 / G rounded up (row / G of the 128 rows of a block).
+  // whole items, and 2^16 / G rounded up (row / G of a row block's 256 at most).
   uint32_t k_page, v_page, page_mul, page_shift;
   int32_t out8, QB, min_run, whole, g_mul;
 };
@@ -60,7 +60,7 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkArgs& a, int s) {
 // paged_chunk_stream.hip: the plan of a call on the matrix cores (runs 0: sizes past
 // its limits) and its launch.
 struct ChunkPlan {
-  int runs, QB, min_run, whole;
+  int runs, waves, QB, min_run, whole;
   size_t bytes;
 };
 ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap);

@@ -70,15 +70,6 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
   const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32)));
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
-__device__ __forceinline__ ChunkSeq chunk_seq_uniform(const ChunkArgs& a, int s) {
-  ChunkSeq r = chunk_seq(a, s);
-  r.ctx = __builtin_amdgcn_readfirstlane(r.ctx);
-  r.n = __builtin_amdgcn_readfirstlane(r.n);
-  r.end = __builtin_amdgcn_readfirstlane(r.end);
-  r.row0 = uniform64(r.row0);
-  return r;
-}
-
 // Where a run starts: block `blk` of row block rb of (sequence s, kv head kvh).
 struct ChunkStart {
   int s, kvh, rb, blk;
@@ -131,7 +122,7 @@ struct ChunkSplit {
 constexpr size_t kChunkHead = 64;  // bytes before the splits: the number of runs
 // A partial result: 32 NW rows, in the order of the lanes' accumulators, then each
 // row's maximum and sum.
-template <int D, int NW> constexpr int chunk_part_floats() { return 32 * NW * (D + 2); }
+__host__ __device__ constexpr int chunk_part_floats(int D, int NW) { return 32 * NW * (D + 2); }
 
 template <int NT>
 __device__ __forceinline__ uint64_t chunk_scan(uint64_t x, uint64_t* waves, uint64_t& total) {
@@ -151,57 +142,80 @@ __device__ __forceinline__ uint64_t chunk_scan(uint64_t x, uint64_t* waves, uint
 }
 
 // The blocks of all items, and the place of block run * per of them, per = the blocks
-// of a run. smem: 64 + 8 bytes. All threads call.
+// of a run. Up to NT sequences are read once. found: in LDS, where the thread that has
+// the run's sequence leaves it; waves: 64 bytes of LDS. All threads call.
+struct ChunkFound {
+  ChunkSeq r;
+  int64_t off, head;  // blocks of the sequence before the start; of one kv head
+  int32_t s;
+};
 template <int NT>
-__device__ __forceinline__ bool chunk_start(const ChunkArgs& a, uint64_t* smem, int P, int64_t& total, int& per, int& run,
-                                            ChunkStart& st) {
+__device__ __forceinline__ bool chunk_start(const ChunkArgs& a, uint64_t* waves, ChunkFound* found, int P, int64_t& total,
+                                            int& per, int& run, ChunkStart& st) {
   const int tid = threadIdx.x, lane = tid & 63;
+  ChunkSeq r{};
+  int64_t head = 0;
   auto weight = [&](int s) -> uint64_t {
     if (s >= a.B) return 0;
-    const ChunkSeq r = chunk_seq(a, s);
-    return static_cast<uint64_t>(chunk_blocks(r.ctx, r.end, a.QB, chunk_row_blocks(r, a.QB))) * a.Hkv;
+    r = chunk_seq(a, s);
+    head = chunk_blocks(r.ctx, r.end, a.QB, chunk_row_blocks(r, a.QB));
+    return static_cast<uint64_t>(head) * a.Hkv;
   };
-  uint64_t mine = 0, sum;
-  for (int s = tid; s < a.B; s += NT) mine += weight(s);
-  chunk_scan<NT>(mine, smem, sum);
+  uint64_t mine = weight(tid), sum;
+  const uint64_t first = mine;
+  for (int s = tid + NT; s < a.B; s += NT) mine += weight(s);
+  uint64_t b = chunk_scan<NT>(mine, waves, sum);
   total = uniform64(static_cast<int64_t>(sum));
-  const int64_t even = (total + P - 1) / P;
+  // (32-bit divisions where they do: a 64-bit one is a hundred instructions)
+  const int64_t even = total < (int64_t{1} << 31) ? (static_cast<uint32_t>(total) + P - 1) / static_cast<uint32_t>(P)
+                                                  : (total + P - 1) / P;
   per = __builtin_amdgcn_readfirstlane(static_cast<int>(even > a.min_run ? even : a.min_run));
-  const int runs = static_cast<int>((total + per - 1) / per);
+  const int runs = total < (int64_t{1} << 31) ? static_cast<int>((static_cast<uint32_t>(total) + per - 1) / static_cast<uint32_t>(per))
+                                              : static_cast<int>((total + per - 1) / per);
   // Runs of an XCD (workgroups go round the XCDs) follow each other.
   const int of_xcd = (runs + 7) >> 3, i = static_cast<int>(blockIdx.x) >> 3;
   run = (static_cast<int>(blockIdx.x) & 7) * of_xcd + i;
   if (i >= of_xcd || run >= runs) return false;
   const uint64_t x0 = static_cast<uint64_t>(run) * per;
   uint64_t before = 0;
-  int32_t* const found = reinterpret_cast<int32_t*>(smem + 8);
   for (int base = 0; base < a.B; base += NT) {
-    const uint64_t w = weight(base + tid), b = before + chunk_scan<NT>(w, smem, sum);
-    if (b <= x0 && x0 < b + w) {
-      found[0] = base + tid;
-      reinterpret_cast<uint64_t*>(found)[1] = x0 - b;
+    uint64_t w = first;
+    if (a.B > NT) {  // (uniform)
+      w = weight(base + tid);
+      b = before + chunk_scan<NT>(w, waves, sum);
+      before += sum;
     }
-    before += sum;
-    if (x0 < before) break;  // (uniform)
+    if (b <= x0 && x0 < b + w) {
+      found->r = r;
+      found->head = head;
+      found->off = static_cast<int64_t>(x0 - b);
+      found->s = base + tid;
+    }
+    if (a.B > NT && x0 < before) break;  // (uniform)
   }
   __syncthreads();
-  st.s = __builtin_amdgcn_readfirstlane(found[0]);
-  int64_t off = uniform64(reinterpret_cast<int64_t*>(found)[1]);
-  __syncthreads();
-  const ChunkSeq r = chunk_seq_uniform(a, st.s);
-  const int RB = chunk_row_blocks(r, a.QB);
-  const int64_t head = uniform64(chunk_blocks(r.ctx, r.end, a.QB, RB));
-  st.kvh = __builtin_amdgcn_readfirstlane(static_cast<int>(off / head));
-  off -= head * st.kvh;
-  int lo = 0, n = RB;  // the row block is one of lo .. lo + n - 1
+  st.s = __builtin_amdgcn_readfirstlane(found->s);
+  int64_t off = uniform64(found->off);
+  const int64_t of_head = uniform64(found->head);
+  const int ctx = __builtin_amdgcn_readfirstlane(found->r.ctx), end = __builtin_amdgcn_readfirstlane(found->r.end);
+  st.kvh = __builtin_amdgcn_readfirstlane(
+      (off | of_head) < (int64_t{1} << 31) ? static_cast<int>(static_cast<uint32_t>(off) / static_cast<uint32_t>(of_head))
+                                           : static_cast<int>(off / of_head));
+  off -= of_head * st.kvh;
+  int lo = 0, n = chunk_row_blocks(found->r, a.QB);  // the row block is one of lo .. lo + n - 1
+  n = __builtin_amdgcn_readfirstlane(n);
+  int64_t at_lo = 0;  // blocks before it
   while (n > 1) {
-    const int step = (n + 63) >> 6, k = min(lo + lane * step, RB);
-    const int at = __builtin_popcountll(__ballot(lane * step < n && chunk_blocks(r.ctx, r.end, a.QB, k) <= off)) - 1;
+    const int step = (n + 63) >> 6;
+    const int64_t mine_at = lane * step < n ? chunk_blocks(ctx, end, a.QB, lo + lane * step) : INT64_MAX;
+    const int at = __builtin_popcountll(__ballot(mine_at <= off)) - 1;
+    at_lo = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine_at >> 32), at))) << 32 |
+                                 static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine_at), at)));
     n = min(step, n - at * step);
     lo += at * step;
   }
   st.rb = lo;
-  st.blk = __builtin_amdgcn_readfirstlane(static_cast<int>(off - chunk_blocks(r.ctx, r.end, a.QB, lo)));
+  st.blk = __builtin_amdgcn_readfirstlane(static_cast<int>(off - at_lo));
   return true;
 }
 
@@ -239,7 +253,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   int per, run;
   ChunkStart st;
   const int P = static_cast<int>(gridDim.x);
-  const bool has = chunk_start<64 * NW>(a, reinterpret_cast<uint64_t*>(smem), P, total, per, run, st);
+  ChunkFound* const found = reinterpret_cast<ChunkFound*>(smem + 64);
+  const bool has = chunk_start<64 * NW>(a, reinterpret_cast<uint64_t*>(smem), found, P, total, per, run, st);
   if (blockIdx.x == 0 && threadIdx.x == 0) *head = static_cast<int32_t>((total + per - 1) / per);
   if (!has) return;
 
@@ -279,7 +294,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   // registers they cost the loop over blocks 160 spilled ones).
   if (tid == 0) {
     splits[run].runs = 0;
-    work->r = chunk_seq(a, st.s);
+    work->r = found->r;
     work->seg.s = st.s;
     work->seg.kvh = st.kvh;
     work->rb = st.rb;
@@ -641,7 +656,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
       } else {
         // Slot 0: of the item that the run starts inside of; 1: of the one it starts.
-        float* const slot = part + (2 * static_cast<int64_t>(run) + (blk0 == 0 ? 1 : 0)) * chunk_part_floats<D, NW>();
+        float* const slot = part + (2 * static_cast<int64_t>(run) + (blk0 == 0 ? 1 : 0)) * chunk_part_floats(D, NW);
         if (active && my_row(o).ok) {
 #pragma unroll
           for (int x = 0; x < NU; ++x)
@@ -687,7 +702,7 @@ __global__ __launch_bounds__(256) void paged_chunk_merge(ChunkArgs a, const int3
 #pragma unroll
   for (int i = 0; i < NU; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int k = -1; k < sp.runs; ++k) {
-    const float* const slot = part + (2 * static_cast<int64_t>(run + k) + (k < 0 ? 1 : 0)) * chunk_part_floats<D, NW>();
+    const float* const slot = part + (2 * static_cast<int64_t>(run + k) + (k < 0 ? 1 : 0)) * chunk_part_floats(D, NW);
     const f32x2 ml = *reinterpret_cast<const f32x2*>(slot + 32 * NW * D + 2 * rw);
     f32x4 v[NU];
 #pragma unroll

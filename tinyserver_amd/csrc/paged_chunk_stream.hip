@@ -4,55 +4,64 @@
 
 namespace tsa {
 
-constexpr int kChunkWaves = 4;
+// Waves of a workgroup: eight (256 rows, one workgroup a CU) where sequences have rows
+// for it, four (128 rows, two a CU) else.
+static int chunk_waves(int64_t T, int64_t G) { return T * G > 192 ? 8 : 4; }
 
-static int chunk_runs() {
+static int chunk_runs(int waves) {
   int dev = 0, cus = 0;
   if (hipGetDevice(&dev) != hipSuccess ||
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
     cus = 256;
-  return (2 * cus + 7) / 8 * 8;  // two workgroups a CU
+  return (8 / waves * cus + 7) / 8 * 8;  // as many as fit at once
 }
 
 ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap) {
   ChunkPlan p{};
-  const int64_t G = Hq / Hkv, R = 32 * kChunkWaves;
+  T = T < N ? T : N;
+  const int64_t G = Hq / Hkv;
+  p.waves = chunk_waves(T, G);
+  const int64_t R = 32 * p.waves;
   if (G > R) return p;
   p.QB = static_cast<int>(R / G);
   p.min_run = 8;
   // Items of this call at most: row blocks of its tokens, one more a sequence.
-  T = T < N ? T : N;
   const int64_t rows = N < B * T ? N : B * T;
   const int64_t items = Hkv * (rows / p.QB + B), blocks = (cap + 31) / 32;
   if (items >= (int64_t{1} << 38) / (blocks + 1)) return p;  // (a run's blocks stay in 31 bits)
   // Items of a few blocks are not cut: there is nothing to gain from a second launch.
   p.whole = blocks <= 16;
   const int64_t most = p.whole ? items : (items * blocks + p.min_run - 1) / p.min_run;
-  const int64_t P = chunk_runs();
+  const int64_t P = chunk_runs(p.waves);
   p.runs = static_cast<int>(P < (most + 7) / 8 * 8 ? P : (most + 7) / 8 * 8);
-  const size_t part = sizeof(float) * (D == 128 ? chunk_part_floats<128, kChunkWaves>() : chunk_part_floats<64, kChunkWaves>());
+  const size_t part = sizeof(float) * (chunk_part_floats(static_cast<int>(D), p.waves));
   const size_t head = (kChunkHead + p.runs * sizeof(ChunkSplit) + 255) / 256 * 256;
   p.bytes = head + (p.whole ? 0 : 2 * p.runs * part);
   return p;
 }
 
-template <typename T, int D>
+template <typename T, int D, int NW>
 static int launch_stream(const ChunkArgs& a, const ChunkPlan& p, void* workspace, hipStream_t stream) {
   int32_t* const head = static_cast<int32_t*>(workspace);
   ChunkSplit* const splits = reinterpret_cast<ChunkSplit*>(static_cast<char*>(workspace) + kChunkHead);
   float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                                (kChunkHead + p.runs * sizeof(ChunkSplit) + 255) / 256 * 256);
-  paged_chunk_stream<T, D, kChunkWaves><<<dim3(p.runs), dim3(64 * kChunkWaves), 0, stream>>>(a, a.bt, head, splits, part);
+  paged_chunk_stream<T, D, NW><<<dim3(p.runs), dim3(64 * NW), 0, stream>>>(a, a.bt, head, splits, part);
   if (int rc = check_launch("tsa_paged_chunk")) return rc;
   if (p.whole || p.runs < 2) return TSA_OK;
-  paged_chunk_merge<T, D, kChunkWaves><<<dim3(p.runs - 1, kChunkWaves), dim3(256), 0, stream>>>(a, head, splits, part);
+  paged_chunk_merge<T, D, NW><<<dim3(p.runs - 1, NW), dim3(256), 0, stream>>>(a, head, splits, part);
   return check_launch("tsa_paged_chunk");
 }
 
+template <typename T>
+static int launch_stream(const ChunkArgs& a, const ChunkPlan& p, void* workspace, hipStream_t stream) {
+  if (p.waves == 8)
+    return a.D == 128 ? launch_stream<T, 128, 8>(a, p, workspace, stream) : launch_stream<T, 64, 8>(a, p, workspace, stream);
+  return a.D == 128 ? launch_stream<T, 128, 4>(a, p, workspace, stream) : launch_stream<T, 64, 4>(a, p, workspace, stream);
+}
+
 int chunk_stream_launch(const ChunkArgs& a, const ChunkPlan& p, int dt, void* workspace, hipStream_t stream) {
-  if (dt == TSA_BF16)
-    return a.D == 128 ? launch_stream<bf16_t, 128>(a, p, workspace, stream) : launch_stream<bf16_t, 64>(a, p, workspace, stream);
-  return a.D == 128 ? launch_stream<f16_t, 128>(a, p, workspace, stream) : launch_stream<f16_t, 64>(a, p, workspace, stream);
+  return dt == TSA_BF16 ? launch_stream<bf16_t>(a, p, workspace, stream) : launch_stream<f16_t>(a, p, workspace, stream);
 }
 
 }  // namespace tsa
