@@ -9,6 +9,12 @@
 
 namespace tsa {
 
+// What a workgroup's second launch needs of run r: the item that r starts inside of.
+struct ChunkSplit {
+  int64_t row0;              // packed row of the item's first query
+  int32_t kvh, queries;      // its kv head and queries
+  int32_t runs;              // runs r .. r + runs - 1 end it; 0: r is not its first cut
+};
 struct ChunkArgs {
   void* out;
   const void* q;
@@ -30,6 +36,10 @@ struct ChunkArgs {
   // whole items, and 2^16 / G rounded up (row / G of a row block's 256 at most).
   uint32_t k_page, v_page, page_mul, page_shift;
   int32_t out8, QB, min_run, whole, g_mul;
+  // Its workspace: the number of runs, their splits and partial results.
+  int32_t* runs;
+  ChunkSplit* splits;
+  float* part;
 };
 
 constexpr float kNegInfC = -INFINITY;
@@ -64,6 +74,6 @@ struct ChunkPlan {
   size_t bytes;
 };
 ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap);
-int chunk_stream_launch(const ChunkArgs& a, const ChunkPlan& p, int dt, void* workspace, hipStream_t stream);
+int chunk_stream_launch(ChunkArgs& a, const ChunkPlan& p, int dt, void* workspace, hipStream_t stream);
 
 }  // namespace tsa

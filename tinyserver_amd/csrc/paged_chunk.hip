@@ -193,8 +193,6 @@ extern "C" int tsa_paged_chunk(const tsa_view* out, const tsa_view* query, const
       TSA_REQUIRE(workspace != nullptr && workspace_bytes >= p.bytes, "workspace of %zu bytes is too small: %zu needed",
                   workspace_bytes, p.bytes);
       TSA_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
-      a.QB = p.QB; a.min_run = p.min_run; a.whole = p.whole;
-      a.g_mul = (65536 + a.G - 1) / a.G;
       return chunk_stream_launch(a, p, query->dtype, workspace, st);
     }
   }

@@ -37,6 +37,7 @@
 #pragma once
 
 #include "nonfinite.h"
+#include "varlen_prefill_gqa.h"
 #include "paged_chunk.h"
 
 namespace tsa {
@@ -82,42 +83,38 @@ struct ChunkSegment {
   int64_t row;                   // packed row of that query
 };
 struct ChunkWork {
-  ChunkSegment seg;
+  ChunkSegment seg[2];  // in turn: the one in hand, and the next
   ChunkSeq r;
-  int32_t rb, left;
-  // The segment from block blk of row block rb on. One thread.
-  __device__ __forceinline__ void set(const ChunkArgs& a, int blk) {
+  int32_t rb, left, run, per;
+  // One thread: the segment from block blk of row block rb on.
+  __device__ __forceinline__ void set(const ChunkArgs& a, ChunkSegment& x, int s, int kvh, int blk) {
     const int q0 = rb * a.QB;
-    seg.nq = min(a.QB, r.n - q0);
-    seg.pos = r.ctx + q0;
-    seg.end = r.end;
-    seg.row = r.row0 + q0;
-    seg.nblk = (min(seg.pos + seg.nq, r.end) + 31) >> 5;  // keys that its last query sees
-    seg.blk0 = blk;
-    seg.blk1 = a.whole ? seg.nblk : min(seg.nblk, blk + left);
-    left -= seg.blk1 - blk;
+    x.s = s;
+    x.kvh = kvh;
+    x.nq = min(a.QB, r.n - q0);
+    x.pos = r.ctx + q0;
+    x.end = r.end;
+    x.row = r.row0 + q0;
+    x.nblk = (min(x.pos + x.nq, r.end) + 31) >> 5;  // keys that its last query sees
+    x.blk0 = blk;
+    x.blk1 = a.whole ? x.nblk : min(x.nblk, blk + left);
+    left -= x.blk1 - blk;
   }
-  __device__ __forceinline__ void next(const ChunkArgs& a) {
-    if (left <= 0) {
-      seg.blk1 = 0;
-      return;
-    }
+  // One thread: the segment behind `from`.
+  __device__ __forceinline__ void next(const ChunkArgs& a, const ChunkSegment& from, ChunkSegment& x) {
+    x.blk1 = 0;
+    if (left <= 0) return;
+    int s = from.s, kvh = from.kvh;
     if (++rb * a.QB >= r.n) {
       rb = 0;
-      if (++seg.kvh == a.Hkv) {
-        seg.kvh = 0;
-        do r = chunk_seq(a, ++seg.s);
-        while (r.n == 0 && seg.s < a.B - 1);
+      if (++kvh == a.Hkv) {
+        kvh = 0;
+        do r = chunk_seq(a, ++s);
+        while (r.n == 0 && s < a.B - 1);
       }
     }
-    set(a, 0);
+    set(a, x, s, kvh, 0);
   }
-};
-// What a workgroup's second launch needs of run r: the item that r starts inside of.
-struct ChunkSplit {
-  int64_t row0;              // packed row of the item's first query
-  int32_t kvh, queries;      // its kv head and queries
-  int32_t runs;              // runs r .. r + runs - 1 end it; 0: r is not its first cut
 };
 constexpr size_t kChunkHead = 64;  // bytes before the splits: the number of runs
 // A partial result: 32 NW rows, in the order of the lanes' accumulators, then each
@@ -233,8 +230,7 @@ template <int D> constexpr int chunk_lds_bytes() { return 2 * kChunkSlots * 32 *
 
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_stream(
-    ChunkArgs a, const int32_t* __restrict__ bt, int32_t* __restrict__ head, ChunkSplit* __restrict__ splits,
-    float* __restrict__ part) {
+    ChunkArgs a) {
   constexpr int KJ = D / 16, NU = D / 32, CPR = D / 8, RB = 2 * D, BLKB = 32 * RB;
   constexpr int NB = kChunkSlots, A = NB - 1;
   constexpr int RPI = 1024 / RB;            // rows of a 1 KB load instruction
@@ -255,7 +251,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   const int P = static_cast<int>(gridDim.x);
   ChunkFound* const found = reinterpret_cast<ChunkFound*>(smem + 64);
   const bool has = chunk_start<64 * NW>(a, reinterpret_cast<uint64_t*>(smem), found, P, total, per, run, st);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *head = static_cast<int32_t>((total + per - 1) / per);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.runs = static_cast<int32_t>((total + per - 1) / per);
   if (!has) return;
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
@@ -280,7 +276,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   // (lane % CPR) ^ swz(that row), where i changes two bits of swz (one at D = 64).
   const uint32_t rpart = static_cast<uint32_t>(row0w % 16 + lrow) * slot_b;
   const uint32_t cpart = 16u * static_cast<uint32_t>((lane % CPR) ^ swz(row0w + lrow));
-  constexpr int NH = IPW > IPH ? 2 : 1;  // halves a wave loads
+  static_assert(IPW <= IPH, "a wave loads rows of one half");
   const int ka0 = c * RB + 16 * (h ^ swz(c));  // K operand j at ka0 ^ 32 j of a slot
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
   int vofs[NU];
@@ -293,21 +289,24 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   // The run's segments, one after the other: thread 0 keeps them in LDS (held in
   // registers they cost the loop over blocks 160 spilled ones).
   if (tid == 0) {
-    splits[run].runs = 0;
+    a.splits[run].runs = 0;
+    work->run = run;
+    work->per = per;
     work->r = found->r;
-    work->seg.s = st.s;
-    work->seg.kvh = st.kvh;
     work->rb = st.rb;
     const int64_t rest = total - static_cast<int64_t>(run) * per;
     work->left = static_cast<int>(rest < per ? rest : per);
-    work->set(a, st.blk);
-    if (a.whole && st.blk > 0) work->next(a);  // (whole items: to the run that their first block is in)
+    work->set(a, work->seg[0], st.s, st.kvh, st.blk);
+    if (a.whole && st.blk > 0) {  // (whole items: to the run that their first block is in)
+      work->seg[1] = work->seg[0];
+      work->next(a, work->seg[1], work->seg[0]);
+    }
   }
-  __syncthreads();
+  lds_barrier();
 #pragma unroll 1
-  while (work->seg.blk1 > 0) {
+  for (int turn = 0; work->seg[turn].blk1 > 0; turn ^= 1) {
     auto of = [&](const int32_t& x) { return __builtin_amdgcn_readfirstlane(x); };
-    const ChunkSegment& seg = work->seg;
+    const ChunkSegment& seg = work->seg[turn];
     const ChunkArgs& g = chunk_args();
     const int blk0 = of(seg.blk0), blk1 = of(seg.blk1), pos = of(seg.pos), end = of(seg.end);
     const bool active = 32 * wave < of(seg.nq) * g.G;
@@ -330,6 +329,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       return row;
     };
     {
+      // The page of the thread's first half block, asked for before Q: it is needed
+      // first.
+      const int last_tile = (end - 1) >> 4;
+      auto page_at = [&](const ChunkArgs& x, int tile) __attribute__((always_inline)) {
+        const uint32_t lb = page_of_tile(static_cast<uint32_t>(min(tile, last_tile)), x.page_mul, x.page_shift);
+        return x.bt[of(seg.s) * x.bt_s0 + min(static_cast<int>(lb), x.max_blocks - 1) * x.bt_s1];
+      };
+      int page0 = page_at(g, 2 * blk0 + tid);
       u32x4 qop[KJ];
       {
         const Row row = my_row(g);
@@ -339,12 +346,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       }
       const char* const pool = k_wave ? static_cast<const char*>(g.kc) + of(seg.kvh) * g.kc_h * 2
                                       : static_cast<const char*>(g.vc) + of(seg.kvh) * g.vc_h * 2;
-      float m = kChunkNone, l = 0.f;
+      float m, l;
       f32x16 acc[NU];
-#pragma unroll
-      for (int x = 0; x < NU; ++x)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[x][e] = 0.f;
       u32x4 kop[KJ];
       // (`it`, the loop's counter, keeps the operands' places from being computed once
       // and held: they would spill.)
@@ -417,56 +420,71 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           for (int x = 0; x < NU; ++x) acc[x] = mfma_k16x32<T>(vop[s2][x], pop[s2], acc[x]);
       };
 
-      // ---- The segment's blocks, kChunkTab at a time.
+      // ---- The segment's blocks, kChunkTab at a time. A first time with every block
+      // whose pages are there in the pipeline; if what that gives is not finite, V of a
+      // key that some row does not see may be why, and those go one at a time.
+#pragma unroll 1
+      for (bool safe = false;; safe = true) {
+      m = kChunkNone;
+      l = 0.f;
+#pragma unroll
+      for (int x = 0; x < NU; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[x][e] = 0.f;
 #pragma unroll 1
       for (int b0 = blk0; b0 < blk1; b0 += kChunkTab) {
         const int n = min(blk1 - b0, kChunkTab);
         if (tid == 0) *first_bad = n;
-        __syncthreads();
+        lds_barrier();
         const ChunkArgs& f = chunk_args();
         for (int i = tid; i < 2 * n; i += 64 * NW) {
-          const uint32_t tile = static_cast<uint32_t>(2 * b0 + i), lb = page_of_tile(tile, f.page_mul, f.page_shift);
-          const bool in = static_cast<int>(16u * tile) < end;
-          const int page = bt[of(seg.s) * f.bt_s0 + min(static_cast<int>(lb), f.max_blocks - 1) * f.bt_s1];
-          const bool ok = in && page >= 0 && page < f.NB;
+          // (halves behind the last key: the last one's place again)
+          const int tile = min(2 * b0 + i, last_tile);
+          const uint32_t lb = page_of_tile(static_cast<uint32_t>(tile), f.page_mul, f.page_shift);
+          const int page = i == tid && b0 == blk0 ? page0 : page_at(f, tile);
+          const bool ok = page >= 0 && page < f.NB;
           const uint32_t slot0 = 16u * tile - lb * static_cast<uint32_t>(f.BS);
           const uint64_t none = uint64_t{1} << 63;
           tab[i] = ok ? static_cast<uint64_t>(page) * f.k_page + slot0 * static_cast<uint64_t>(2 * f.kc_s) : none;
           tab[2 * kChunkTab + i] = ok ? static_cast<uint64_t>(page) * f.v_page + slot0 * static_cast<uint64_t>(2 * f.vc_s) : none;
           if (!ok) atomicMin(first_bad, i >> 1);
         }
-        __syncthreads();
-        // The first masked block: some row does not see it whole.
-        const int jm = min(__builtin_amdgcn_readfirstlane(*first_bad),
-                           max((min(pos + 1, end) >> 5) - b0, 0));
+        lds_barrier();
+        if (tid == 0 && b0 == blk0 && !safe) work->next(chunk_args(), seg, work->seg[turn ^ 1]);
+        // The first block that some row does not see whole, and the first outside the
+        // pipeline.
+        const int jc = max((min(pos + 1, end) >> 5) - b0, 0);
+        const int jm = min(__builtin_amdgcn_readfirstlane(*first_bad), safe ? jc : n);
         // The wave's places of a block; the loads of one, and of the places of the one
         // after it.
-        uint64_t at[NH];
+        uint64_t at;
         const uint64_t* const my_tab = tab + (k_wave ? 0 : 2 * kChunkTab) + row0w / 16;
-        auto look_up = [&](int blk) __attribute__((always_inline)) {
-          const int j = min(blk, n - 1);
-#pragma unroll
-          for (int y = 0; y < NH; ++y) at[y] = my_tab[2 * j + y];
-        };
+        auto look_up = [&](int blk) __attribute__((always_inline)) { at = my_tab[2 * min(blk, n - 1)]; };
         auto load_block = [&](int blk, int slot) __attribute__((always_inline)) {
           uint32_t lds0 = lds_w;
           asm("" : "+s"(lds0) : "s"(blk));  // (each load's place is added to it here: sixteen of them held would spill)
-          const char* base[NH];
+          const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at));
+          const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32)) & 0x7FFFFFFFu;
+          const char* const base = pool + ((static_cast<uint64_t>(hi) << 32) | lo);
+          constexpr uint32_t kBits = D == 128 ? 16u : 32u;
+          if (32 * (b0 + min(blk, n - 1)) + 32 <= end) {
 #pragma unroll
-          for (int y = 0; y < NH; ++y) {
-            const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at[y]));
-            const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at[y] >> 32)) & 0x7FFFFFFFu;
-            base[y] = pool + ((static_cast<uint64_t>(hi) << 32) | lo);
-          }
+            for (int i = 0; i < IPW; ++i) {
+              // (rpart + (cpart ^ bits of i), made here)
+              uint32_t off;
+              const uint32_t x = kBits * (D == 128 ? i & 3 : i & 1);
+              asm("v_xad_u32 %0, %1, %2, %3" : "=v"(off) : "v"(cpart), "n"(x), "v"(rpart), "s"(blk));
+              dma16_sv(base + static_cast<uint32_t>(i * RPI) * slot_b, off, lds0 + slot * BLKB + i * 1024);
+            }
+          } else {  // The last block: rows behind the last key repeat its row (no row sees them, but 0 times NaN is NaN).
+            const int there = end - 16 * (2 * (b0 + min(blk, n - 1)) + row0w / 16), most = there >= 16 ? 15 : (end - 1) & 15;
 #pragma unroll
-          for (int i = 0; i < IPW; ++i) {
-            // (rpart + (cpart ^ bits of i), made here)
-            uint32_t off;
-            constexpr uint32_t kBits = D == 128 ? 16u : 32u;
-            const uint32_t x = kBits * (D == 128 ? i & 3 : i & 1);
-            asm("v_xad_u32 %0, %1, %2, %3" : "=v"(off) : "v"(cpart), "n"(x), "v"(rpart), "s"(blk));
-            dma16_sv(base[NH == 1 ? 0 : i / IPH] + static_cast<uint32_t>((i % IPH) * RPI) * slot_b, off,
-                     lds0 + slot * BLKB + i * 1024);
+            for (int i = 0; i < IPW; ++i) {
+              int t = threadIdx.x;
+              asm("" : "+v"(t) : "s"(blk));
+              const uint32_t row = static_cast<uint32_t>(min(row0w % 16 + i * RPI + (t & 63) / CPR, most));
+              dma16_sv(base, row * slot_b + (cpart ^ (kBits * (D == 128 ? i & 3 : i & 1))), lds0 + slot * BLKB + i * 1024);
+            }
           }
           look_up(blk + 1);
         };
@@ -483,8 +501,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           there = below(end - k0) & ((e0 < 0 ? 0u : 0xFFFFu) | (e1 < 0 ? 0u : 0xFFFF0000u));
           vis = below(sees - k0) & there;
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (!((vis >> (8 * (e >> 2) + 4 * hm + (e & 3))) & 1)) sc[e] = kNegInfC;
+          for (int e = 0; e < 16; ++e) sc[e] = masked_score(sc[e], vis >> (4 * hm), 8 * (e >> 2) + (e & 3));
         };
         auto fix_v = [&]() __attribute__((always_inline)) {
           bool bad = false;
@@ -530,9 +547,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           }
         };
         f32x16 sca, scb;  // S of the even / odd blocks
-        // One block that every row sees whole: on entry S(j) is in registers, K block
-        // j + 1 and V block j in their slots, and (PREV) block j - 1's P and V
-        // operands in registers.
+        // One block in the pipeline: on entry S(j) is in registers, K block j + 1 and V
+        // block j in their slots, and (PREV) block j - 1's P and V operands in registers.
         auto full = [&](int j, auto S, auto prev) __attribute__((always_inline)) {
           constexpr int s0 = decltype(S)::value;
           f32x16& cur = (s0 & 1) ? scb : sca;
@@ -540,6 +556,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           const bool issue = j < n - A;
           if (issue) load_block(j + A + (k_wave ? 1 : 0), k_wave ? s0 : (s0 + NB - 1) % NB);
           if (active) {
+            if (j >= jc) {  // (uniform) the chunk's own last blocks
+              int hm = h;
+              asm("" : "+v"(hm) : "s"(j));
+              const int upto = min(pos + my_row(chunk_args()).q + 1, end) - 32 * (b0 + j) - 4 * hm;
+              const uint32_t keep = upto >= 32 ? ~0u : upto > 0 ? (1u << upto) - 1u : 0u;  // (of the lane's keys, from its first)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) cur[e] = masked_score(cur[e], keep, 8 * (e >> 2) + (e & 3));
+            }
             kread((s0 + 1) % NB, j);
             if constexpr (decltype(prev)::value) pv();
             const float mt = block_max(cur);
@@ -627,6 +651,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           lds_barrier();
         }
       }
+      // (P's sum is 0 times NaN where an unseen key's V is; l tells of NaN scores)
+      float finite = l * 0.f;
+#pragma unroll
+      for (int x = 0; x < NU; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) finite = fmaf(acc[x][e], 0.f, finite);
+      if (safe || !__syncthreads_or(active && finite != 0.f)) break;
+      }
       // ---- What the segment gives: the item's rows, or a partial result.
       l += __builtin_bit_cast(float, xor_lane32<32>(__builtin_bit_cast(uint32_t, l), lane));
       const ChunkArgs& o = chunk_args();
@@ -656,7 +688,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
       } else {
         // Slot 0: of the item that the run starts inside of; 1: of the one it starts.
-        float* const slot = part + (2 * static_cast<int64_t>(run) + (blk0 == 0 ? 1 : 0)) * chunk_part_floats(D, NW);
+        const int run = of(work->run), per = of(work->per);
+        float* const slot = o.part + (2 * static_cast<int64_t>(run) + (blk0 == 0 ? 1 : 0)) * chunk_part_floats(D, NW);
         if (active && my_row(o).ok) {
 #pragma unroll
           for (int x = 0; x < NU; ++x)
@@ -674,26 +707,22 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           sp.queries = seg.nq;
           sp.runs = item >= static_cast<int64_t>(run - 1) * per
                         ? static_cast<int>((item + seg.nblk - 1) / per) - run + 1 : 0;
-          splits[run] = sp;
+          o.splits[run] = sp;
         }
       }
     }
-    __syncthreads();
-    if (tid == 0) work->next(chunk_args());
-    __syncthreads();
   }
 }
 
 // Items that a cut goes through: the first run that starts inside of one puts its
 // partial results together, a wave's rows a workgroup.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(256) void paged_chunk_merge(ChunkArgs a, const int32_t* __restrict__ head,
-                                                         const ChunkSplit* __restrict__ splits,
-                                                         const float* __restrict__ part) {
+__global__ __launch_bounds__(256) void paged_chunk_merge(ChunkArgs a) {
   constexpr int NU = D / 32;
   const int run = static_cast<int>(blockIdx.x) + 1, wave = blockIdx.y;
-  if (run >= *head) return;
-  const ChunkSplit sp = splits[run];
+  if (run >= *a.runs) return;
+  const ChunkSplit sp = a.splits[run];
+  const float* __restrict__ const part = a.part;
   if (sp.runs == 0 || 32 * wave >= sp.queries * a.G) return;
   const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31, rw = 32 * wave + c, rq = (rw * a.g_mul) >> 16;
   if (rq >= sp.queries) return;

@@ -41,27 +41,30 @@ ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, i
 }
 
 template <typename T, int D, int NW>
-static int launch_stream(const ChunkArgs& a, const ChunkPlan& p, void* workspace, hipStream_t stream) {
-  int32_t* const head = static_cast<int32_t*>(workspace);
-  ChunkSplit* const splits = reinterpret_cast<ChunkSplit*>(static_cast<char*>(workspace) + kChunkHead);
-  float* const part = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                               (kChunkHead + p.runs * sizeof(ChunkSplit) + 255) / 256 * 256);
-  paged_chunk_stream<T, D, NW><<<dim3(p.runs), dim3(64 * NW), 0, stream>>>(a, a.bt, head, splits, part);
+static int launch_stream(const ChunkArgs& a, const ChunkPlan& p, hipStream_t stream) {
+  paged_chunk_stream<T, D, NW><<<dim3(p.runs), dim3(64 * NW), 0, stream>>>(a);
   if (int rc = check_launch("tsa_paged_chunk")) return rc;
   if (p.whole || p.runs < 2) return TSA_OK;
-  paged_chunk_merge<T, D, NW><<<dim3(p.runs - 1, NW), dim3(256), 0, stream>>>(a, head, splits, part);
+  paged_chunk_merge<T, D, NW><<<dim3(p.runs - 1, NW), dim3(256), 0, stream>>>(a);
   return check_launch("tsa_paged_chunk");
 }
 
 template <typename T>
-static int launch_stream(const ChunkArgs& a, const ChunkPlan& p, void* workspace, hipStream_t stream) {
-  if (p.waves == 8)
-    return a.D == 128 ? launch_stream<T, 128, 8>(a, p, workspace, stream) : launch_stream<T, 64, 8>(a, p, workspace, stream);
-  return a.D == 128 ? launch_stream<T, 128, 4>(a, p, workspace, stream) : launch_stream<T, 64, 4>(a, p, workspace, stream);
+static int launch_stream(const ChunkArgs& a, const ChunkPlan& p, hipStream_t stream) {
+  if (p.waves == 8) return a.D == 128 ? launch_stream<T, 128, 8>(a, p, stream) : launch_stream<T, 64, 8>(a, p, stream);
+  return a.D == 128 ? launch_stream<T, 128, 4>(a, p, stream) : launch_stream<T, 64, 4>(a, p, stream);
 }
 
-int chunk_stream_launch(const ChunkArgs& a, const ChunkPlan& p, int dt, void* workspace, hipStream_t stream) {
-  return dt == TSA_BF16 ? launch_stream<bf16_t>(a, p, workspace, stream) : launch_stream<f16_t>(a, p, workspace, stream);
+int chunk_stream_launch(ChunkArgs& a, const ChunkPlan& p, int dt, void* workspace, hipStream_t stream) {
+  char* const ws = static_cast<char*>(workspace);
+  a.QB = p.QB;
+  a.min_run = p.min_run;
+  a.whole = p.whole;
+  a.g_mul = (65536 + a.G - 1) / a.G;
+  a.runs = reinterpret_cast<int32_t*>(ws);
+  a.splits = reinterpret_cast<ChunkSplit*>(ws + kChunkHead);
+  a.part = reinterpret_cast<float*>(ws + (kChunkHead + p.runs * sizeof(ChunkSplit) + 255) / 256 * 256);
+  return dt == TSA_BF16 ? launch_stream<bf16_t>(a, p, stream) : launch_stream<f16_t>(a, p, stream);
 }
 
 }  // namespace tsa
