@@ -85,7 +85,8 @@ struct ChunkSegment {
 struct ChunkWork {
   ChunkSegment seg[2];  // in turn: the one in hand, and the next
   ChunkSeq r;
-  int32_t rb, left, run, per;
+  int32_t rb, left, run, per;  // left: blocks (whole items: items) of the run
+  int32_t bad[2];       // of each segment: its first block (from its table's first) with a page that is not there
   // One thread: the segment from block blk of row block rb on.
   __device__ __forceinline__ void set(const ChunkArgs& a, ChunkSegment& x, int s, int kvh, int blk) {
     const int q0 = rb * a.QB;
@@ -98,7 +99,7 @@ struct ChunkWork {
     x.nblk = (min(x.pos + x.nq, r.end) + 31) >> 5;  // keys that its last query sees
     x.blk0 = blk;
     x.blk1 = a.whole ? x.nblk : min(x.nblk, blk + left);
-    left -= x.blk1 - blk;
+    left -= a.whole ? 1 : x.blk1 - blk;
   }
   // One thread: the segment behind `from`.
   __device__ __forceinline__ void next(const ChunkArgs& a, const ChunkSegment& from, ChunkSegment& x) {
@@ -139,7 +140,7 @@ __device__ __forceinline__ uint64_t chunk_scan(uint64_t x, uint64_t* waves, uint
 }
 
 // The blocks of all items, and the place of block run * per of them, per = the blocks
-// of a run. Up to NT sequences are read once. found: in LDS, where the thread that has
+// of a run. (Whole items: their number, and item run * per.) Up to NT sequences are read once. found: in LDS, where the thread that has
 // the run's sequence leaves it; waves: 64 bytes of LDS. All threads call.
 struct ChunkFound {
   ChunkSeq r;
@@ -155,7 +156,8 @@ __device__ __forceinline__ bool chunk_start(const ChunkArgs& a, uint64_t* waves,
   auto weight = [&](int s) -> uint64_t {
     if (s >= a.B) return 0;
     r = chunk_seq(a, s);
-    head = chunk_blocks(r.ctx, r.end, a.QB, chunk_row_blocks(r, a.QB));
+    head = chunk_row_blocks(r, a.QB);
+    if (!a.whole) head = chunk_blocks(r.ctx, r.end, a.QB, static_cast<int>(head));
     return static_cast<uint64_t>(head) * a.Hkv;
   };
   uint64_t mine = weight(tid), sum;
@@ -199,6 +201,9 @@ __device__ __forceinline__ bool chunk_start(const ChunkArgs& a, uint64_t* waves,
       (off | of_head) < (int64_t{1} << 31) ? static_cast<int>(static_cast<uint32_t>(off) / static_cast<uint32_t>(of_head))
                                            : static_cast<int>(off / of_head));
   off -= of_head * st.kvh;
+  st.rb = static_cast<int>(off);
+  st.blk = 0;
+  if (a.whole) return true;
   int lo = 0, n = chunk_row_blocks(found->r, a.QB);  // the row block is one of lo .. lo + n - 1
   n = __builtin_amdgcn_readfirstlane(n);
   int64_t at_lo = 0;  // blocks before it
@@ -226,7 +231,7 @@ __device__ __forceinline__ const ChunkArgs& chunk_args() {
   return *(const ChunkArgs*)p;
 }
 
-template <int D> constexpr int chunk_lds_bytes() { return 2 * kChunkSlots * 32 * 2 * D + kChunkTab * 32 + 16 + sizeof(ChunkWork); }
+template <int D> constexpr int chunk_lds_bytes() { return 2 * kChunkSlots * 32 * 2 * D + kChunkTab * 32 + sizeof(ChunkWork); }
 
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void paged_chunk_stream(
@@ -242,8 +247,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   // For the halves (16 keys) of a segment's blocks, the byte offset of the first row
   // in the K pool, then (kChunkTab blocks on) in the V pool; bit 63: no such page.
   uint64_t* const tab = reinterpret_cast<uint64_t*>(smem + TOFF);
-  int32_t* const first_bad = reinterpret_cast<int32_t*>(tab + 4 * kChunkTab);  // the first block with such a half
-  ChunkWork* const work = reinterpret_cast<ChunkWork*>(first_bad + 4);
+  ChunkWork* const work = reinterpret_cast<ChunkWork*>(tab + 4 * kChunkTab);
 
   int64_t total;
   int per, run;
@@ -292,15 +296,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     a.splits[run].runs = 0;
     work->run = run;
     work->per = per;
+    work->bad[0] = INT32_MAX;
     work->r = found->r;
     work->rb = st.rb;
     const int64_t rest = total - static_cast<int64_t>(run) * per;
     work->left = static_cast<int>(rest < per ? rest : per);
     work->set(a, work->seg[0], st.s, st.kvh, st.blk);
-    if (a.whole && st.blk > 0) {  // (whole items: to the run that their first block is in)
-      work->seg[1] = work->seg[0];
-      work->next(a, work->seg[1], work->seg[0]);
-    }
   }
   lds_barrier();
 #pragma unroll 1
@@ -434,8 +435,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 #pragma unroll 1
       for (int b0 = blk0; b0 < blk1; b0 += kChunkTab) {
         const int n = min(blk1 - b0, kChunkTab);
-        if (tid == 0) *first_bad = n;
-        lds_barrier();
+        int32_t* const first_bad = &work->bad[turn];
+        if (safe || b0 != blk0) {  // (else the one before left it so)
+          if (tid == 0) *first_bad = INT32_MAX;
+          lds_barrier();
+        }
         const ChunkArgs& f = chunk_args();
         for (int i = tid; i < 2 * n; i += 64 * NW) {
           // (halves behind the last key: the last one's place again)
@@ -450,13 +454,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           if (!ok) atomicMin(first_bad, i >> 1);
         }
         lds_barrier();
-        if (tid == 0 && b0 == blk0 && !safe) work->next(chunk_args(), seg, work->seg[turn ^ 1]);
         // The first block that some row does not see whole, and the first outside the
         // pipeline.
         const int jc = max((min(pos + 1, end) >> 5) - b0, 0);
-        const int jm = min(__builtin_amdgcn_readfirstlane(*first_bad), safe ? jc : n);
+        const int jm = min(min(__builtin_amdgcn_readfirstlane(*first_bad), n), safe ? jc : n);
         // The wave's places of a block; the loads of one, and of the places of the one
         // after it.
+        const int whole = 32 * (b0 + n) > end ? n - 1 : n + A + 2;  // blocks below it have all their keys
         uint64_t at;
         const uint64_t* const my_tab = tab + (k_wave ? 0 : 2 * kChunkTab) + row0w / 16;
         auto look_up = [&](int blk) __attribute__((always_inline)) { at = my_tab[2 * min(blk, n - 1)]; };
@@ -467,7 +471,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32)) & 0x7FFFFFFFu;
           const char* const base = pool + ((static_cast<uint64_t>(hi) << 32) | lo);
           constexpr uint32_t kBits = D == 128 ? 16u : 32u;
-          if (32 * (b0 + min(blk, n - 1)) + 32 <= end) {
+          if (blk < whole) {
 #pragma unroll
             for (int i = 0; i < IPW; ++i) {
               // (rpart + (cpart ^ bits of i), made here)
@@ -477,7 +481,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
               dma16_sv(base + static_cast<uint32_t>(i * RPI) * slot_b, off, lds0 + slot * BLKB + i * 1024);
             }
           } else {  // The last block: rows behind the last key repeat its row (no row sees them, but 0 times NaN is NaN).
-            const int there = end - 16 * (2 * (b0 + min(blk, n - 1)) + row0w / 16), most = there >= 16 ? 15 : (end - 1) & 15;
+            const int there = end - 16 * (2 * (b0 + n - 1) + row0w / 16), most = there >= 16 ? 15 : (end - 1) & 15;
 #pragma unroll
             for (int i = 0; i < IPW; ++i) {
               int t = threadIdx.x;
@@ -603,6 +607,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           for (int x = 0; x < A; ++x)
             if (x < n) load_block(x, x);
         }
+        if (tid == 0 && b0 == blk0 && !safe) {  // (while they are on their way)
+          work->next(chunk_args(), seg, work->seg[turn ^ 1]);
+          work->bad[turn ^ 1] = INT32_MAX;
+        }
         // K(0) and step 0. (Also the Q loads, which the compiler's own waits would
         // otherwise put into the loop.)
         if (n >= A) wait_vmcnt<kInFlight>();
@@ -652,12 +660,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
       }
       // (P's sum is 0 times NaN where an unseen key's V is; l tells of NaN scores)
-      float finite = l * 0.f;
+      float finite[4] = {l * 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int x = 0; x < NU; ++x)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) finite = fmaf(acc[x][e], 0.f, finite);
-      if (safe || !__syncthreads_or(active && finite != 0.f)) break;
+        for (int e = 0; e < 16; ++e) finite[e & 3] = fmaf(acc[x][e], 0.f, finite[e & 3]);
+      if (safe || !__syncthreads_or(active && (finite[0] + finite[1]) + (finite[2] + finite[3]) != 0.f)) break;
       }
       // ---- What the segment gives: the item's rows, or a partial result.
       l += __builtin_bit_cast(float, xor_lane32<32>(__builtin_bit_cast(uint32_t, l), lane));

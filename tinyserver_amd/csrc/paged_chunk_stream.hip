@@ -5,8 +5,11 @@
 namespace tsa {
 
 // Waves of a workgroup: eight (256 rows, one workgroup a CU) where sequences have rows
-// for it, four (128 rows, two a CU) else.
-static int chunk_waves(int64_t T, int64_t G) { return T * G > 192 ? 8 : 4; }
+// for it on average, four (128 rows, two a CU) else: half the K/V reads against twice
+// the items in flight. (28 sequences with one token beside four with 128-512, 32/8
+// heads: 100 us in fours, 127 in eights; 16 with 64-512: 214 in eights, 217 in fours;
+// 2048 over 30720, 64/8 heads: 1.96 ms and 2.2.)
+static int chunk_waves(int64_t B, int64_t rows, int64_t G) { return rows * G > 192 * B ? 8 : 4; }
 
 static int chunk_runs(int waves) {
   int dev = 0, cus = 0;
@@ -20,17 +23,17 @@ ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, i
   ChunkPlan p{};
   T = T < N ? T : N;
   const int64_t G = Hq / Hkv;
-  p.waves = chunk_waves(T, G);
+  const int64_t rows = N < B * T ? N : B * T;
+  p.waves = G > 128 ? 8 : chunk_waves(B, rows, G);
   const int64_t R = 32 * p.waves;
   if (G > R) return p;
   p.QB = static_cast<int>(R / G);
-  p.min_run = 8;
   // Items of this call at most: row blocks of its tokens, one more a sequence.
-  const int64_t rows = N < B * T ? N : B * T;
   const int64_t items = Hkv * (rows / p.QB + B), blocks = (cap + 31) / 32;
   if (items >= (int64_t{1} << 38) / (blocks + 1)) return p;  // (a run's blocks stay in 31 bits)
   // Items of a few blocks are not cut: there is nothing to gain from a second launch.
   p.whole = blocks <= 16;
+  p.min_run = p.whole ? 1 : 8;
   const int64_t most = p.whole ? items : (items * blocks + p.min_run - 1) / p.min_run;
   const int64_t P = chunk_runs(p.waves);
   p.runs = static_cast<int>(P < (most + 7) / 8 * 8 ? P : (most + 7) / 8 * 8);
