@@ -44,15 +44,18 @@ namespace tsa {
 
 constexpr int kChunkSlots = 4;       // K/V blocks in LDS
 constexpr int kChunkTab = 480;       // 32-key blocks whose places the table in LDS holds
+// What an item costs beside its blocks, in blocks (its table, Q, first loads and
+// results: 5 us where a block takes 0.9), which the deal counts at its start.
+constexpr int kItemCost = 6;
 constexpr float kChunkRescale = 8.f; // log2 units a maximum grows before it moves
 constexpr float kChunkNone = -3.402823466e38f;  // the maximum of no score: below every one but -inf, and its weights 0
 
 // ---- The plan on the device.
 // 32-key blocks of a sequence's row blocks 0 .. i - 1: sum of ceil(min(ctx + (k + 1)
-// QB, end) / 32). With QB = 32 qh + ql the remainders of ql repeat after 32 terms.
+// QB, end) / 32), and kItemCost for each. With QB = 32 qh + ql the remainders of ql repeat after 32 terms.
 __device__ __forceinline__ int64_t chunk_blocks(int ctx, int end, int QB, int i) {
   const int full = min(i, (end - ctx) / QB), ql = QB & 31, y = ctx + QB + 31;
-  int64_t sum = static_cast<int64_t>(i - full) * ((end + 31) >> 5) + static_cast<int64_t>(y >> 5) * full +
+  int64_t sum = static_cast<int64_t>(i) * kItemCost + static_cast<int64_t>(i - full) * ((end + 31) >> 5) + static_cast<int64_t>(y >> 5) * full +
                 static_cast<int64_t>(QB >> 5) * full * (full - 1) / 2;
   if (ql) {
     const int K = full >> 5, J = full & 31;
@@ -71,7 +74,8 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
   const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32)));
   return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
 }
-// Where a run starts: block `blk` of row block rb of (sequence s, kv head kvh).
+// Where a run starts: block `blk` of row block rb of (sequence s, kv head kvh), or -blk
+// of its cost before the first.
 struct ChunkStart {
   int s, kvh, rb, blk;
 };
@@ -86,9 +90,10 @@ struct ChunkWork {
   ChunkSegment seg[2];  // in turn: the one in hand, and the next
   ChunkSeq r;
   int32_t rb, left, run, per;  // left: blocks (whole items: items) of the run
+  int32_t redo;         // what a segment gave is not finite
   int32_t bad[2];       // of each segment: its first block (from its table's first) with a page that is not there
-  // One thread: the segment from block blk of row block rb on.
-  __device__ __forceinline__ void set(const ChunkArgs& a, ChunkSegment& x, int s, int kvh, int blk) {
+  // One thread: the segment from block blk of row block rb on, `cost` before it.
+  __device__ __forceinline__ void set(const ChunkArgs& a, ChunkSegment& x, int s, int kvh, int blk, int cost) {
     const int q0 = rb * a.QB;
     x.s = s;
     x.kvh = kvh;
@@ -98,11 +103,13 @@ struct ChunkWork {
     x.row = r.row0 + q0;
     x.nblk = (min(x.pos + x.nq, r.end) + 31) >> 5;  // keys that its last query sees
     x.blk0 = blk;
-    x.blk1 = a.whole ? x.nblk : min(x.nblk, blk + left);
+    left -= cost;
+    x.blk1 = left <= 0 ? 0 : a.whole ? x.nblk : min(x.nblk, blk + left);
     left -= a.whole ? 1 : x.blk1 - blk;
   }
   // One thread: the segment behind `from`.
   __device__ __forceinline__ void next(const ChunkArgs& a, const ChunkSegment& from, ChunkSegment& x) {
+    x = from;  // (without a next, its Q and first page are read again)
     x.blk1 = 0;
     if (left <= 0) return;
     int s = from.s, kvh = from.kvh;
@@ -114,7 +121,7 @@ struct ChunkWork {
         while (r.n == 0 && s < a.B - 1);
       }
     }
-    set(a, x, s, kvh, 0);
+    set(a, x, s, kvh, 0, a.whole ? 0 : kItemCost);
   }
 };
 constexpr size_t kChunkHead = 64;  // bytes before the splits: the number of runs
@@ -217,7 +224,7 @@ __device__ __forceinline__ bool chunk_start(const ChunkArgs& a, uint64_t* waves,
     lo += at * step;
   }
   st.rb = lo;
-  st.blk = __builtin_amdgcn_readfirstlane(static_cast<int>(off - at_lo));
+  st.blk = __builtin_amdgcn_readfirstlane(static_cast<int>(off - at_lo)) - kItemCost;  // (below 0: in what it costs)
   return true;
 }
 
@@ -297,54 +304,58 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
     work->run = run;
     work->per = per;
     work->bad[0] = INT32_MAX;
+    work->redo = 0;
     work->r = found->r;
     work->rb = st.rb;
     const int64_t rest = total - static_cast<int64_t>(run) * per;
     work->left = static_cast<int>(rest < per ? rest : per);
-    work->set(a, work->seg[0], st.s, st.kvh, st.blk);
+    work->set(a, work->seg[0], st.s, st.kvh, max(st.blk, 0), max(-st.blk, 0));
   }
   lds_barrier();
+  auto of = [&](const int32_t& x) { return __builtin_amdgcn_readfirstlane(x); };
+  // The lane's row of a segment, looked up where it is used: query and q-head, and the
+  // packed row of q/out. (Rows past the item's last: its query again, never stored.)
+  struct Row {
+    int q, head;
+    int64_t at;
+    bool ok;
+  };
+  auto my_row = [&](const ChunkArgs& x, const ChunkSegment& seg) __attribute__((always_inline)) {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    const int rw = (t >> 6) * 32 + (t & 31), rq = (rw * x.g_mul) >> 16;
+    Row row;
+    row.q = min(rq, of(seg.nq) - 1);
+    row.head = of(seg.kvh) * x.G + rw - rq * x.G;
+    row.at = seg.row + row.q;
+    row.ok = rq < of(seg.nq);
+    return row;
+  };
+  auto page_at = [&](const ChunkArgs& x, const ChunkSegment& seg, int tile) __attribute__((always_inline)) {
+    // (halves behind the last key: the last one's place again)
+    const uint32_t lb = page_of_tile(static_cast<uint32_t>(min(tile, (of(seg.end) - 1) >> 4)), x.page_mul, x.page_shift);
+    return x.bt[of(seg.s) * x.bt_s0 + min(static_cast<int>(lb), x.max_blocks - 1) * x.bt_s1];
+  };
+  // A segment's Q, and the page of the thread's first half block: asked for while the
+  // one before stores its results.
+  u32x4 qop[KJ];
+  int page0;
+  auto ask = [&](const ChunkSegment& seg) __attribute__((always_inline)) {
+    const ChunkArgs& g = chunk_args();
+    page0 = page_at(g, seg, 2 * of(seg.blk0) + tid);
+    const Row row = my_row(g, seg);
+    const T* const qp = static_cast<const T*>(g.q) + row.at * g.q_sr + row.head * g.q_sh + 8 * h;
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) qop[j] = *reinterpret_cast<const u32x4*>(qp + 16 * j);
+  };
+  ask(work->seg[0]);
 #pragma unroll 1
   for (int turn = 0; work->seg[turn].blk1 > 0; turn ^= 1) {
-    auto of = [&](const int32_t& x) { return __builtin_amdgcn_readfirstlane(x); };
     const ChunkSegment& seg = work->seg[turn];
     const ChunkArgs& g = chunk_args();
     const int blk0 = of(seg.blk0), blk1 = of(seg.blk1), pos = of(seg.pos), end = of(seg.end);
     const bool active = 32 * wave < of(seg.nq) * g.G;
-    // The lane's row, looked up where it is used: query and q-head, and the packed
-    // row of q/out. (Rows past the item's last: its query again, never stored.)
-    struct Row {
-      int q, head;
-      int64_t at;
-      bool ok;
-    };
-    auto my_row = [&](const ChunkArgs& x) __attribute__((always_inline)) {
-      int t = threadIdx.x;
-      asm volatile("" : "+v"(t));
-      const int rw = (t >> 6) * 32 + (t & 31), rq = (rw * x.g_mul) >> 16;
-      Row row;
-      row.q = min(rq, of(seg.nq) - 1);
-      row.head = of(seg.kvh) * x.G + rw - rq * x.G;
-      row.at = seg.row + row.q;
-      row.ok = rq < of(seg.nq);
-      return row;
-    };
     {
-      // The page of the thread's first half block, asked for before Q: it is needed
-      // first.
-      const int last_tile = (end - 1) >> 4;
-      auto page_at = [&](const ChunkArgs& x, int tile) __attribute__((always_inline)) {
-        const uint32_t lb = page_of_tile(static_cast<uint32_t>(min(tile, last_tile)), x.page_mul, x.page_shift);
-        return x.bt[of(seg.s) * x.bt_s0 + min(static_cast<int>(lb), x.max_blocks - 1) * x.bt_s1];
-      };
-      int page0 = page_at(g, 2 * blk0 + tid);
-      u32x4 qop[KJ];
-      {
-        const Row row = my_row(g);
-        const T* const qp = static_cast<const T*>(g.q) + row.at * g.q_sr + row.head * g.q_sh + 8 * h;
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) qop[j] = *reinterpret_cast<const u32x4*>(qp + 16 * j);
-      }
       const char* const pool = k_wave ? static_cast<const char*>(g.kc) + of(seg.kvh) * g.kc_h * 2
                                       : static_cast<const char*>(g.vc) + of(seg.kvh) * g.vc_h * 2;
       float m, l;
@@ -437,22 +448,30 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const int n = min(blk1 - b0, kChunkTab);
         int32_t* const first_bad = &work->bad[turn];
         if (safe || b0 != blk0) {  // (else the one before left it so)
-          if (tid == 0) *first_bad = INT32_MAX;
+          lds_barrier();
+          if (tid == 0) {
+            *first_bad = INT32_MAX;
+            work->redo = 0;
+          }
           lds_barrier();
         }
         const ChunkArgs& f = chunk_args();
-        for (int i = tid; i < 2 * n; i += 64 * NW) {
-          // (halves behind the last key: the last one's place again)
-          const int tile = min(2 * b0 + i, last_tile);
+        auto put = [&](int i, int page) __attribute__((always_inline)) {
+          const int tile = min(2 * b0 + i, (end - 1) >> 4);
           const uint32_t lb = page_of_tile(static_cast<uint32_t>(tile), f.page_mul, f.page_shift);
-          const int page = i == tid && b0 == blk0 ? page0 : page_at(f, tile);
           const bool ok = page >= 0 && page < f.NB;
           const uint32_t slot0 = 16u * tile - lb * static_cast<uint32_t>(f.BS);
           const uint64_t none = uint64_t{1} << 63;
           tab[i] = ok ? static_cast<uint64_t>(page) * f.k_page + slot0 * static_cast<uint64_t>(2 * f.kc_s) : none;
           tab[2 * kChunkTab + i] = ok ? static_cast<uint64_t>(page) * f.v_page + slot0 * static_cast<uint64_t>(2 * f.vc_s) : none;
           if (!ok) atomicMin(first_bad, i >> 1);
+        };
+        int from = tid;
+        if (b0 == blk0 && !safe) {
+          if (tid < 2 * n) put(tid, page0);
+          from += 64 * NW;
         }
+        for (int i = from; i < 2 * n; i += 64 * NW) put(i, page_at(f, seg, 2 * b0 + i));
         lds_barrier();
         // The first block that some row does not see whole, and the first outside the
         // pipeline.
@@ -563,7 +582,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
             if (j >= jc) {  // (uniform) the chunk's own last blocks
               int hm = h;
               asm("" : "+v"(hm) : "s"(j));
-              const int upto = min(pos + my_row(chunk_args()).q + 1, end) - 32 * (b0 + j) - 4 * hm;
+              const int upto = min(pos + my_row(chunk_args(), seg).q + 1, end) - 32 * (b0 + j) - 4 * hm;
               const uint32_t keep = upto >= 32 ? ~0u : upto > 0 ? (1u << upto) - 1u : 0u;  // (of the lane's keys, from its first)
 #pragma unroll
               for (int e = 0; e < 16; ++e) cur[e] = masked_score(cur[e], keep, 8 * (e >> 2) + (e & 3));
@@ -637,7 +656,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
         // ---- The others, one at a time: masks and what they need stay out of the
         // pipeline's registers.
-        if (n1 < n) sees = min(pos + my_row(chunk_args()).q + 1, end);
+        if (n1 < n) sees = min(pos + my_row(chunk_args(), seg).q + 1, end);
 #pragma unroll 1
         for (int j = n1; j < n; ++j) {
           if (active) kread(j % NB, j);
@@ -665,15 +684,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
       for (int x = 0; x < NU; ++x)
 #pragma unroll
         for (int e = 0; e < 16; ++e) finite[e & 3] = fmaf(acc[x][e], 0.f, finite[e & 3]);
-      if (safe || !__syncthreads_or(active && (finite[0] + finite[1]) + (finite[2] + finite[3]) != 0.f)) break;
+      if (safe) break;
+      if (active && (finite[0] + finite[1]) + (finite[2] + finite[3]) != 0.f) work->redo = 1;
+      lds_barrier();
+      if (of(work->redo) == 0) break;
       }
+      ask(work->seg[turn ^ 1]);
       // ---- What the segment gives: the item's rows, or a partial result.
       l += __builtin_bit_cast(float, xor_lane32<32>(__builtin_bit_cast(uint32_t, l), lane));
       const ChunkArgs& o = chunk_args();
       int he = h;
       asm volatile("" : "+v"(he));
       if (blk0 == 0 && blk1 == of(seg.nblk)) {
-        const Row row = my_row(o);
+        const Row row = my_row(o, seg);
         if (active && row.ok) {
           T* const out = static_cast<T*>(o.out) + row.at * o.o_sr + row.head * o.o_sh;
           const int64_t o_sd = o.o_sd;
@@ -698,7 +721,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         // Slot 0: of the item that the run starts inside of; 1: of the one it starts.
         const int run = of(work->run), per = of(work->per);
         float* const slot = o.part + (2 * static_cast<int64_t>(run) + (blk0 == 0 ? 1 : 0)) * chunk_part_floats(D, NW);
-        if (active && my_row(o).ok) {
+        if (active && my_row(o, seg).ok) {
 #pragma unroll
           for (int x = 0; x < NU; ++x)
 #pragma unroll

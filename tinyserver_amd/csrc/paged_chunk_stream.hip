@@ -30,11 +30,11 @@ ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, i
   p.QB = static_cast<int>(R / G);
   // Items of this call at most: row blocks of its tokens, one more a sequence.
   const int64_t items = Hkv * (rows / p.QB + B), blocks = (cap + 31) / 32;
-  if (items >= (int64_t{1} << 38) / (blocks + 1)) return p;  // (a run's blocks stay in 31 bits)
+  if (items >= (int64_t{1} << 38) / (blocks + kItemCost)) return p;  // (a run's blocks stay in 31 bits)
   // Items of a few blocks are not cut: there is nothing to gain from a second launch.
   p.whole = blocks <= 16;
   p.min_run = p.whole ? 1 : 8;
-  const int64_t most = p.whole ? items : (items * blocks + p.min_run - 1) / p.min_run;
+  const int64_t most = p.whole ? items : (items * (blocks + kItemCost) + p.min_run - 1) / p.min_run;
   const int64_t P = chunk_runs(p.waves);
   p.runs = static_cast<int>(P < (most + 7) / 8 * 8 ? P : (most + 7) / 8 * 8);
   const size_t part = sizeof(float) * (chunk_part_floats(static_cast<int>(D), p.waves));
