@@ -26,7 +26,7 @@ HOST = PKG / "_tsa_host.so"
 SOURCES = ["tsa_common.hip", "kv_store.hip", "qk_norm_rope.hip", "paged_decode.hip", "paged_decode_f32.hip",
            "varlen_prefill.hip", "varlen_prefill_w64.hip", "varlen_prefill_f32.hip", "varlen_prefill_window.hip", "sampling.hip",
            "kv_quant.hip", "paged_rows.hip", "paged_rows_unit.hip", "paged_rows_stream.hip",
-           "paged_rows_tree.hip", "paged_chunk.hip", "paged_chunk_stream.hip",
+           "paged_rows_tree.hip", "paged_chunk.hip", "paged_chunk_stream.hip", "paged_chunk_f32.hip",
            "step_tables.hip", "token_logprobs.hip"]
 ARCH = "gfx950"
 # Packed-fp32 VALU instructions are disabled: the compiler may not form them.

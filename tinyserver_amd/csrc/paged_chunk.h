@@ -31,8 +31,8 @@ struct ChunkArgs {
   int32_t T;      // rows of a sequence that are computed, at most
   float scale_log2;
   // The matrix-core form: page strides in bytes, the tiles (16 tokens) of a page as
-  // a multiplier and a shift (page_of_tile), whether output rows go in 8-byte
-  // pieces; the queries of a row block, the least blocks of a run, whether runs are
+  // a multiplier and a shift (page_of_tile), whether output rows go in pieces
+  // of four; the queries of a row block, the least blocks of a run, whether runs are
   // whole items, and 2^16 / G rounded up (row / G of a row block's 256 at most).
   uint32_t k_page, v_page, page_mul, page_shift;
   int32_t out8, QB, min_run, whole, g_mul;
@@ -68,12 +68,13 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkArgs& a, int s) {
 }
 
 // paged_chunk_stream.hip: the plan of a call on the matrix cores (runs 0: sizes past
-// its limits) and its launch.
+// its limits) and its launch; paged_chunk_f32.hip: that of float32 calls.
 struct ChunkPlan {
   int runs, waves, QB, min_run, whole;
   size_t bytes;
 };
-ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap);
+ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap, bool f32);
 int chunk_stream_launch(ChunkArgs& a, const ChunkPlan& p, int dt, void* workspace, hipStream_t stream);
+int chunk_f32_launch(const ChunkArgs& a, const ChunkPlan& p, hipStream_t stream);
 
 }  // namespace tsa

@@ -95,23 +95,22 @@ static int launch_generic(const ChunkArgs& a, hipStream_t stream) {
   return check_launch("tsa_paged_chunk");
 }
 
-// The matrix-core form: 16-bit types, head_dim 64 or 128, pages of whole 16-token
-// tiles, unit-stride rows of 16-byte pieces, strides whose offsets within a page fit
-// 31 bits (a page's own 32), and a positive scale (its maximum is one of raw scores).
-// Fills what it needs of a.
+// The matrix-core forms: head_dim 64 or 128, pages of whole 16-token tiles, unit-stride
+// rows of 16-byte pieces, strides whose offsets within a page fit 31 bits (a page's own
+// 32), and in 16 bits a positive scale (their maximum is one of raw scores). Fills what
+// they need of a.
 static bool takes_mfma(ChunkArgs& a, const tsa_view* out, const tsa_view* query, const tsa_view* k_cache,
                        const tsa_view* v_cache) {
-  if ((query->dtype != TSA_BF16 && query->dtype != TSA_F16) || (a.D != 64 && a.D != 128) || a.BS % 16 ||
-      a.max_blocks == 0 || !(a.scale_log2 > 0.f))
-    return false;
+  const bool f32 = query->dtype == TSA_F32;
+  if ((a.D != 64 && a.D != 128) || a.BS % 16 || a.max_blocks == 0 || !(f32 || a.scale_log2 > 0.f)) return false;
   if (!rows_vec16(query) || !rows_vec16(k_cache) || !rows_vec16(v_cache)) return false;
   auto fits = [&](int64_t page, int64_t slot) {
-    return page >= 0 && page < (int64_t{1} << 31) && slot >= 0 && slot < (int64_t{1} << 30) / a.BS;
+    return page >= 0 && page < (int64_t{1} << 31) && slot >= 0 && slot < (int64_t{1} << 30) / a.BS;  // (elements)
   };
   if (!fits(a.kc_b, a.kc_s) || !fits(a.vc_b, a.vc_s)) return false;
   a.k_page = static_cast<uint32_t>(a.kc_b * 2);
   a.v_page = static_cast<uint32_t>(a.vc_b * 2);
-  a.out8 = a.o_sd == 1 && a.o_sr % 4 == 0 && a.o_sh % 4 == 0 && reinterpret_cast<uintptr_t>(out->data) % 8 == 0;
+  a.out8 = a.o_sd == 1 && a.o_sr % 4 == 0 && a.o_sh % 4 == 0 && reinterpret_cast<uintptr_t>(out->data) % (f32 ? 16 : 8) == 0;
   page_div(a.BS, a.page_mul, a.page_shift);
   return true;
 }
@@ -188,7 +187,8 @@ extern "C" int tsa_paged_chunk(const tsa_view* out, const tsa_view* query, const
   if (a.B == 0 || a.T == 0 || a.Hq == 0 || a.D == 0) return TSA_OK;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (takes_mfma(a, out, query, k_cache, v_cache)) {
-    const ChunkPlan p = chunk_plan(a.B, a.N, a.T, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS);
+    const ChunkPlan p = chunk_plan(a.B, a.N, a.T, a.Hq, a.Hkv, a.D, int64_t{a.max_blocks} * a.BS,
+                                   query->dtype == TSA_F32);
     if (p.runs > 0) {
       TSA_REQUIRE(workspace != nullptr && workspace_bytes >= p.bytes, "workspace of %zu bytes is too small: %zu needed",
                   workspace_bytes, p.bytes);
@@ -212,5 +212,8 @@ extern "C" size_t tsa_paged_chunk_workspace_bytes(int64_t num_seqs, int64_t num_
       max_blocks_per_seq <= 0 || max_blocks_per_seq >= (int64_t{1} << 27) ||
       max_blocks_per_seq * block_size >= (int64_t{1} << 27))
     return 0;  // (calls of such sizes are refused, have nothing to do, or take no workspace)
-  return chunk_plan(num_seqs, num_tokens, max_seqlen, num_heads, num_kv_heads, head_dim, max_blocks_per_seq * block_size).bytes;
+  const int64_t cap = max_blocks_per_seq * block_size;
+  const size_t f16 = chunk_plan(num_seqs, num_tokens, max_seqlen, num_heads, num_kv_heads, head_dim, cap, false).bytes;
+  const size_t f32 = chunk_plan(num_seqs, num_tokens, max_seqlen, num_heads, num_kv_heads, head_dim, cap, true).bytes;
+  return f16 > f32 ? f16 : f32;
 }

@@ -107,6 +107,30 @@ struct ChunkWork {
     x.blk1 = left <= 0 ? 0 : a.whole ? x.nblk : min(x.nblk, blk + left);
     left -= a.whole ? 1 : x.blk1 - blk;
   }
+  // One thread: run `run`, from st on.
+  __device__ __forceinline__ void start(const ChunkArgs& a, const ChunkSeq& first, const ChunkStart& st, int64_t total,
+                                        int run_, int per_) {
+    a.splits[run_].runs = 0;
+    run = run_;
+    per = per_;
+    bad[0] = INT32_MAX;
+    redo = 0;
+    r = first;
+    rb = st.rb;
+    const int64_t rest = total - static_cast<int64_t>(run) * per;
+    left = static_cast<int>(rest < per ? rest : per);
+    set(a, seg[0], st.s, st.kvh, max(st.blk, 0), max(-st.blk, 0));
+  }
+  // What the second launch needs of segment x, which the run starts inside of.
+  __device__ __forceinline__ ChunkSplit split(const ChunkSegment& x) const {
+    const int64_t item = static_cast<int64_t>(run) * per - x.blk0;  // its first block
+    ChunkSplit sp;
+    sp.row0 = x.row;
+    sp.kvh = x.kvh;
+    sp.queries = x.nq;
+    sp.runs = item >= static_cast<int64_t>(run - 1) * per ? static_cast<int>((item + x.nblk - 1) / per) - run + 1 : 0;
+    return sp;
+  }
   // One thread: the segment behind `from`.
   __device__ __forceinline__ void next(const ChunkArgs& a, const ChunkSegment& from, ChunkSegment& x) {
     x = from;  // (without a next, its Q and first page are read again)
@@ -299,18 +323,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 
   // The run's segments, one after the other: thread 0 keeps them in LDS (held in
   // registers they cost the loop over blocks 160 spilled ones).
-  if (tid == 0) {
-    a.splits[run].runs = 0;
-    work->run = run;
-    work->per = per;
-    work->bad[0] = INT32_MAX;
-    work->redo = 0;
-    work->r = found->r;
-    work->rb = st.rb;
-    const int64_t rest = total - static_cast<int64_t>(run) * per;
-    work->left = static_cast<int>(rest < per ? rest : per);
-    work->set(a, work->seg[0], st.s, st.kvh, max(st.blk, 0), max(-st.blk, 0));
-  }
+  if (tid == 0) work->start(a, found->r, st, total, run, per);
   lds_barrier();
   auto of = [&](const int32_t& x) { return __builtin_amdgcn_readfirstlane(x); };
   // The lane's row of a segment, looked up where it is used: query and q-head, and the
@@ -719,8 +732,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         }
       } else {
         // Slot 0: of the item that the run starts inside of; 1: of the one it starts.
-        const int run = of(work->run), per = of(work->per);
-        float* const slot = o.part + (2 * static_cast<int64_t>(run) + (blk0 == 0 ? 1 : 0)) * chunk_part_floats(D, NW);
+        float* const slot = o.part + (2 * static_cast<int64_t>(of(work->run)) + (blk0 == 0 ? 1 : 0)) * chunk_part_floats(D, NW);
         if (active && my_row(o, seg).ok) {
 #pragma unroll
           for (int x = 0; x < NU; ++x)
@@ -730,16 +742,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
                   f32x4{acc[x][e], acc[x][e + 1], acc[x][e + 2], acc[x][e + 3]};
           if (h == 0) *reinterpret_cast<f32x2*>(slot + 32 * NW * D + 2 * (32 * wave + c)) = f32x2{m, l};
         }
-        if (blk0 > 0 && tid == 0) {
-          const int64_t item = static_cast<int64_t>(run) * per - blk0;  // (the run starts with this segment)
-          ChunkSplit sp;
-          sp.row0 = seg.row;
-          sp.kvh = seg.kvh;
-          sp.queries = seg.nq;
-          sp.runs = item >= static_cast<int64_t>(run - 1) * per
-                        ? static_cast<int>((item + seg.nblk - 1) / per) - run + 1 : 0;
-          o.splits[run] = sp;
-        }
+        if (blk0 > 0 && tid == 0) o.splits[work->run] = work->split(seg);
       }
     }
   }

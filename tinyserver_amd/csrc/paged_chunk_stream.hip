@@ -16,15 +16,16 @@ static int chunk_runs(int waves) {
   if (hipGetDevice(&dev) != hipSuccess ||
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
     cus = 256;
-  return (8 / waves * cus + 7) / 8 * 8;  // as many as fit at once
+  return ((waves == 8 ? cus : 2 * cus) + 7) / 8 * 8;  // as many as fit at once
 }
 
-ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap) {
+ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t cap,
+                     bool f32) {
   ChunkPlan p{};
   T = T < N ? T : N;
   const int64_t G = Hq / Hkv;
   const int64_t rows = N < B * T ? N : B * T;
-  p.waves = G > 128 ? 8 : chunk_waves(B, rows, G);
+  p.waves = f32 ? 1 : G > 128 ? 8 : chunk_waves(B, rows, G);  // (float32: 32 rows a workgroup)
   const int64_t R = 32 * p.waves;
   if (G > R) return p;
   p.QB = static_cast<int>(R / G);
@@ -67,6 +68,7 @@ int chunk_stream_launch(ChunkArgs& a, const ChunkPlan& p, int dt, void* workspac
   a.runs = reinterpret_cast<int32_t*>(ws);
   a.splits = reinterpret_cast<ChunkSplit*>(ws + kChunkHead);
   a.part = reinterpret_cast<float*>(ws + (kChunkHead + p.runs * sizeof(ChunkSplit) + 255) / 256 * 256);
+  if (dt == TSA_F32) return chunk_f32_launch(a, p, stream);
   return dt == TSA_BF16 ? launch_stream<bf16_t>(a, p, stream) : launch_stream<f16_t>(a, p, stream);
 }
 
