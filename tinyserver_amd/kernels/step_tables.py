@@ -84,7 +84,7 @@ def step_tables(
     dev = _lib.require_device(tables, context_lens, query_lens, rows, free_blocks, num_free)
     b = context_lens.shape[0]
     sizes = (b * width, b + 1, b, num_tokens, num_tokens, num_tokens, 1)
-    parts = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes)  # (one allocation)
+    parts = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split_with_sizes(sizes)  # (one allocation)
     left = parts[6] if free_blocks is not None else None
     block_tables = parts[0].view(b, width)
     _lib.launch("tsa_step_tables", "step_tables", dev, block_tables, *parts[1:6], left, tables, rows, context_lens,
