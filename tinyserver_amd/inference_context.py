@@ -4,7 +4,8 @@ Mirrors server/model/inference_context.py:18-48: ``InferenceContext{mode,
 sequences}`` with ``sequences[i] = {"num_tokens": int, "block_table":
 list[int]}`` in the order of the flattened batch, a module-global current
 context, and ``inference_context(ctx)`` to swap it for the duration of a
-forward. As in the reference the global is unsynchronised: one engine thread
+forward. A step of mode "chunk" gives each sequence's "context_len" too, the
+tokens that its pages hold before the step. As in the reference the global is unsynchronised: one engine thread
 drives the forward and the swap.
 
 The model patch reads the engine's own context module when it imports

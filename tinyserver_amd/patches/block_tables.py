@@ -85,10 +85,10 @@ class BlockTableMirror:
                 self._grow(2 * self.table.shape[0] + batch_size, 0)
         return self.free_rows.pop()
 
-    def gather(self, tables: Sequence[list], extra: Sequence[int] = ()) -> tuple[torch.Tensor, torch.Tensor]:
-        """The (len(tables), width) zero-padded int32 block tables on the
-        device, width = the longest table (at least 1), and `extra` (int32) on
-        the device, from one transfer."""
+    def sync(self, tables: Sequence[list], extra: Sequence[int] = ()) -> tuple[torch.Tensor, torch.Tensor, int]:
+        """Bring `table` up to date with the lists; their rows in it and
+        `extra` (both int32) on the device, from one transfer, and the longest
+        list's length (at least 1)."""
         self.step += 1
         n = len(tables)
         width = max(max((len(t) for t in tables), default=0), 1)
@@ -138,5 +138,11 @@ class BlockTableMirror:
             base = n + len(extra)
             ur, uc, uv = dev[base:base + k].long(), dev[base + k:base + 2 * k].long(), dev[base + 2 * k:]
             self.table.index_put_((ur, uc), uv)
-        out = torch.index_select(self.table[:, :width], 0, dev[:n].long())
-        return out, dev[n:n + len(extra)]
+        return dev[:n], dev[n:n + len(extra)], width
+
+    def gather(self, tables: Sequence[list], extra: Sequence[int] = ()) -> tuple[torch.Tensor, torch.Tensor]:
+        """The (len(tables), width) zero-padded int32 block tables on the
+        device, width = the longest table (at least 1), and `extra` (int32) on
+        the device, from one transfer."""
+        rows, extra, width = self.sync(tables, extra)
+        return torch.index_select(self.table[:, :width], 0, rows.long()), extra

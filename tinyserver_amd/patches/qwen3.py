@@ -24,6 +24,14 @@ reuse it), not once per layer and per sequence: the block tables live on the
 device (block_tables.BlockTableMirror) and a step uploads only the blocks
 appended since the last one, with cu_seqlens, in one transfer.
 
+Beside the reference's two modes there is "chunk": every sequence brings
+``num_tokens`` new tokens (one or more) behind the ``context_len`` that its
+pages hold already, as a prompt does that is brought in pieces, or whose first
+part was found in the cache, and a step that decodes some sequences and brings
+pieces of others. Its tables and positions are made on the GPU (step_tables),
+its tokens stored at their positions, and attention runs over the cache
+(paged_attention_chunk).
+
 Same errors as the reference: ValueError for prefill lengths that do not sum
 to the flattened length or are not positive (:182-187) and for a missing
 position_ids (:231-236, :329-330); MemoryError when not even one KV block
@@ -42,7 +50,8 @@ import numpy as np
 import torch
 
 from .. import inference_context as _own_context
-from ..kernels import flash_attn_varlen_func, paged_attention_forward, paged_decode_step, qk_norm_rope_store
+from ..kernels import (flash_attn_varlen_func, paged_attention_chunk, paged_attention_forward, paged_decode_step,
+                       qk_norm_rope_store, step_tables)
 from .block_tables import BlockTableMirror
 
 ENGINE_CONTEXT_MODULE = "server.model.inference_context"
@@ -93,9 +102,10 @@ class DeviceMetadata:
     block_tables: torch.Tensor  # (B, max_blocks) int32, zero-padded
     cu_seqlens: torch.Tensor    # (B + 1,) int32 offsets into the flattened tokens
     max_seqlen: int
-    positions: torch.Tensor | None  # decode: (B,) int32 position of each new token
-    seq_lens: torch.Tensor | None   # decode: (B,) int32 = positions + 1
+    positions: torch.Tensor | None  # decode and chunk: int32 position of each new token
+    seq_lens: torch.Tensor | None   # decode and chunk: (B,) int32 cached and new tokens
     table_slots: int = 0            # sum of the block tables' lengths (host-side size of the step's KV)
+    context_lens: torch.Tensor | None = None  # chunk: (B,) int32 tokens in the cache before the step
 
 
 # The device-resident block tables, one mirror per device.
@@ -109,7 +119,7 @@ _last_build: tuple | None = None
 
 
 def device_metadata(ctx: Any, position_ids: torch.Tensor | None, num_tokens: int,
-                    device: torch.device) -> DeviceMetadata:
+                    device: torch.device, block_size: int | None = None) -> DeviceMetadata:
     """Build the padded block tables, cu_seqlens and, for a decode step, the
     positions and sequence lengths, with the reference's checks. The block
     tables come from the device's BlockTableMirror, which uploads only the
@@ -124,19 +134,33 @@ def device_metadata(ctx: Any, position_ids: torch.Tensor | None, num_tokens: int
     cache holds only a weak reference to it, so a later step -- or a context
     at a recycled address -- never hits a stale entry. A context that cannot
     be weakly referenced is rebuilt per layer. The context's sequences must
-    not be changed in place during a forward."""
+    not be changed in place during a forward. A chunk step, whose positions are
+    made here, needs the cache's block_size."""
     global _last_build
-    key = (ctx.mode, num_tokens, str(device), getattr(position_ids, "_version", None))
+    key = (ctx.mode, num_tokens, str(device), getattr(position_ids, "_version", None),
+           block_size if ctx.mode == "chunk" else None)
     last = _last_build
     if last is not None and last[0]() is ctx and last[1] is position_ids and last[2] == key:
         return last[3]
     seqs = ctx.sequences
-    if ctx.mode == "prefill":
+    contexts: list[int] = []
+    if ctx.mode in ("prefill", "chunk"):
+        what = ctx.mode.capitalize()
         lengths = [int(s["num_tokens"]) for s in seqs]
         if sum(lengths) != num_tokens:
-            raise ValueError(f"Prefill sequence lengths sum to {sum(lengths)}, expected flattened seq_len {num_tokens}")
+            raise ValueError(f"{what} sequence lengths sum to {sum(lengths)}, expected flattened seq_len {num_tokens}")
         if any(n <= 0 for n in lengths):
-            raise ValueError("Prefill sequence lengths must all be positive")
+            raise ValueError(f"{what} sequence lengths must all be positive")
+        if ctx.mode == "chunk":
+            if block_size is None:
+                raise ValueError("A chunk step needs the cache's block_size")
+            contexts = [int(s["context_len"]) for s in seqs]
+            if any(n < 0 for n in contexts):
+                raise ValueError("Chunk context lengths must not be negative")
+            for s, c, n in zip(seqs, contexts, lengths):
+                if len(s["block_table"]) * block_size < c + n:
+                    raise ValueError(f"A block table of {len(s['block_table'])} blocks of {block_size} tokens does not "
+                                     f"hold {c} cached and {n} new tokens")
     else:
         if position_ids is None:
             raise ValueError("Position ids should not be None for decode attention")
@@ -149,13 +173,19 @@ def device_metadata(ctx: Any, position_ids: torch.Tensor | None, num_tokens: int
     mirror = _mirrors.get(device)
     if mirror is None:
         mirror = _mirrors[device] = BlockTableMirror(device)
-    block_tables, cu_seqlens = mirror.gather(tables, cu)
-    positions = seq_lens = None
-    if ctx.mode != "prefill":
+    positions = seq_lens = context_lens = None
+    if ctx.mode == "chunk":
+        rows, given, width = mirror.sync(tables, contexts + lengths)
+        context_lens = given[: len(seqs)]
+        step = step_tables(mirror.table, context_lens, given[len(seqs) :], block_size, num_tokens, rows=rows, width=width)
+        block_tables, cu_seqlens, seq_lens, positions = step[:4]
+    else:
+        block_tables, cu_seqlens = mirror.gather(tables, cu)
+    if ctx.mode not in ("prefill", "chunk"):
         positions = position_ids.reshape(-1).to(device=device, dtype=torch.int32)
         seq_lens = positions + 1
     meta = DeviceMetadata(block_tables, cu_seqlens, max(lengths, default=0), positions, seq_lens,
-                          sum(len(t) for t in tables))
+                          sum(len(t) for t in tables), context_lens)
     try:
         ref = weakref.ref(ctx)
     except TypeError:  # (e.g. a slotted class without __weakref__): no caching
@@ -207,14 +237,21 @@ def _patch_single_layer(layer: torch.nn.Module,
         sin = sin.reshape(-1, head_dim)
 
         ctx = get_context()
-        meta = device_metadata(ctx, position_ids, batch * seq_len, hidden_states.device)
         block_size = attn.k_cache.shape[2]
+        meta = device_metadata(ctx, position_ids, batch * seq_len, hidden_states.device, block_size)
         if ctx.mode == "prefill":
             q_rot, k_rot = qk_norm_rope_store(q, k, v, attn.q_norm.weight, attn.k_norm.weight, cos, sin,
                                               attn.q_norm.variance_epsilon, attn.k_cache, attn.v_cache,
                                               meta.block_tables, meta.cu_seqlens)
             out = flash_attn_varlen_func(q_rot, k_rot, v, meta.cu_seqlens, meta.cu_seqlens, meta.max_seqlen,
                                          meta.max_seqlen, causal=True, softmax_scale=head_dim**-0.5)
+        elif ctx.mode == "chunk":
+            q_rot, _ = qk_norm_rope_store(q, k, v, attn.q_norm.weight, attn.k_norm.weight, cos, sin,
+                                          attn.q_norm.variance_epsilon, attn.k_cache, attn.v_cache,
+                                          meta.block_tables, meta.cu_seqlens, meta.positions, return_k=False)
+            out = paged_attention_chunk(q_rot, attn.k_cache, attn.v_cache, meta.block_tables, block_size,
+                                        meta.context_lens, meta.cu_seqlens, max_seqlen=meta.max_seqlen,
+                                        softmax_scale=head_dim**-0.5)
         elif (getattr(attn, "_tsa_fused_decode", True)
               and meta.table_slots * block_size // 16 * num_kv_heads <= FUSED_DECODE_MAX_TILES):
             try:
