@@ -298,20 +298,11 @@ __global__ __launch_bounds__(256) void paged_chunk_f32_merge(ChunkArgs a) {
   if (run >= *a.runs) return;
   const ChunkSplit sp = a.splits[run];
   if (sp.runs == 0 || r >= sp.queries * a.G) return;
-  float M = kChunkNone, den = 0.f;
   f32x4 o[D / 32];
-#pragma unroll
-  for (int x = 0; x < D / 32; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int k = -1; k < sp.runs; ++k) {
-    const float* const slot = a.part + (2 * static_cast<int64_t>(run + k) + (k < 0 ? 1 : 0)) * chunk_part_floats(D, 1);
-    const f32x2 ml = *reinterpret_cast<const f32x2*>(slot + kF32Rows * D + 2 * r);
-    const float mn = fmaxf(M, ml[0]), c_old = fast_exp2(M - mn), c_new = fast_exp2(ml[0] - mn);
-#pragma unroll
-    for (int x = 0; x < D / 32; ++x)
-      o[x] = o[x] * c_old + *reinterpret_cast<const f32x4*>(slot + r * D + 4 * ((tid & 7) + 8 * x)) * c_new;
-    den = fmaf(ml[1], c_new, den * c_old);
-    M = mn;
-  }
+  const float den = chunk_join<D / 32>(
+      sp.runs + 1, kF32Rows * D, r,
+      [&](int k) { return a.part + (2 * static_cast<int64_t>(run + k - 1) + (k == 0 ? 1 : 0)) * chunk_part_floats(D, 1); },
+      [&](int x) { return r * D + 4 * ((tid & 7) + 8 * x); }, o);
   const int qq = (r * a.g_mul) >> 16;
   float* const out = static_cast<float*>(a.out) + (sp.row0 + qq) * a.o_sr + (sp.kvh * a.G + r - qq * a.G) * a.o_sh;
 #pragma unroll
