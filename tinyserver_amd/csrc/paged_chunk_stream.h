@@ -292,6 +292,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, c = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const float cs = a.scale_log2;  // > 0 here
+  // Of two workgroups on a CU the one that came first has its waves served first, and
+  // the other ran 20 us alone at the end of 80: three blocks of four it goes first now
+  // (2 x 12-40 tokens over 24000-32768: 89 -> 85.5 us; all four: 87).
+  const bool second = NW == 4 && (blockIdx.x >> 3) * 16 >= gridDim.x;
+  if (NW == 4 && !second) __builtin_amdgcn_s_setprio(1);
 
   // ---- Loads: waves 0 .. NW / 2 - 1 the K rows, the others the V rows, IPW
   // instructions of RPI rows; lane l of one whose first row is R0 fetches the
@@ -589,6 +594,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
           constexpr int s0 = decltype(S)::value;
           f32x16& cur = (s0 & 1) ? scb : sca;
           f32x16& nxt = (s0 & 1) ? sca : scb;
+          if (second) __builtin_amdgcn_s_setprio(s0 ? 2 : 0);
           const bool issue = j < n - A;
           if (issue) load_block(j + A + (k_wave ? 1 : 0), k_wave ? s0 : (s0 + NB - 1) % NB);
           if (active) {
