@@ -8,8 +8,12 @@ namespace tsa {
 // for it on average, four (128 rows, two a CU) else: half the K/V reads against twice
 // the items in flight. (28 sequences with one token beside four with 128-512, 32/8
 // heads: 100 us in fours, 127 in eights; 16 with 64-512: 214 in eights, 217 in fours;
-// 2048 over 30720, 64/8 heads: 1.96 ms and 2.2.)
-static int chunk_waves(int64_t B, int64_t rows, int64_t G) { return rows * G > 192 * B ? 8 : 4; }
+// 2048 over 30720, 64/8 heads: 1.96 ms and 2.2.) Eight also from 128 rows on where no
+// sequence has more than 256: K/V are read once then. (20 tokens each over 2 x
+// 24000-32768, 64/8 heads: 81 us, 94 in fours; 12 and 40 each: 108 and 98.)
+static int chunk_waves(int64_t B, int64_t rows, int64_t G, int64_t T) {
+  return rows * G > (T * G <= 256 ? 128 : 192) * B ? 8 : 4;
+}
 
 static int chunk_runs(int waves) {
   int dev = 0, cus = 0;
@@ -25,7 +29,7 @@ ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, i
   T = T < N ? T : N;
   const int64_t G = Hq / Hkv;
   const int64_t rows = N < B * T ? N : B * T;
-  p.waves = f32 ? 1 : G > 128 ? 8 : chunk_waves(B, rows, G);  // (float32: 32 rows a workgroup)
+  p.waves = f32 ? 1 : G > 128 ? 8 : chunk_waves(B, rows, G, T);  // (float32: 32 rows a workgroup)
   const int64_t R = 32 * p.waves;
   if (G > R) return p;
   p.QB = static_cast<int>(R / G);
