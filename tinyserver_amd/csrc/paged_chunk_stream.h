@@ -27,11 +27,13 @@
 // block j - 1 under its maximum; two workgroups a CU give a SIMD two waves, of which
 // one's exponentials run under the other's products.
 //
-// Blocks that every row sees whole take no mask. The others (the chunk's own last
-// ones, and those with a page that is not there) leave the pipeline and follow one at
-// a time: there scores that a row does not see become -inf, V rows that are not there
-// become 0, and elements of V that are not finite reach the rows that see them through
-// a product of flags (a weight of 0 times one would be NaN).
+// The chunk's own last blocks take their masks in the pipeline; blocks before them
+// need none, and those with a page that is not there leave it and follow one at a time.
+// Rows of V that no row sees repeat the last key's there. Where an item's sums are not
+// finite, V of a key that some row does not see may be why (a weight of 0 times NaN):
+// the item goes again with every masked block one at a time, where V rows that are not
+// there become 0 and elements of V that are not finite reach the rows that see them
+// through a product of flags.
 // A weight goes to the second product rounded once to T, off by at most 2^-8 (f16:
 // 2^-11) of itself, as in the prefill kernels.
 #pragma once
@@ -171,8 +173,9 @@ __device__ __forceinline__ uint64_t chunk_scan(uint64_t x, uint64_t* waves, uint
 }
 
 // The blocks of all items, and the place of block run * per of them, per = the blocks
-// of a run. (Whole items: their number, and item run * per.) Up to NT sequences are read once. found: in LDS, where the thread that has
-// the run's sequence leaves it; waves: 64 bytes of LDS. All threads call.
+// of a run. (Whole items: their number, and item run * per.) Up to NT sequences are
+// read once. found: in LDS, where the thread that has the run's sequence leaves it;
+// waves: 64 bytes of LDS. All threads call.
 struct ChunkFound {
   ChunkSeq r;
   int64_t off, head;  // blocks of the sequence before the start; of one kv head
@@ -756,8 +759,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
 
 // The partial results of an item that a cut goes through, put together, the reads of
 // four runs' in flight at once (32 runs an item 21 -> 11.5 us, two 13 -> 11; eight at once
-// by four times the threads: 12.3 and 12 to 14). slot(k): the k-th of n; row: the thread's, whose maximum
-// and sum are behind the slot's first `sums` floats; at(i): its i-th four floats.
+// by four times the threads: 12.3 and 12 to 14). slot(k): the k-th of n; row: the
+// thread's, whose maximum and sum are behind the slot's first `sums` floats; at(i): its
+// i-th four floats.
 template <int NU, typename S, typename F>
 __device__ __forceinline__ float chunk_join(int n, int sums, int row, S slot, F at, f32x4 (&o)[NU]) {
   float M = kChunkNone, den = 0.f;
