@@ -361,6 +361,7 @@ __device__ __forceinline__ void candidates(const Row<T>& r, int top, int per, co
     for (int i = 0; i < kUnroll * (kThreads / 64); ++i) {
       const int p = y * kTilePieces + (i >> 2) * kThreads + tid;
       floor = prune(c, top, kCand - 64 * VE, floor);
+      __syncthreads();  // (every wave has read the count that prune left)
       if (may && tid >> 6 == (i & 3) && p < r.pieces) {
 #pragma unroll 1
         for (int e = 0; e < VE; ++e) {
