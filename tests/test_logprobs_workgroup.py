@@ -53,6 +53,20 @@ def check(lib, x, top):
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("v", [5003, 40001])  # whole rows, and rows cut into parts
+@pytest.mark.parametrize("allowed", [908, 909, 1000, 1024, 1025])
+@pytest.mark.parametrize("top", [50, 64])
+def test_allowed_tokens_in_one_place(lib, top, allowed, v, dtype):
+    """A mask of consecutive tokens, which lie in fewer groups of threads than alternatives are asked for; the list
+    has 1,024 places, and up to 2 top + 16 of the masked ones are added to it."""
+    g = torch.Generator().manual_seed(allowed + top)
+    x = torch.full((2, v), -INF).to(dtype)
+    x[0, 1600 : 1600 + allowed] = torch.randn(allowed, generator=g).to(dtype)
+    x[1, v - 3 - allowed : v - 3] = torch.randn(allowed, generator=g).to(dtype)
+    check(lib, x, top)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("v", [5003, 40001])
 @pytest.mark.parametrize("kind", ["rising", "stairs", "few", "nan"])
 def test_rows_a_piece_at_a_time(lib, kind, v, dtype):
     """Rows with more candidates than the list holds."""

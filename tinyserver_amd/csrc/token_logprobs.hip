@@ -343,6 +343,7 @@ __device__ __forceinline__ void candidates(const Row<T>& r, int top, int per, co
   if (gather(true)) {
     // Many tie at the threshold (a mask's value, with fewer tokens allowed than asked
     // for): those of them among the row's first logits are the lowest.
+    __syncthreads();  // (every wave has read the count)
     if (tid < min(r.V, 2 * top + 16) && to_float(r.x[tid]) == threshold) append(rank_of(threshold, tid));
     __syncthreads();
     if (c.count >= top && c.count <= kCand) return;
