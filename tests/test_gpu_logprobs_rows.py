@@ -1,10 +1,11 @@
 """Log probabilities of rows that the first tests do not have: a mask that allows about as
-many consecutive tokens as the list of candidates holds (1,024)."""
+many consecutive tokens as the list of candidates holds (1,024); and the same rows again."""
 
 import pytest
 import torch
 
 from tests.test_gpu_logprobs import _check
+from tinyserver_amd.kernels import token_logprobs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -22,3 +23,16 @@ def test_allowed_tokens_in_one_place(allowed, n, v, dtype):
     tokens = torch.randint(1600, 1600 + allowed, (n,), generator=g, device=DEV)
     for top in (50, 64):
         _check(x, tokens, top, f"{allowed} allowed, {n} x {v}, top {top}, {dtype}")
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("n,v", [(3, 151936), (64, 40001), (600, 5003)])
+def test_the_same_again(n, v, dtype):
+    """Call after call, bit for bit, whichever thread writes an alternative."""
+    for seed in range(5):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        x = (3 * torch.randn(n, v, generator=g, device=DEV)).to(dtype)
+        tokens = torch.randint(v, (n,), generator=g, device=DEV)
+        first = token_logprobs(x, tokens, 20)
+        for _ in range(12):
+            assert all(torch.equal(a, b) for a, b in zip(first, token_logprobs(x, tokens, 20))), f"{n} x {v}, {dtype}, seed {seed}"

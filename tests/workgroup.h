@@ -28,6 +28,7 @@
 #define __syncthreads() wg::block_wait(__LINE__, false)
 #define __syncthreads_or(x) wg::block_wait(__LINE__, (x) != 0)
 #define __builtin_amdgcn_readlane(v, l) wg::from_lane(static_cast<int>(v), l)
+#define __builtin_amdgcn_readfirstlane(v) wg::from_lane(static_cast<int>(v), 0)
 #define __shfl_xor(v, off, n) wg::from_lane(v, (threadIdx.x & 63) ^ (off))
 
 struct dim3 {

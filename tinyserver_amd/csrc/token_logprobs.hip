@@ -179,7 +179,10 @@ __device__ __forceinline__ Sums wave_sums(Sums v) {
     o.e = __shfl_xor(v.e, off, 64);
     v.join(o);
   }
-  return v;
+  // (Lanes round their joins in different orders; a row's results are written by threads
+  // that the order of an atomic chooses.)
+  auto first = [](float x) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
+  return Sums{first(v.m), first(v.s), first(v.e)};
 }
 __device__ __forceinline__ Sums block_sums(Sums v, Sums* waves) {
   v = wave_sums(v);
