@@ -1,9 +1,11 @@
 """Log probabilities of rows that the first tests do not have: a mask that allows about as
-many consecutive tokens as the list of candidates holds (1,024); and the same rows again."""
+many consecutive tokens as the list of candidates holds (1,024); the same rows again; and how near sure, flat
+and sparse rows come to 64 bits (the tolerance: logprobs_reference)."""
 
 import pytest
 import torch
 
+from tests.logprobs_reference import near, rows
 from tests.test_gpu_logprobs import _check
 from tinyserver_amd.kernels import token_logprobs
 
@@ -36,3 +38,18 @@ def test_the_same_again(n, v, dtype):
         first = token_logprobs(x, tokens, 20)
         for _ in range(12):
             assert all(torch.equal(a, b) for a, b in zip(first, token_logprobs(x, tokens, 20))), f"{n} x {v}, {dtype}, seed {seed}"
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("kind,n,v", [
+    ("few", 600, 1003), ("few", 20, 20011), ("one_thread", 600, 5003), ("one_thread", 100, 20011), ("sure", 520, 5003),
+    ("sure", 70, 151936), ("even", 5, 151936), ("plain", 8, 151936)])
+def test_accuracy(kind, n, v, dtype):
+    x, tokens = rows(kind, n, v, dtype, DEV)
+    near(x, tokens, token_logprobs(x, tokens, 2), f"{kind}, {n} x {v}, {dtype}")
+
+
+@pytest.mark.parametrize("kind", ["few", "one_thread", "sure", "even"])
+def test_accuracy_of_other_strides(kind):
+    x, tokens = rows(kind, 40, 5003, F32, DEV)
+    near(x, tokens, token_logprobs(x.t().contiguous().t(), tokens, 2), f"{kind}, columns first", side_by_side=False)

@@ -26,11 +26,11 @@ def _aligned(n):
     return x[start : start + n]
 
 
-def run(lib, x, tokens, top):
+def run(lib, x, tokens, top, waves=4):
     """(logprobs, entropy, top_logprobs, top_tokens), the same whichever wave is the first."""
     n, v = x.shape
     first = None
-    for wave in range(4):
+    for wave in range(waves):
         out = (torch.empty(n), torch.empty(n), torch.empty(n, top), torch.empty(n, top, dtype=torch.int64))
         ws = _aligned(lib.tsa_token_logprobs_workspace_bytes(n, v, top))
         lib.wg_order(wave)

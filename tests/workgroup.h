@@ -29,6 +29,7 @@
 #define __syncthreads_or(x) wg::block_wait(__LINE__, (x) != 0)
 #define __builtin_amdgcn_readlane(v, l) wg::from_lane(static_cast<int>(v), l)
 #define __builtin_amdgcn_readfirstlane(v) wg::from_lane(static_cast<int>(v), 0)
+#define __any(x) wg::any_lane(x)
 #define __shfl_xor(v, off, n) wg::from_lane(v, (threadIdx.x & 63) ^ (off))
 
 struct dim3 {
@@ -93,6 +94,14 @@ inline T from_lane(T v, int lane) {
   stop(kAtWave, 0);
   T r;
   std::memcpy(&r, &slots[t][(me & ~63) + lane], sizeof(T));
+  return r;
+}
+inline bool any_lane(bool x) {
+  const int me = current, t = turn[me] ^= 1;
+  slots[t][me] = x;
+  stop(kAtWave, 0);
+  bool r = false;
+  for (int l = 0; l < 64; ++l) r |= slots[t][(me & ~63) + l] != 0;
   return r;
 }
 inline void enter() {

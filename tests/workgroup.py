@@ -19,6 +19,7 @@ void set_error(const char* fmt, ...) {}
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 inline float fast_exp2(float x) { return exp2f(x); }
+template <int J> inline uint32_t xor_lane32(uint32_t v, int lane) { return wg::from_lane(v, lane ^ J); }
 template <int J> inline uint64_t xor_lane64(uint64_t v, int lane) { return wg::from_lane(v, lane ^ J); }
 }  // namespace tsa
 """

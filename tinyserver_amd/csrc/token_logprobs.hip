@@ -4,9 +4,11 @@
 // For a row x of V logits with m = max x, t_i = x_i - m <= 0, S = sum exp(t_i) and
 // E = sum exp(t_i) t_i:
 //   log p_i = t_i - ln S,   H = -sum p_i ln p_i = ln S - E / S
-// (both terms of H are non-negative: nothing cancels). A logit of -inf has p = 0 and
-// adds nothing; a NaN, a +inf or a row of nothing but -inf makes S NaN, and with it
-// the row's results.
+// (both terms of H are non-negative: nothing cancels). The sums are taken relative to the
+// largest logit that the wave has met, and end relative to m itself: S is at least 1 and
+// E at most 0 however they round, so no log p is above 0 and no H below. A logit of -inf
+// has p = 0 and adds nothing; a NaN, a +inf or a row of nothing but -inf makes S NaN,
+// and with it the row's results.
 //
 // One read of the logits; what bounds it: HBM for many rows (a large copy's rate), and
 // for a few the chain load -> sums -> threshold -> candidates -> rank. The vector
@@ -143,10 +145,9 @@ __device__ __forceinline__ void write_top(Candidates& c, int k, F write) {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kNoMax = -3.402823466e38f;  // the reference of no logit
-constexpr float kMove = 16.f;               // a logit may pass the reference by so much
 
-// Sums over logits x, relative to a reference m that is within kMove below the
-// largest: s = sum 2^y, e = sum 2^y y, y = (x - m) log2 e.
+// Sums over logits x, relative to the largest of them, m: s = sum 2^y, e = sum 2^y y, y
+// = (x - m) log2 e.
 struct Sums {
   float m, s, e;
   __device__ __forceinline__ void move(float to) {
@@ -192,6 +193,19 @@ __device__ __forceinline__ Sums block_sums(Sums v, Sums* waves) {
 #pragma unroll
   for (int w = 1; w < kThreads / 64; ++w) v.join(waves[w]);
   return v;
+}
+
+// The largest of the wave's numbers.
+__device__ __forceinline__ float wave_max(float x) {
+  const int lane = threadIdx.x & 63;
+  auto step = [&](auto J) { x = fmaxf(x, __uint_as_float(xor_lane32<decltype(J)::value>(__float_as_uint(x), lane))); };
+  step(std::integral_constant<int, 1>{});
+  step(std::integral_constant<int, 2>{});
+  step(std::integral_constant<int, 4>{});
+  step(std::integral_constant<int, 8>{});
+  step(std::integral_constant<int, 16>{});
+  step(std::integral_constant<int, 32>{});
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
 }
 
 // 16 bytes of logits.
@@ -254,8 +268,11 @@ struct Row {
     }
   }
   // Sums over tiles t .. end - 1; the thread's largest of them. A piece is summed by
-  // itself, then a tile, then all: with one float32 sum over a thread's logits (600 at a
-  // vocabulary of 151936) entropies of 7.5 were off by up to 2.6e-5, by this 2.4e-6.
+  // itself, then a tile, then all. All lanes of a wave have one reference, which moves
+  // at a new largest logit, a few times a row. (4,096 rows of 151,936: log probabilities
+  // and entropies off by at most 1.2e-6 and 1.5e-6; with one float32 sum over a thread's
+  // 600 logits 6.2e-6 and 5.8e-6; with references of the lanes' own that a logit may pass
+  // by 16, whose offsets then cancel, 2.5e-6 and 7.9e-6, and 231 us, not 217.)
   __device__ __forceinline__ float sum(Sums& v, int t, int end) const {
     float gm = -INFINITY;
     for (; t < end; ++t) {
@@ -268,7 +285,7 @@ struct Row {
         float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < VE; i += 2) mx = fmaxf(fmaxf(mx, PT::at(w[u], i)), PT::at(w[u], i + 1));
-        if (mx > tile.m + kMove) tile.move(mx);
+        if (__any(mx > tile.m)) tile.move(wave_max(mx));
         gm = fmaxf(gm, mx);
         Sums piece{tile.m, 0.f, 0.f};
 #pragma unroll
@@ -286,7 +303,7 @@ struct Row {
     const int e = edge();
     if (e < 0) return;
     const float xe = to_float(x[e]);
-    if (xe > v.m + kMove) v.move(xe);
+    if (xe > v.m) v.move(xe);
     v.add(xe);
   }
 };
