@@ -86,7 +86,8 @@ __global__ __launch_bounds__(kStepThreads) void step_tables_kernel(StepArgs a) {
         row = a.rows ? a.rows[s * a.rows_s] : s;
         if (row >= a.R) row = -1;
       }
-      const uint32_t cc = c > 0 ? min(c, 1 << 30) : 0, nn = n > 0 ? min(n, (1 << 30) - 1) : 0;
+      constexpr int kLongest = (1 << 30) - 1;
+      const uint32_t cc = c > 0 ? min(c, kLongest) : 0, nn = n > 0 ? min(n, kLongest) : 0;
       const uint32_t W = static_cast<uint32_t>(a.W);
       const uint32_t need = min((cc + nn + a.BS - 1) / a.BS, W);
       const uint32_t have = a.take ? min((cc + a.BS - 1) / a.BS, W) : need;
