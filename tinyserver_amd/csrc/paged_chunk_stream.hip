@@ -36,10 +36,18 @@ ChunkPlan chunk_plan(int64_t B, int64_t N, int64_t T, int64_t Hq, int64_t Hkv, i
   // Items of this call at most: row blocks of its tokens, one more a sequence.
   const int64_t items = Hkv * (rows / p.QB + B), blocks = (cap + 31) / 32;
   if (items >= (int64_t{1} << 38) / (blocks + kItemCost)) return p;  // (a run's blocks stay in 31 bits)
-  // Items of a few blocks are not cut: there is nothing to gain from a second launch (4
-  // sequences of 1-8 tokens over up to 512: 16.6 us, cut 11.9 and 4.0 apart). Else runs
-  // are as short as four blocks (over up to 1000: 17.6 us with eight, 15.6).
-  p.whole = blocks <= 16;
+  // Items of a few blocks are not cut, which saves the second launch and the partial
+  // results; few items of more blocks are, as there are workgroups left for their runs.
+  // (16/8 heads. f16: 4 sequences of one token under tables of 256 tokens 11.2 us whole
+  // and 13.9 cut, of 8 under 512 16.1 and 14.4; 16 of 8 under 512 17.1 and 19.8, under 768
+  // 21.3 and 22.4, under 1024 25.5 and 24.3. float32: 4 of one token under 256 17.0 and
+  // 16.3, under 512 24.6 and 17.0; 16 under 512 27.6 and 27.8, 4 of 64 28.3 and 32. Over
+  // 87 bf16 calls of each table of 12, 14 and 16 blocks, 1 to 192 items, these bounds lie 0.6,
+  // 0.9 and 0.6% above the better side on average; float32, 58 calls, 0.5, 0.1 and 0.5%.)
+  // Longer tables are always cut: their sequences may be of very different lengths. Runs
+  // are as short as four blocks (4 sequences of 1-8 tokens over up to 1000: 17.6 us with
+  // eight, 15.6).
+  p.whole = blocks <= (f32 ? 8 : 12) || (blocks <= 16 && items >= (f32 ? 112 : 64));
   p.min_run = p.whole ? 1 : 4;
   const int64_t most = p.whole ? items : (items * (blocks + kItemCost) + p.min_run - 1) / p.min_run;
   const int64_t P = chunk_runs(p.waves);
