@@ -28,14 +28,16 @@
 // one's exponentials run under the other's products.
 //
 // The chunk's own last blocks take their masks in the pipeline; blocks before them
-// need none, and those with a page that is not there leave it and follow one at a time.
-// Rows of V that no row sees repeat the last key's there. Where an item's sums are not
+// need none. From the first block with a page that is not there on, the blocks of a
+// table's 480 go one at a time, behind the pipeline. Rows of V that no row sees repeat the last key's there. Where an item's sums are not
 // finite, V of a key that some row does not see may be why (a weight of 0 times NaN):
 // the item goes again with every masked block one at a time, where V rows that are not
 // there become 0 and elements of V that are not finite reach the rows that see them
 // through a product of flags.
 // A weight goes to the second product rounded once to T, off by at most 2^-8 (f16:
 // 2^-11) of itself, as in the prefill kernels.
+//
+// At head_dim 128 the kernel holds 256 registers and spills 17; 190 and none at 64.
 #pragma once
 
 #include "nonfinite.h"

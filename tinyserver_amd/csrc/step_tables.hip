@@ -11,7 +11,7 @@
 // store). Every workgroup sums all lengths itself, kSeqs at a time, rather than wait
 // for another's sums, then takes its own run of tokens (a binary search over the
 // sums in LDS) and its own requests' table columns. Measured: 8 requests of one token
-// 4.7 us; 512 of 1-128 tokens (33,000 tokens, 512 x 512 columns) 7.0 with 256 tokens and
+// 4.8 us; 512 of 1-128 tokens (33,000 tokens, 512 x 512 columns) 6.9 with 256 tokens and
 // a request a workgroup, 12.4 with 1,024 and two.
 #include "tsa_common.h"
 
