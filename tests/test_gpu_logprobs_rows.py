@@ -1,6 +1,9 @@
 """Log probabilities of rows that the first tests do not have: a mask that allows about as
-many consecutive tokens as the list of candidates holds (1,024); the same rows again; and how near sure, flat
-and sparse rows come to 64 bits (the tolerance: logprobs_reference)."""
+many consecutive tokens as the list of candidates holds (1,024); the same rows again;
+and how near sure, flat and sparse rows come to 64 bits (the tolerance:
+logprobs_reference)."""
+
+import math
 
 import pytest
 import torch
@@ -53,3 +56,16 @@ def test_accuracy(kind, n, v, dtype):
 def test_accuracy_of_other_strides(kind):
     x, tokens = rows(kind, 40, 5003, F32, DEV)
     near(x, tokens, token_logprobs(x.t().contiguous().t(), tokens, 2), f"{kind}, columns first", side_by_side=False)
+
+
+def test_many_equal_weights():
+    """2^20 logits of weights that one float32 sum over a thread's 4,096 of them rounds down at nearly every addition
+    (it ends 6e-5 of itself too low): sums by piece, tile and row stay within a few of their roundings."""
+    v, rest = 1 << 20, 0.99 * 2.0**-13  # weights of (1 + rest) / 2, an ulp of 2^-13 from a sum of 1,024 on
+    x = torch.full((1, v), math.log1p(rest) - math.log(2.0), device=DEV)
+    x[:, :1024:256] = 0.0  # each wave's largest, in its first piece
+    tokens = torch.tensor([5], device=DEV)
+    whole = token_logprobs(x.expand(520, -1), tokens.expand(520), 2)
+    near(x, tokens, [a[:1] for a in whole], "whole rows")
+    assert all(torch.equal(a, a[:1].expand_as(a)) for a in whole)
+    near(x, tokens, token_logprobs(x, tokens, 2), "a row in parts")
